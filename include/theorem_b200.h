@@ -212,6 +212,85 @@ int thm_sp_prefix_fold(const float* M, const float* S, const float* x0, float* o
                        thm_stream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * gated_scan -- per-channel gated linear recurrence over time, channel-last, and
+ * its gradients. No reference counterpart: the per-channel sibling of
+ * chunk_fwd_h's state recurrence.
+ *
+ *   s = sigmoid(r_t), L = decay s, a_t = e^-L, p = sigmoid(i_t)
+ *   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) p x_t,   y_t = h_t
+ *
+ * x, r, i, dy [B,T,D] in `dtype`, unit stride over D, strides *_bs (batch) and
+ * *_ts (time) in elements; y, dx, dr, di [B,T,D] contiguous in `dtype`; decay
+ * [D] >= 0, h0, final_state, dfinal, dh0 [nseq,D] fp32 (h0, final_state, states,
+ * dfinal, dh0 may be NULL; final_state may be h0, dh0 may be dfinal). A token
+ * with r < -43 (-inf) holds the state and gets zero gradients, whatever x and i
+ * are there.
+ * cu_seqlens NULL: nseq = B sequences of T tokens. Otherwise B = 1 and sequence
+ * n is rows cu_seqlens[n] .. cu_seqlens[n+1] (int32, nseq + 1 device values;
+ * values outside [0, T] or out of order are clamped). zero_rest != 0: rows before
+ * cu_seqlens[0] and from cu_seqlens[nseq] on are set to 0, else left as they are.
+ * states fp32: the state entering each 64-token chunk, slot
+ * n * ceil(T / 64) + c, or cu_seqlens[n] / 64 + n + c when packed
+ * ([T / 64 + nseq, D]; unused slots are not written). The backward call reads
+ * the states that the forward call wrote. ddecay [D] is summed in a fixed order;
+ * workspace [nseq, D] fp32.
+ * ------------------------------------------------------------------------- */
+int thm_gated_scan_fwd(const void* x, const void* r, const void* i, const float* decay, const float* h0,
+                       const int* cu_seqlens, void* y, float* final_state, float* states, long long x_bs,
+                       long long x_ts, long long r_bs, long long r_ts, long long i_bs, long long i_ts, int B, int T,
+                       int D, int nseq, int zero_rest, int dtype, thm_stream_t stream);
+int thm_gated_scan_bwd(const void* x, const void* r, const void* i, const float* decay, const float* states,
+                       const void* dy, const float* dfinal, const int* cu_seqlens, void* dx, void* dr, void* di,
+                       float* ddecay, float* dh0, float* workspace, long long x_bs, long long x_ts, long long r_bs,
+                       long long r_ts, long long i_bs, long long i_ts, long long dy_bs, long long dy_ts, int B,
+                       int T, int D, int nseq, int zero_rest, int dtype, thm_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * group_norm -- norm over groups of G consecutive channels of each row,
+ * channel-last, with SiLU or a gate, and its gradients. No reference counterpart.
+ *
+ *   xh = (x - mean) rs with rs = 1 / sqrt(var + eps)   (center = 0: x rs, rs = 1 / sqrt(mean(x^2) + eps))
+ *   u = xh weight + bias;  y = act(u), or u act(gate) when gate != NULL
+ *
+ * x, gate, dy [R, C] in `dtype`, unit stride over C, row strides *_rs in
+ * elements; y, dx, dgate [R, C] contiguous; weight, bias [C] fp32 or NULL (1 and
+ * 0); dweight, dbias [C] fp32 or NULL, summed in a fixed order. C % G == 0,
+ * G <= 4096. workspace: [thm_group_norm_bwd_parts(R, C, G), 2, C] fp32, needed
+ * when dweight or dbias is given.
+ * ------------------------------------------------------------------------- */
+int thm_group_norm_fwd(const void* x, const void* gate, const float* weight, const float* bias, void* y,
+                       long long x_rs, long long gate_rs, long long R, int C, int G, int center, int activation,
+                       float eps, int dtype, thm_stream_t stream);
+int thm_group_norm_bwd(const void* x, const void* gate, const float* weight, const float* bias, const void* dy,
+                       void* dx, void* dgate, float* dweight, float* dbias, float* workspace, long long x_rs,
+                       long long gate_rs, long long dy_rs, long long R, int C, int G, int center, int activation,
+                       float eps, int dtype, thm_stream_t stream);
+int thm_group_norm_bwd_parts(long long R, int C, int G);
+
+/* ---------------------------------------------------------------------------
+ * causal_conv1d continued from a carried state, and its gradients (channel-last;
+ * kernels/causal_conv1d/kernel.py:170-230 is the forward pass from zeros).
+ *
+ * step: out[t] = act(bias + sum_k weight[:, k] z[t + k]), z = [state; x] with
+ *   state [B, W-1, D] the inputs before x [B, S, D]; state_out = the last W - 1
+ *   rows of z (may be state). Meant for S of one to some tens: a thread walks a
+ *   sequence's S tokens.
+ * bwd: dx [B,S,D], dweight [D,W], dbias [D] of thm_causal_conv1d_fwd
+ *   (THM_LAYOUT_BSD, l2norm_group 0); sums over tokens in a fixed order.
+ *   workspace [thm_causal_conv1d_bwd_parts(B, S, D), W + 1, D] fp32.
+ * x, dy in `dtype`, unit stride over D, strides *_bs, *_ts in elements; out, dx,
+ * states contiguous; weight, bias fp32; 1 <= W <= 8.
+ * ------------------------------------------------------------------------- */
+int thm_causal_conv1d_step(const void* x, const void* state, const float* weight, const float* bias, void* out,
+                           void* state_out, long long x_bs, long long x_ts, int B, int S, int D, int W, int dtype,
+                           int activation, thm_stream_t stream);
+int thm_causal_conv1d_bwd(const void* x, const float* weight, const float* bias, const void* dy, void* dx,
+                          float* dweight, float* dbias, float* workspace, long long x_bs, long long x_ts,
+                          long long dy_bs, long long dy_ts, int B, int S, int D, int W, int dtype, int activation,
+                          thm_stream_t stream);
+int thm_causal_conv1d_bwd_parts(int B, int S, int D);
+
+/* ---------------------------------------------------------------------------
  * Utilities
  * ------------------------------------------------------------------------- */
 /* Human-readable name of a thm_status. */

@@ -236,3 +236,138 @@ def gated_delta_chain(xq, xk, xv, wq, bq, wk, bk, wv, bv, beta, g, H, K, V,
         scale = K ** -0.5
     o = chunk_fwd_o(q, k, vnew, g, h, scale)
     return o, final
+
+
+# --------------------------------------------------------------------------
+# recurrent block: gated scan, group norm, conv step and gradients (extensions, no reference)
+# --------------------------------------------------------------------------
+def _sigmoid(x):
+    with np.errstate(over="ignore"):
+        return 1.0 / (1.0 + np.exp(-x))
+
+
+def scan_gates(x, r, i, decay):
+    """(s, L, a, p, m, x) of every token; a token with r < -43 or L = 0 holds the state (L = p = x = 0)."""
+    x, r, i, decay = map(_f64, (x, r, i, decay))
+    with np.errstate(invalid="ignore"):
+        s = _sigmoid(r)
+        L = np.where(r < -43.0, 0.0, decay * s)
+        held = L == 0.0
+        a = np.exp(-L)
+        p = np.where(held, 0.0, _sigmoid(i))
+        m = np.sqrt(-np.expm1(-2.0 * L))
+        return s, L, a, p, m, np.where(held, 0.0, x)
+
+
+def gated_scan(x, r, i, decay, h0=None):
+    """h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(i_t) x_t, a_t = exp(-decay sigmoid(r_t)).
+
+    x, r, i [B, T, D], decay [D], h0 [B, D]. Returns (y [B, T, D], final [B, D],
+    states [B, ceil(T / 64), D]: the state entering each 64-token chunk)."""
+    _, _, a, p, m, x = scan_gates(x, r, i, decay)
+    B, T, D = x.shape
+    h = np.zeros((B, D)) if h0 is None else _f64(h0).copy()
+    y = np.zeros((B, T, D))
+    states = np.zeros((B, (T + BT - 1) // BT, D))
+    for t in range(T):
+        if t % BT == 0:
+            states[:, t // BT] = h
+        h = a[:, t] * h + m[:, t] * p[:, t] * x[:, t]
+        y[:, t] = h
+    return y, h, states
+
+
+def gated_scan_bwd(x, r, i, decay, h0, dy, dfinal=None):
+    """Gradients of gated_scan: (dx, dr, di, ddecay, dh0). A held token's are zero."""
+    s, L, a, p, m, xv = scan_gates(x, r, i, decay)
+    B, T, D = xv.shape
+    y, _, _ = gated_scan(x, r, i, decay, h0)
+    first = np.zeros((B, 1, D)) if h0 is None else _f64(h0)[:, None]
+    prev = np.concatenate([first, y[:, :-1]], 1) if T else y
+    dy = _f64(dy)
+    carry = np.zeros((B, D)) if dfinal is None else _f64(dfinal).copy()
+    dh = np.zeros((B, T, D))
+    for t in range(T - 1, -1, -1):
+        dh[:, t] = dy[:, t] + carry
+        carry = a[:, t] * dh[:, t]
+    inv_m = np.where(L == 0.0, 0.0, 1.0 / np.where(L == 0.0, 1.0, m))
+    dL = dh * (a * a * inv_m * p * xv - a * prev)
+    dx = dh * m * p
+    di = dh * m * xv * p * (1.0 - p)
+    return dx, dL * L * (1.0 - s), di, (dL * s).sum((0, 1)), carry
+
+
+def group_norm(x, group, weight=None, bias=None, gate=None, activation=None, center=True, eps=1e-5):
+    """u = xh weight + bias over runs of ``group`` channels; act(u), or u act(gate)."""
+    x = _f64(x)
+    C = x.shape[-1]
+    g = x.reshape(x.shape[:-1] + (C // group, group))
+    if center:
+        g = g - g.mean(-1, keepdims=True)
+    u = (g / np.sqrt((g * g).mean(-1, keepdims=True) + eps)).reshape(x.shape)
+    if weight is not None:
+        u = u * _f64(weight)
+    if bias is not None:
+        u = u + _f64(bias)
+    if gate is not None:
+        z = _f64(gate)
+        return u * (silu(z) if activation == "silu" else z)
+    return silu(u) if activation == "silu" else u
+
+
+def silu_grad(x):
+    s = _sigmoid(x)
+    return s * (1.0 + x * (1.0 - s))
+
+
+def group_norm_bwd(x, dy, group, weight=None, bias=None, gate=None, activation=None, center=True, eps=1e-5):
+    """Gradients of group_norm: (dx, dgate or None, dweight or None, dbias or None)."""
+    x, dy = _f64(x), _f64(dy)
+    C = x.shape[-1]
+    shape3 = x.shape[:-1] + (C // group, group)
+    g = x.reshape(shape3)
+    if center:
+        g = g - g.mean(-1, keepdims=True)
+    rs = 1.0 / np.sqrt((g * g).mean(-1, keepdims=True) + eps)
+    xh3 = g * rs
+    xh = xh3.reshape(x.shape)
+    w = np.ones(C) if weight is None else _f64(weight)
+    u = xh * w + (0.0 if bias is None else _f64(bias))
+    silu_on = activation == "silu"
+    dgate = None
+    if gate is not None:
+        z = _f64(gate)
+        dgate = dy * u * (silu_grad(z) if silu_on else 1.0)
+        du = dy * (silu(z) if silu_on else z)
+    else:
+        du = dy * (silu_grad(u) if silu_on else 1.0)
+    axes = tuple(range(x.ndim - 1))
+    dxh = (du * w).reshape(shape3)
+    dx = dxh - xh3 * (dxh * xh3).mean(-1, keepdims=True)
+    if center:
+        dx = dx - dxh.mean(-1, keepdims=True)
+    return ((dx * rs).reshape(x.shape), dgate, None if weight is None else (du * xh).sum(axes),
+            None if bias is None else du.sum(axes))
+
+
+def causal_conv1d_step(x, state, weight, bias, activation=None):
+    """causal_conv1d ("bsd") continued from the W - 1 inputs before x: (out, new state)."""
+    z = np.concatenate([_f64(state), _f64(x)], 1)
+    W = _f64(weight).shape[1]
+    out = causal_conv1d(z, weight, bias, activation, "bsd")[:, W - 1:]
+    return out, z[:, z.shape[1] - (W - 1):]
+
+
+def causal_conv1d_bwd(x, weight, bias, dy, activation=None):
+    """Gradients of causal_conv1d ("bsd"): (dx, dweight [D, W], dbias [D])."""
+    x, w, dy = _f64(x), _f64(weight), _f64(dy)
+    B, S, D = x.shape
+    W = w.shape[1]
+    du = dy
+    if activation == "silu":
+        du = dy * silu_grad(causal_conv1d(x, w, bias, None, "bsd"))
+    xp = np.concatenate([np.zeros((B, W - 1, D)), x], 1)
+    dup = np.concatenate([du, np.zeros((B, W - 1, D))], 1)
+    dx = sum(w[:, k] * dup[:, W - 1 - k:W - 1 - k + S] for k in range(W))
+    dw = np.stack([(du * xp[:, k:k + S]).sum((0, 1)) for k in range(W)], 1)
+    return dx, dw, du.sum((0, 1))

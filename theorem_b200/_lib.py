@@ -28,6 +28,7 @@ THM_ACT_NONE, THM_ACT_SILU = 0, 1
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
+_Q = ctypes.c_longlong
 
 _SIGNATURES = {
     "thm_causal_conv1d_fwd": [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P],
@@ -40,6 +41,14 @@ _SIGNATURES = {
     "thm_chunk_local_cumsum_fwd": [_P, _P, _I, _I, _I, _F, _P],
     "thm_gated_delta_fwd_ho": [_P, _P, _P, _P, _P, _P, _P, _P, _F, _I, _I, _I, _I, _I, _I, _P],
     "thm_sp_prefix_fold": [_P, _P, _P, _P, _I, _I, _I, _I, _P],
+    "thm_gated_scan_fwd": [_P] * 9 + [_Q] * 6 + [_I] * 6 + [_P],
+    "thm_gated_scan_bwd": [_P] * 14 + [_Q] * 8 + [_I] * 6 + [_P],
+    "thm_group_norm_fwd": [_P] * 5 + [_Q] * 3 + [_I] * 4 + [_F, _I, _P],
+    "thm_group_norm_bwd": [_P] * 10 + [_Q] * 4 + [_I] * 4 + [_F, _I, _P],
+    "thm_group_norm_bwd_parts": [_Q, _I, _I],
+    "thm_causal_conv1d_step": [_P] * 6 + [_Q] * 2 + [_I] * 6 + [_P],
+    "thm_causal_conv1d_bwd": [_P] * 8 + [_Q] * 4 + [_I] * 6 + [_P],
+    "thm_causal_conv1d_bwd_parts": [_I, _I, _I],
     "thm_selftest_wait_timeout": [ctypes.c_longlong, _P, _P],
     "thm_status_string": [_I],
     "thm_get_device_status": [ctypes.POINTER(_I), _I],

@@ -1,0 +1,98 @@
+// rowops.cuh -- device helpers of the channel-last row kernels (gated scan, group
+// norm, conv step and backward): vectors of channels in and out of registers, and
+// the sigmoid / SiLU pair with its derivative.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "sm100.cuh"
+
+namespace thm {
+
+// VEC consecutive elements of T as one memory access of VEC * sizeof(T) bytes
+// (the caller guarantees that alignment), widened to or rounded from fp32.
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+  T v[VEC];
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T* p, float* f) {
+  const Pack<T, VEC> q = *reinterpret_cast<const Pack<T, VEC>*>(p);
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) f[j] = to_f32<T>(q.v[j]);
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(T* p, const float* f) {
+  Pack<T, VEC> q;
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) q.v[j] = from_f32<T>(f[j]);
+  *reinterpret_cast<Pack<T, VEC>*>(p) = q;
+}
+
+// e^x: the hardware exponential where the result is rounded to 16 bits (its error
+// grows as |x| 2^-24), expf where fp32 leaves the kernel.
+template <typename T>
+__device__ __forceinline__ float exp_for(float x) {
+  if constexpr (sizeof(T) == 2)
+    return __expf(x);
+  else
+    return expf(x);
+}
+
+// 1 / (1 + e^-x): 0 at -inf, 1 at +inf, NaN for NaN.
+template <typename T>
+__device__ __forceinline__ float sigmoid(float x) {
+  const float d = 1.f + exp_for<T>(-x);
+  if constexpr (sizeof(T) == 2)
+    return __fdividef(1.f, d);
+  else
+    return 1.f / d;
+}
+
+// silu(x) = x s and silu'(x) = s (1 + x (1 - s)), s = sigmoid(x).
+template <typename T>
+__device__ __forceinline__ float silu_of(float x) {
+  return x * sigmoid<T>(x);
+}
+template <typename T>
+__device__ __forceinline__ void silu_grad(float x, float& y, float& dy) {
+  const float s = sigmoid<T>(x);
+  y = x * s;
+  dy = s * (1.f + x * (1.f - s));
+}
+
+// out[map(c)] = sum over the n rows of part [n, M], column c: the second half of a
+// reduction over all tokens whose first half left one row per block. 8 threads share a
+// column (rows k, k + 8, ... each) and are added in a fixed order, so the result does not
+// depend on the order in which blocks ran.
+template <typename Map>
+__global__ void __launch_bounds__(256) sum_parts_kernel(const float* __restrict__ part, int n, int M, Map map) {
+  __shared__ float sh[8][33];
+  const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane;
+  float acc = 0.f;
+  if (c < M) {
+#pragma unroll 4
+    for (int j = k; j < n; j += 8) acc += part[(long long)j * M + c];
+  }
+  sh[k][lane] = acc;
+  __syncthreads();
+  if (k == 0 && c < M) {
+#pragma unroll
+    for (int j = 1; j < 8; ++j) acc += sh[j][lane];
+    map(c, acc);
+  }
+}
+
+template <typename Map>
+inline void sum_parts(const float* part, int n, int M, Map map, cudaStream_t st) {
+  sum_parts_kernel<<<(M + 31) / 32, 256, 0, st>>>(part, n, M, map);
+}
+
+}  // namespace thm

@@ -335,3 +335,264 @@ def chunk_local_cumsum(g_inc, scale: float = 1.0, out=None):
     L.check(L.load().thm_chunk_local_cumsum_fwd(L.ptr(g_inc), L.ptr(out), B, T, H, float(scale), st),
             "thm_chunk_local_cumsum_fwd")
     return out
+
+
+# ---------------------------------------------------------------------------
+# Recurrent block: gated scan, group norm, the conv's carried-state form and gradients
+# ---------------------------------------------------------------------------
+def _same(ref, **ts):
+    """Each given tensor has ref's shape, dtype and device."""
+    for name, t in ts.items():
+        if t is not None:
+            assert t.shape == ref.shape and t.dtype == ref.dtype and t.device == ref.device, \
+                f"{name} must be {tuple(ref.shape)} {ref.dtype} on {ref.device}"
+
+
+def _dense(ref, shape, dtype, **ts):
+    """Each given tensor is a contiguous ``shape`` of ``dtype`` on ref's device."""
+    for name, t in ts.items():
+        if t is not None:
+            assert t.shape == tuple(shape) and t.dtype == dtype and t.device == ref.device and t.is_contiguous(), \
+                f"{name} must be a contiguous {tuple(shape)} {dtype} on {ref.device}"
+
+
+def _unit_channels(**ts):
+    for name, t in ts.items():
+        if t is not None:
+            assert t.shape[-1] <= 1 or t.stride(-1) == 1, f"{name} must have unit stride over channels"
+
+
+def _float_in(x):
+    assert x.dtype in (torch.float32, torch.bfloat16), f"unsupported dtype {x.dtype} (float32 or bfloat16)"
+
+
+def _scan_args(x, r, i, decay, cu_seqlens):
+    _cuda(x, r, i, decay, cu_seqlens)
+    assert x.dim() == 3, "x must be [B, T, D]"
+    _float_in(x)
+    _same(x, r=r, i=i)
+    _unit_channels(x=x, r=r, i=i)
+    B, T, D = x.shape
+    _dense(x, (D,), torch.float32, decay=decay)
+    n = B
+    if cu_seqlens is not None:
+        assert B == 1, "packed sequences share one batch entry: x must be [1, T, D]"
+        assert cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 2, "cu_seqlens must hold N + 1 >= 2 row offsets"
+        n = cu_seqlens.numel() - 1
+        _dense(x, (n + 1,), torch.int32, cu_seqlens=cu_seqlens)
+    slots = T // BT + n if cu_seqlens is not None else (T + BT - 1) // BT
+    return B, T, D, n, (B, slots, D)
+
+
+@_on_input_device
+def gated_scan(x, r, i, decay, h0=None, cu_seqlens=None, want_states: bool = False, y=None, final=None):
+    """Per-channel gated linear recurrence over time (no reference counterpart: the
+    per-channel sibling of ``chunk_fwd_h``), channel-last:
+
+        a_t = exp(-decay sigmoid(r_t)),  h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(i_t) x_t
+
+    x, r, i [B, T, D] fp32 or bf16 of one dtype, unit stride over D, any strides over B and
+    T; decay [D] fp32 >= 0; h0 [N, D] fp32 (zeros if None). Any T: T = 1 with ``final=h0`` is
+    the in-place single-token step. A token with r < -43 (sigmoid(r) < 2^-62, -inf) holds the
+    state, whatever x and i hold there (pad a batch with it and ``final`` is each sequence's own).
+
+    ``cu_seqlens`` [N + 1] int32: N packed sequences, rows cu[n] .. cu[n+1] of a batch of one,
+    each from its h0; cu[0] may be > 0 and sequences may be empty (final = h0). Rows before the
+    first sequence and behind the last are 0 in a fresh y and left as they are in a given one.
+
+    Returns (y [B, T, D] in x's dtype, final [N, D] fp32, states). The state is carried in fp32.
+    ``want_states`` keeps the state entering each 64-token chunk for ``gated_scan_bwd``:
+    [B, ceil(T / 64), D] fp32; packed, sequence n's start at slot cu[n] // 64 + n of
+    [1, T // 64 + N, D] and unused slots are 0.
+    """
+    B, T, D, n, sshape = _scan_args(x, r, i, decay, cu_seqlens)
+    _dense(x, (n, D), torch.float32, h0=h0, final=final)
+    _dense(x, x.shape, x.dtype, y=y)
+    fresh = y is None
+    if fresh:
+        y = torch.empty(B, T, D, device=x.device, dtype=x.dtype)
+    if final is None:
+        final = torch.empty(n, D, device=x.device, dtype=torch.float32)
+    states = None
+    if want_states:
+        make = torch.zeros if cu_seqlens is not None else torch.empty
+        states = make(sshape, device=x.device, dtype=torch.float32)
+    L.check(L.load().thm_gated_scan_fwd(L.ptr(x), L.ptr(r), L.ptr(i), L.ptr(decay), L.ptr(h0), L.ptr(cu_seqlens),
+                                        L.ptr(y), L.ptr(final), L.ptr(states), x.stride(0), x.stride(1), r.stride(0),
+                                        r.stride(1), i.stride(0), i.stride(1), B, T, D, n, int(fresh),
+                                        L.dtype_code(x), L.stream_of(x)), "thm_gated_scan_fwd")
+    return y, final, states
+
+
+@_on_input_device
+def gated_scan_bwd(x, r, i, decay, states, dy, dfinal=None, cu_seqlens=None, dx=None, dr=None, di=None):
+    """Gradients of ``gated_scan``: (dx, dr, di [B, T, D] in x's dtype, ddecay [D], dh0 [N, D] fp32).
+
+    ``states`` is what the forward pass returned for the same inputs with want_states; dy like
+    y (any strides over B and T), dfinal [N, D] fp32 the gradient of ``final`` (None: zeros).
+    Tokens that held the state (r < -43) get zero gradients. Rows that no sequence holds are
+    treated as in ``gated_scan``. Sums over tokens are in fp32 in a fixed order, so results
+    repeat bit for bit.
+    """
+    B, T, D, n, sshape = _scan_args(x, r, i, decay, cu_seqlens)
+    _cuda(states, dy, dfinal)
+    _same(x, dy=dy)
+    _unit_channels(dy=dy)
+    _dense(x, sshape, torch.float32, states=states)
+    _dense(x, (n, D), torch.float32, dfinal=dfinal)
+    _dense(x, x.shape, x.dtype, dx=dx, dr=dr, di=di)
+    given = [t is not None for t in (dx, dr, di)]
+    assert all(given) or not any(given), "dx, dr, di are given together or not at all"
+    if not given[0]:
+        dx, dr, di = (torch.empty(B, T, D, device=x.device, dtype=x.dtype) for _ in range(3))
+    ddecay = torch.empty(D, device=x.device, dtype=torch.float32)
+    dh0 = torch.empty(n, D, device=x.device, dtype=torch.float32)
+    work = torch.empty(n, D, device=x.device, dtype=torch.float32)
+    L.check(L.load().thm_gated_scan_bwd(L.ptr(x), L.ptr(r), L.ptr(i), L.ptr(decay), L.ptr(states), L.ptr(dy),
+                                        L.ptr(dfinal), L.ptr(cu_seqlens), L.ptr(dx), L.ptr(dr), L.ptr(di),
+                                        L.ptr(ddecay), L.ptr(dh0), L.ptr(work), x.stride(0), x.stride(1), r.stride(0),
+                                        r.stride(1), i.stride(0), i.stride(1), dy.stride(0), dy.stride(1), B, T, D, n,
+                                        int(not given[0]), L.dtype_code(x), L.stream_of(x)), "thm_gated_scan_bwd")
+    return dx, dr, di, ddecay, dh0
+
+
+def _rows(name, t):
+    """(rows, row stride) of a [..., C] tensor whose leading dimensions collapse to one."""
+    _unit_channels(**{name: t})
+    rows, stride = 1, None
+    for size, st in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size != 1:
+            assert stride is None or rows == 0 or st == stride * rows, f"{name}'s leading dimensions must collapse to rows"
+            stride = st if stride is None else stride
+        rows *= size
+    return rows, (t.shape[-1] if stride is None else stride)
+
+
+def _norm_args(x, group, weight, bias, gate, activation):
+    _cuda(x, weight, bias, gate)
+    assert x.dim() >= 1, "x must be [..., C]"
+    _float_in(x)
+    _same(x, gate=gate)
+    C = x.shape[-1]
+    assert group >= 1 and C % group == 0, f"C={C} is not a multiple of the group size {group}"
+    _dense(x, (C,), torch.float32, weight=weight, bias=bias)
+    assert activation in _ACT, f"unknown activation {activation!r}"
+    return C
+
+
+@_on_input_device
+def group_norm(x, group: int, weight=None, bias=None, gate=None, activation=None, center: bool = True,
+               eps: float = 1e-5, out=None):
+    """Norm over runs of ``group`` consecutive channels of each token, channel-last (no
+    reference counterpart; torch's group_norm on [tokens, C] with C / group groups):
+
+        u = xh weight + bias,  y = act(u),  or y = u act(gate) with a gate
+
+    xh = (x - mean) / sqrt(var + eps), or x / sqrt(mean(x^2) + eps) with ``center=False``
+    (RMS norm per head). x, gate [..., C] fp32 or bf16 of one dtype, unit stride over C, the
+    leading dimensions collapsible to rows (any row stride); weight, bias [C] fp32 or None;
+    activation None or "silu"; group <= 4096. Statistics in fp32, variance from centred
+    values. Returns y, contiguous, like x.
+    """
+    C = _norm_args(x, group, weight, bias, gate, activation)
+    R, xs = _rows("x", x)
+    zs = _rows("gate", gate)[1] if gate is not None else 0
+    _dense(x, x.shape, x.dtype, out=out)
+    if out is None:
+        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    L.check(L.load().thm_group_norm_fwd(L.ptr(x), L.ptr(gate), L.ptr(weight), L.ptr(bias), L.ptr(out), xs, zs, R, C,
+                                        int(group), int(bool(center)), _ACT[activation], float(eps), L.dtype_code(x),
+                                        L.stream_of(x)), "thm_group_norm_fwd")
+    return out
+
+
+@_on_input_device
+def group_norm_bwd(x, dy, group: int, weight=None, bias=None, gate=None, activation=None, center: bool = True,
+                   eps: float = 1e-5):
+    """Gradients of ``group_norm``: (dx, dgate, dweight, dbias), None for what was None.
+
+    Statistics are recomputed from x; dweight and dbias are fp32 sums over all tokens in a
+    fixed order, so results repeat bit for bit.
+    """
+    C = _norm_args(x, group, weight, bias, gate, activation)
+    _cuda(dy)
+    _same(x, dy=dy)
+    R, xs = _rows("x", x)
+    gs = _rows("dy", dy)[1]
+    zs = _rows("gate", gate)[1] if gate is not None else 0
+    dev = x.device
+    dx = torch.empty(x.shape, device=dev, dtype=x.dtype)
+    dgate = torch.empty(x.shape, device=dev, dtype=x.dtype) if gate is not None else None
+    dweight = torch.empty(C, device=dev, dtype=torch.float32) if weight is not None else None
+    dbias = torch.empty(C, device=dev, dtype=torch.float32) if bias is not None else None
+    work = None
+    if weight is not None or bias is not None:
+        work = torch.empty(L.load().thm_group_norm_bwd_parts(R, C, int(group)), 2, C, device=dev, dtype=torch.float32)
+    L.check(L.load().thm_group_norm_bwd(L.ptr(x), L.ptr(gate), L.ptr(weight), L.ptr(bias), L.ptr(dy), L.ptr(dx),
+                                        L.ptr(dgate), L.ptr(dweight), L.ptr(dbias), L.ptr(work), xs, zs, gs, R, C,
+                                        int(group), int(bool(center)), _ACT[activation], float(eps), L.dtype_code(x),
+                                        L.stream_of(x)), "thm_group_norm_bwd")
+    return dx, dgate, dweight, dbias
+
+
+def _conv_args(x, weight, bias, activation):
+    _cuda(x, weight, bias)
+    assert x.dim() == 3, "x must be [B, S, D]"
+    _float_in(x)
+    _unit_channels(x=x)
+    B, S, D = x.shape
+    assert weight.dim() == 2 and weight.shape[1] >= 1, "weight must be [D, W]"
+    W = weight.shape[1]
+    _dense(x, (D, W), torch.float32, weight=weight)
+    _dense(x, (D,), torch.float32, bias=bias)
+    assert activation in _ACT, f"unknown activation {activation!r}"
+    return B, S, D, W
+
+
+@_on_input_device
+def causal_conv1d_step(x, state, weight, bias, activation=None, out=None, state_out=None):
+    """``causal_conv1d(..., "bsd")`` continued from the inputs before x, for decoding:
+    x [B, S, D] (S <= 64: one token, a few drafted ones), state [B, W - 1, D] in x's dtype.
+
+    Returns (out [B, S, D], the state after x: the last W - 1 rows of [state; x]).
+    ``state_out`` may be ``state`` (in place). A zero state is a sequence's start; after a
+    prefill it is the last W - 1 rows of its input. x has unit stride over D, any strides over
+    B and S; W <= 8; weight, bias fp32 (kernels/causal_conv1d/kernel.py:170-230 from zeros).
+    """
+    B, S, D, W = _conv_args(x, weight, bias, activation)
+    assert S <= 64, f"S={S}: the carried-state form takes at most 64 tokens (causal_conv1d takes long runs)"
+    _cuda(state)
+    _dense(x, (B, W - 1, D), x.dtype, state=state, state_out=state_out)
+    _dense(x, x.shape, x.dtype, out=out)
+    if out is None:
+        out = torch.empty(B, S, D, device=x.device, dtype=x.dtype)
+    if state_out is None:
+        state_out = torch.empty_like(state)
+    L.check(L.load().thm_causal_conv1d_step(L.ptr(x), L.ptr(state), L.ptr(weight), L.ptr(bias), L.ptr(out),
+                                            L.ptr(state_out), x.stride(0), x.stride(1), B, S, D, W, L.dtype_code(x),
+                                            _ACT[activation], L.stream_of(x)), "thm_causal_conv1d_step")
+    return out, state_out
+
+
+@_on_input_device
+def causal_conv1d_bwd(x, weight, bias, dy, activation=None):
+    """Gradients of ``causal_conv1d(x, weight, bias, activation, "bsd")`` without the L2
+    norm: (dx [B, S, D] in x's dtype, dweight [D, W], dbias [D] fp32).
+
+    x, dy [B, S, D] fp32 or bf16 of one dtype, unit stride over D, any strides over B and S;
+    W <= 8. Sums over tokens are in fp32 in a fixed order, so results repeat bit for bit.
+    """
+    B, S, D, W = _conv_args(x, weight, bias, activation)
+    _cuda(dy)
+    _same(x, dy=dy)
+    _unit_channels(dy=dy)
+    dx = torch.empty(B, S, D, device=x.device, dtype=x.dtype)
+    dweight = torch.empty(D, W, device=x.device, dtype=torch.float32)
+    dbias = torch.empty(D, device=x.device, dtype=torch.float32)
+    parts = L.load().thm_causal_conv1d_bwd_parts(B, S, D)
+    work = torch.empty(max(parts, 0), W + 1, D, device=x.device, dtype=torch.float32)
+    L.check(L.load().thm_causal_conv1d_bwd(L.ptr(x), L.ptr(weight), L.ptr(bias), L.ptr(dy), L.ptr(dx), L.ptr(dweight),
+                                           L.ptr(dbias), L.ptr(work), x.stride(0), x.stride(1), dy.stride(0),
+                                           dy.stride(1), B, S, D, W, L.dtype_code(x), _ACT[activation],
+                                           L.stream_of(x)), "thm_causal_conv1d_bwd")
+    return dx, dweight, dbias
