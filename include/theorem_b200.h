@@ -233,7 +233,7 @@ int thm_sp_prefix_fold(const float* M, const float* S, const float* x0, float* o
  * n * ceil(T / 64) + c, or cu_seqlens[n] / 64 + n + c when packed
  * ([T / 64 + nseq, D]; unused slots are not written). The backward call reads
  * the states that the forward call wrote. ddecay [D] is summed in a fixed order;
- * workspace [nseq, D] fp32.
+ * workspace [thm_gated_scan_bwd_parts(T, D, nseq, cu_seqlens != NULL, dtype), D] fp32.
  * ------------------------------------------------------------------------- */
 int thm_gated_scan_fwd(const void* x, const void* r, const void* i, const float* decay, const float* h0,
                        const int* cu_seqlens, void* y, float* final_state, float* states, long long x_bs,
@@ -244,6 +244,7 @@ int thm_gated_scan_bwd(const void* x, const void* r, const void* i, const float*
                        float* ddecay, float* dh0, float* workspace, long long x_bs, long long x_ts, long long r_bs,
                        long long r_ts, long long i_bs, long long i_ts, long long dy_bs, long long dy_ts, int B,
                        int T, int D, int nseq, int zero_rest, int dtype, thm_stream_t stream);
+int thm_gated_scan_bwd_parts(int T, int D, int nseq, int packed, int dtype);
 
 /* ---------------------------------------------------------------------------
  * group_norm -- norm over groups of G consecutive channels of each row,

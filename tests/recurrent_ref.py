@@ -47,7 +47,7 @@ def p_floor(dtype):
     return 2.0 ** -62 if dtype == torch.bfloat16 else 0.0
 
 
-def scan_errors(x, r, i, decay, h0, dtype):
+def scan_errors(x, r, i, decay, h0, dtype, bwd=False):
     """Relative errors of a_t and of the injected term, and the bound E_t on |h_t's error|.
 
     L = decay s carries s's error and a rounding; a = e^-L turns L's relative error into L
@@ -60,10 +60,13 @@ def scan_errors(x, r, i, decay, h0, dtype):
     E_t = a_t E_{t-1} + da a_t |h|_{t-1} + db |b_t| + 2 u (...), |h| the recurrence of the
     magnitudes; twice that covers the products of errors. The bf16 kernels keep e^-i under 2^62, so
     p is off by an absolute 2^-62 below that (1e-12 of a rounding step of a state of size x).
+    The backward kernels keep t and take a as 1 + t, which adds an absolute u to a.
     """
     s, L, a, p, m, xv = orc.scan_gates(x, r, i, decay)
     dL = sigmoid_rel(r, dtype) + U
     da = dL * L + 2 * (2 + 1.173 * L) * U + U
+    if bwd:
+        da = da + U / np.maximum(a, 1e-37)
     db = (12 + 5 + 2) * U + dL + sigmoid_rel(i, dtype)
     b = np.abs(m * p * xv)
     flush = p_floor(dtype) * np.abs(m * xv)
@@ -83,7 +86,7 @@ def scan_bwd_bounds(x, r, i, decay, h0, dy, dfinal, dtype):
     """The oracle's gradients and their bounds. dh has the recurrence of magnitudes of h with dy in
     place of b; the rest is the product rule over the factors of each gradient, 1 - s and 1 - p
     being off by an absolute 8 u at most."""
-    e = scan_errors(x, r, i, decay, h0, dtype)
+    e = scan_errors(x, r, i, decay, h0, dtype, bwd=True)
     s, L, a, p, m, xv = (e[k] for k in ("s", "L", "a", "p", "m", "x"))
     ref = orc.gated_scan_bwd(x, r, i, decay, h0, dy, dfinal)
     B, T, D = s.shape

@@ -43,6 +43,7 @@ _SIGNATURES = {
     "thm_sp_prefix_fold": [_P, _P, _P, _P, _I, _I, _I, _I, _P],
     "thm_gated_scan_fwd": [_P] * 9 + [_Q] * 6 + [_I] * 6 + [_P],
     "thm_gated_scan_bwd": [_P] * 14 + [_Q] * 8 + [_I] * 6 + [_P],
+    "thm_gated_scan_bwd_parts": [_I] * 5,
     "thm_group_norm_fwd": [_P] * 5 + [_Q] * 3 + [_I] * 4 + [_F, _I, _P],
     "thm_group_norm_bwd": [_P] * 10 + [_Q] * 4 + [_I] * 4 + [_F, _I, _P],
     "thm_group_norm_bwd_parts": [_Q, _I, _I],

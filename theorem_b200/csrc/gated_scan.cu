@@ -18,6 +18,8 @@
 #include "host_util.h"
 #include "rowops.cuh"
 
+THM_DEFINE_STATUS(g_status_scan)
+
 namespace thm {
 namespace gscan {
 
@@ -63,70 +65,55 @@ __device__ __forceinline__ long long rest_row(const Args& p, long long t) {
 }
 
 // --------------------------------------------------------------------------- channel pairs
-// A lane works on two channels at a time (packed fp32x2 arithmetic): neighbours 2 l, 2 l + 1
-// read as one access where addresses and strides allow it (ADJ), else l and l + 32.
+// A lane works on two neighbouring channels at a time, in packed fp32x2 arithmetic.
 template <typename T>
 struct RawPair;
 template <>
 struct RawPair<__nv_bfloat16> {
   uint32_t v;
-  static constexpr uint32_t kHold = 0xff80ff80u;  // -inf, -inf
   __device__ __forceinline__ float2 get() const {
     return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
   }
-  __device__ __forceinline__ void hold() { v = kHold; }
-  __device__ __forceinline__ void zero() { v = 0u; }
+  static __device__ __forceinline__ RawPair of(float2 f) { return {pack_bf16x2(f.x, f.y)}; }
 };
 template <>
 struct RawPair<float> {
   float2 v;
   __device__ __forceinline__ float2 get() const { return v; }
-  __device__ __forceinline__ void hold() { v = make_float2(-INFINITY, -INFINITY); }
-  __device__ __forceinline__ void zero() { v = make_float2(0.f, 0.f); }
+  static __device__ __forceinline__ RawPair of(float2 f) { return {f}; }
 };
 
-template <typename T, bool ADJ>
-__device__ __forceinline__ void load_pair(RawPair<T>& q, const T* p, bool on1) {
-  if constexpr (ADJ) {
-    q.v = *reinterpret_cast<const decltype(q.v)*>(p);
-  } else if constexpr (sizeof(T) == 2) {
-    const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
-    q.v = u[0] | (on1 ? (uint32_t)u[32] << 16 : 0u);
-  } else {
-    q.v = make_float2(p[0], on1 ? p[32] : 0.f);
-  }
+// The pair at p as one access (PAIRED: addresses and strides allow it) or as two.
+template <typename T, bool PAIRED>
+__device__ __forceinline__ RawPair<T> load_pair(const T* p, bool two) {
+  if constexpr (PAIRED) return *reinterpret_cast<const RawPair<T>*>(p);
+  return RawPair<T>::of(make_float2(to_f32<T>(p[0]), two ? to_f32<T>(p[1]) : 0.f));
 }
-template <typename T, bool ADJ>
-__device__ __forceinline__ void store_pair(T* p, float2 f, bool on1) {
-  if constexpr (ADJ) {
-    if constexpr (sizeof(T) == 2)
-      *reinterpret_cast<uint32_t*>(p) = pack_bf16x2(f.x, f.y);
-    else
-      *reinterpret_cast<float2*>(p) = f;
+template <typename T, bool PAIRED>
+__device__ __forceinline__ void store_pair(T* p, float2 f, bool two) {
+  if constexpr (PAIRED) {
+    *reinterpret_cast<RawPair<T>*>(p) = RawPair<T>::of(f);
   } else {
     p[0] = from_f32<T>(f.x);
-    if (on1) p[32] = from_f32<T>(f.y);
+    if (two) p[1] = from_f32<T>(f.y);
   }
 }
 
-// A lane's channels: c0 (its first), whether it has one or two, and the second's offset.
-template <bool ADJ>
+// A lane's channels c, c + 1, and which of them there are.
 struct Lane {
-  int c0;
-  bool on0, on1;
-  static constexpr int kNext = ADJ ? 1 : 32;
+  int c;
+  bool on, two;
   __device__ __forceinline__ Lane(int base, int D) {
-    const int l = threadIdx.x & 31;
-    c0 = base + (ADJ ? 2 * l : l);
-    on0 = c0 < D;
-    on1 = c0 + kNext < D;
+    c = base + 2 * (threadIdx.x & 31);
+    on = c < D;
+    two = c + 1 < D;
   }
-  __device__ __forceinline__ float2 load(const float* p) const {  // p at c0
-    return make_float2(on0 ? p[0] : 0.f, on1 ? p[kNext] : 0.f);
+  __device__ __forceinline__ float2 load(const float* p) const {  // p at channel 0
+    return make_float2(on ? p[c] : 0.f, two ? p[c + 1] : 0.f);
   }
   __device__ __forceinline__ void store(float* p, float2 v) const {
-    if (on0) p[0] = v.x;
-    if (on1) p[kNext] = v.y;
+    if (on) p[c] = v.x;
+    if (two) p[c + 1] = v.y;
   }
 };
 
@@ -159,57 +146,63 @@ constexpr float kHoldBelow = -43.f;
 // e^-87 is the smallest decay of one token that stays a normal number.
 constexpr float kMaxDecay = 87.f;
 
-// s = sigmoid(r), p = sigmoid(i) of one channel. For bf16 inputs the two share a reciprocal,
-// 1 / ((1 + e^-r)(1 + e^-i)), with both exponentials kept under 2^62 so that the product stays
-// finite: the special-function unit is what this kernel would be bound by (16 lanes a clock
-// and SM), and this takes three of its operations instead of four.
-template <typename T>
-__device__ __forceinline__ void sigmoids(float r, float i, float& s, float& p) {
+// s = sigmoid(r), p = sigmoid(i). For bf16 inputs the two share a reciprocal,
+// 1 / ((1 + e^-r)(1 + e^-i)): three operations of the special-function unit, which runs at an
+// eighth of the FMA rate, instead of four. e^-i is kept under 2^62, so the product is finite
+// unless the token is held; there i (which may be NaN) is taken as 0 so that it does not reach
+// s, and p comes out as NaN unless FINITE asks for e^-r to be limited too.
+template <typename T, bool FINITE>
+__device__ __forceinline__ void sigmoids(float2 r, float2 i, float2& s, float2& p) {
+  i = make_float2(r.x < kHoldBelow ? 0.f : i.x, r.y < kHoldBelow ? 0.f : i.y);
   if constexpr (sizeof(T) == 2) {
-    constexpr float kNegLog2e = -1.4426950408889634f;
-    i = r < kHoldBelow ? 0.f : i;  // a held token's NaN must not reach s through the shared product
-    const float A = 1.f + ex2_approx(min_nan(r * kNegLog2e, 62.f));
-    const float B = 1.f + ex2_approx(min_nan(i * kNegLog2e, 62.f));
-    const float q = rcp_approx(A * B);
-    s = q * B;
-    p = q * A;
+    float2 nr = __fmul2_rn(r, f2(-1.4426950408889634f));
+    if constexpr (FINITE) nr = make_float2(min_nan(nr.x, 62.f), min_nan(nr.y, 62.f));
+    const float2 ni = __fmul2_rn(i, f2(-1.4426950408889634f));
+    const float2 A = __fadd2_rn(make_float2(ex2_approx(nr.x), ex2_approx(nr.y)), f2(1.f));
+    const float2 B =
+        __fadd2_rn(make_float2(ex2_approx(min_nan(ni.x, 62.f)), ex2_approx(min_nan(ni.y, 62.f))), f2(1.f));
+    const float2 d = __fmul2_rn(A, B);
+    const float2 q = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+    s = __fmul2_rn(q, B);
+    p = __fmul2_rn(q, A);
   } else {
-    s = 1.f / (1.f + expf(-r));
-    p = 1.f / (1.f + expf(-i));
+    s = make_float2(1.f / (1.f + expf(-r.x)), 1.f / (1.f + expf(-r.y)));
+    p = make_float2(1.f / (1.f + expf(-i.x)), 1.f / (1.f + expf(-i.y)));
   }
 }
 
-// a = e^-L and m^2 = 1 - a^2 for 0 <= L <= 87, both to fp32 accuracy and without the
-// special-function unit, whose exponential is off by up to 2^-22 always to the same side: in a
+// a = e^-L and t = a - 1 for 0 <= L <= 87, both to fp32 accuracy and without the
+// special-function unit, whose exponential is off by up to 2^-22, always to the same side: in a
 // product over a memory of hundreds of tokens that adds up. -L = k ln 2 + f; e^f - 1 is a
 // polynomial fitted by reweighted least squares over |f| <= ln 2 / 2 (largest relative error
-// 1.3e-8); t = a - 1 = 2^k (e^f - 1) + (2^k - 1) does not cancel, so neither does
-// m^2 = -t (2 + t).
-__device__ __forceinline__ void decay_pair(float2 L, float2& a, float2& m2) {
+// 1.3e-8); t = 2^k (e^f - 1) + (2^k - 1) does not cancel, and so neither does
+// m^2 = 1 - a^2 = -t (2 + t).
+__device__ __forceinline__ void decay_pair(float2 L, float2& a, float2& t) {
   constexpr float kMagic = 12582912.f;  // 1.5 2^23: adding it rounds to an integer in the low bits
   const float2 km = __ffma2_rn(L, f2(-1.4426950408889634f), f2(kMagic));
   const float2 k = __fadd2_rn(km, f2(-kMagic));
   const float2 scale = make_float2(__int_as_float((__float_as_int(km.x) << 23) + 0x3f800000),
                                    __int_as_float((__float_as_int(km.y) << 23) + 0x3f800000));
-  const float2 nL = __fmul2_rn(L, f2(-1.f));
-  const float2 f = __ffma2_rn(k, f2(-1.42860677e-6f), __ffma2_rn(k, f2(-0.693145752f), nL));
+  const float2 f = __ffma2_rn(k, f2(-1.42860677e-6f), __ffma2_rn(k, f2(-0.693145752f), make_float2(-L.x, -L.y)));
   float2 c = __ffma2_rn(f, f2(0.00138825101f), f2(0.00836658047f));
   c = __ffma2_rn(f, c, f2(0.0416672018f));
   c = __ffma2_rn(f, c, f2(0.166665432f));
   c = __ffma2_rn(f, c, f2(0.499999981f));
   const float2 q = __ffma2_rn(__fmul2_rn(f, f), c, f);
   a = __ffma2_rn(scale, q, scale);
-  const float2 t = __ffma2_rn(scale, q, __fadd2_rn(scale, f2(-1.f)));
-  m2 = __fmul2_rn(__fmul2_rn(t, f2(-1.f)), __fadd2_rn(t, f2(2.f)));
+  t = __ffma2_rn(scale, q, __fadd2_rn(scale, f2(-1.f)));
+}
+__device__ __forceinline__ float2 m2_of(float2 t) {
+  return __fmul2_rn(make_float2(-t.x, -t.y), __fadd2_rn(t, f2(2.f)));
 }
 
 // One token of two channels: h -> a h + b. `decay` is already limited to kMaxDecay.
 template <typename T>
 __device__ __forceinline__ void token_pair(float2 x, float2 r, float2 i, float2 decay, float2& a, float2& b) {
-  float2 s, p, m2;
-  sigmoids<T>(r.x, i.x, s.x, p.x);
-  sigmoids<T>(r.y, i.y, s.y, p.y);
-  decay_pair(__fmul2_rn(decay, s), a, m2);
+  float2 s, p, t;
+  sigmoids<T, false>(r, i, s, p);
+  decay_pair(__fmul2_rn(decay, s), a, t);
+  const float2 m2 = m2_of(t);
   const float2 m = make_float2(sqrt_approx(m2.x), sqrt_approx(m2.y));
   const float2 v = __fmul2_rn(__fmul2_rn(m, p), x);
   b = make_float2(r.x < kHoldBelow ? 0.f : v.x, r.y < kHoldBelow ? 0.f : v.y);
@@ -224,50 +217,56 @@ __device__ __forceinline__ float2 limit_decay(float2 d) {
 // is nothing to split along time and a launch is all the latency there is.
 constexpr int kDirectThreads = 64;
 
-template <typename T, bool ADJ>
+template <typename T, bool PAIRED>
 __global__ void __launch_bounds__(kDirectThreads) scan_direct(const Args p) {
-  const Lane<ADJ> ln(((blockIdx.x * kDirectThreads + threadIdx.x) >> 5) * 64, p.D);
+  const Lane ln(((blockIdx.x * kDirectThreads + threadIdx.x) >> 5) * 64, p.D);
   const int n = blockIdx.y;
-  if (!ln.on0) return;
-  const int c = ln.c0;
-  T* y = static_cast<T*>(p.y) + c;
+  if (!ln.on) return;
+  T* y = static_cast<T*>(p.y) + ln.c;
   if (n == p.nseq) {  // rows of no sequence
-    for (long long t = rest_row(p, 0); t < p.T; t = rest_row(p, t + 1)) store_pair<T, ADJ>(y + t * p.D, f2(0.f), ln.on1);
+    for (long long t = rest_row(p, 0); t < p.T; t = rest_row(p, t + 1))
+      store_pair<T, PAIRED>(y + t * p.D, f2(0.f), ln.two);
     return;
   }
   const Seq q = sequence(p, n);
-  const T* x = static_cast<const T*>(p.x) + q.batch * p.xb + q.lo * p.xt + c;
-  const T* r = static_cast<const T*>(p.r) + q.batch * p.rb + q.lo * p.rt + c;
-  const T* i = static_cast<const T*>(p.i) + q.batch * p.ib + q.lo * p.it + c;
+  const T* x = static_cast<const T*>(p.x) + q.batch * p.xb + q.lo * p.xt + ln.c;
+  const T* r = static_cast<const T*>(p.r) + q.batch * p.rb + q.lo * p.rt + ln.c;
+  const T* i = static_cast<const T*>(p.i) + q.batch * p.ib + q.lo * p.it + ln.c;
   y += (q.batch * p.T + q.lo) * p.D;
-  const float2 decay = limit_decay(ln.load(p.decay + c));
-  float2 h = p.h0 != nullptr ? ln.load(p.h0 + (long long)n * p.D + c) : f2(0.f);
+  const float2 decay = limit_decay(ln.load(p.decay));
+  float2 h = p.h0 != nullptr ? ln.load(p.h0 + (long long)n * p.D) : f2(0.f);
   for (int k = 0; k < q.len; ++k) {
-    if (p.states != nullptr && k % kChunk == 0) ln.store(p.states + (q.slot + k / kChunk) * p.D + c, h);
-    RawPair<T> xv, rv, iv;
-    load_pair<T, ADJ>(xv, x + k * p.xt, ln.on1);
-    load_pair<T, ADJ>(rv, r + k * p.rt, ln.on1);
-    load_pair<T, ADJ>(iv, i + k * p.it, ln.on1);
+    if (p.states != nullptr && k % kChunk == 0) ln.store(p.states + (q.slot + k / kChunk) * p.D, h);
     float2 a, b;
-    token_pair<T>(xv.get(), rv.get(), iv.get(), decay, a, b);
+    token_pair<T>(load_pair<T, PAIRED>(x + k * p.xt, ln.two).get(), load_pair<T, PAIRED>(r + k * p.rt, ln.two).get(),
+                  load_pair<T, PAIRED>(i + k * p.it, ln.two).get(), decay, a, b);
     h = __ffma2_rn(a, h, b);
-    store_pair<T, ADJ>(y + (long long)k * p.D, h, ln.on1);
+    store_pair<T, PAIRED>(y + (long long)k * p.D, h, ln.two);
   }
-  if (p.final_state != nullptr) ln.store(p.final_state + (long long)n * p.D + c, h);
+  if (p.final_state != nullptr) ln.store(p.final_state + (long long)n * p.D, h);
 }
 
-// --------------------------------------------------------------------------- forward, many tokens
-// A block takes 64 channels and tiles of 64 tokens (one chunk), 8 tokens a warp. A warp's lanes
-// scan their 8 tokens from zero and leave the run's map h -> A h + S in shared memory; after one
-// barrier every lane composes the maps before its own with the state that enters the tile, and
-// its tokens' states are local + (product of a) x (entering state). Loads of the next tile are
-// issued before the barrier.
+// --------------------------------------------------------------------------- tiles
+// A block takes 64 channels and tiles of 64 tokens (one chunk), 8 tokens a warp, two channels
+// a lane. A lane scans its 8 tokens from zero and leaves the run's map h -> A h + S in shared
+// memory; after one barrier every lane composes the maps before its own with the state that
+// enters the tile, and its tokens' states are local + (product of a) x (entering state).
+//
+// Tiles come by TMA, up to two ahead, and leave by TMA from the slots they came in: neither
+// loads nor stores cost the warps an address. A sequence's last, partial tile leaves by plain
+// stores, because the rows behind it may be another sequence's. Where addresses or strides are
+// no multiples of 16 bytes (TMA false), the lanes fill their own slots with plain loads.
 //
 // Where there are too few channels to fill the GPU, a cluster of up to 8 blocks shares a
 // sequence: block k takes tiles k, k + n, ... . The blocks exchange their tiles' maps through
 // distributed shared memory once a round, so the chain along time costs one cluster barrier for
-// n tiles and x, r, i are still read once.
-constexpr int kWarps = 8, kRows = 8;
+// n tiles, and x, r, i are still read once.
+constexpr int kWarps = 8, kRows = 8, kCols = 64;
+static_assert(kWarps * kRows == kChunk, "a tile is a chunk");
+
+struct Maps {  // in place of the pointers where TMA carries the tiles
+  CUtensorMap in[4], out[3];
+};
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -296,66 +295,135 @@ __device__ __forceinline__ float2 apply(float4 m, float2 h) {
   return __ffma2_rn(make_float2(m.x, m.y), h, make_float2(m.z, m.w));
 }
 
-template <typename T, bool ADJ>
-struct Tile {  // a lane's 8 tokens, as loaded
-  RawPair<T> x[kRows], r[kRows], i[kRows];
-  // Rows row0 .. row0 + 7 of a sequence of len rows; rows past its end hold the state.
-  __device__ __forceinline__ void load(const T* xp, const T* rp, const T* ip, const Args& p, int row0, int len,
-                                       const Lane<ADJ>& ln) {
-#pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      if (ln.on0 && row0 + k < len) {
-        load_pair<T, ADJ>(r[k], rp + (long long)(row0 + k) * p.rt, ln.on1);
-        load_pair<T, ADJ>(i[k], ip + (long long)(row0 + k) * p.it, ln.on1);
-        load_pair<T, ADJ>(x[k], xp + (long long)(row0 + k) * p.xt, ln.on1);
-      } else {
-        r[k].hold();
-        i[k].zero();
-        x[k].zero();
+// The ring of stages that a block's tiles pass through: NIN input tiles a stage.
+template <typename T, bool TMA, int NIN, int NSTAGE>
+struct Ring {
+  static constexpr int kTile = kChunk * kCols * (int)sizeof(T);
+  static constexpr int kStage = NIN * kTile;
+  static constexpr int kBytes = NSTAGE * kStage;
+  uint8_t* base;
+  uint64_t* full;
+  int asked;  // loads issued (thread 0)
+  bool ok;
+
+  __device__ __forceinline__ Ring(uint8_t* b, uint64_t* f) : base(b), full(f), asked(0), ok(true) {
+    if constexpr (TMA) {
+      if (threadIdx.x == 0) {
+        for (int k = 0; k < NSTAGE; ++k) mbar_init(&full[k], 1);
+        fence_mbar_init();
       }
+      __syncthreads();
     }
+  }
+  __device__ __forceinline__ uint8_t* slot(int j, int in) const { return base + (j % NSTAGE) * kStage + in * kTile; }
+  // Thread 0: ask for the tile of step j, rows from `row` of batch entry `batch`.
+  __device__ __forceinline__ void ask(const CUtensorMap* in, int j, int col, int row, int batch) {
+    uint64_t* bar = &full[j % NSTAGE];
+    mbar_arrive_expect_tx(bar, kStage);
+#pragma unroll
+    for (int k = 0; k < NIN; ++k) tma_load_3d(slot(j, k), &in[k], bar, col, row, batch);
+  }
+  // All threads: the tile of step j is there. After a wait that ran out no further one is
+  // entered: the kernel ends, and the device status says why.
+  __device__ __forceinline__ void wait(int j, unsigned* status) {
+    if (ok) ok = mbar_wait(&full[j % NSTAGE], (j / NSTAGE) & 1, status);
   }
 };
 
-template <typename T, bool ADJ>
-__global__ void __launch_bounds__(32 * kWarps) scan_tiles(const Args p) {
-  __shared__ float4 maps[2][kWarps][32];
-  __shared__ float4 tiles[2][8][32];  // the cluster's blocks
+template <typename T>
+__device__ __forceinline__ RawPair<T> get_pair(const uint8_t* tile, int k) {
+  return *reinterpret_cast<const RawPair<T>*>(tile + k * kCols * sizeof(T));
+}
+template <typename T>
+__device__ __forceinline__ void put_pair(uint8_t* tile, int k, float2 f) {
+  *reinterpret_cast<RawPair<T>*>(tile + k * kCols * sizeof(T)) = RawPair<T>::of(f);
+}
+
+template <typename T>
+constexpr int fwd_stages() {
+  return sizeof(T) == 2 ? 2 : 2;
+}
+template <typename T>
+constexpr int bwd_stages() {
+  return sizeof(T) == 2 ? 3 : 2;
+}
+
+// Resident blocks an SM: bounded by registers (bf16) or shared memory (fp32).
+template <typename T>
+constexpr int fwd_per_sm() {
+  return sizeof(T) == 2 ? 3 : 2;
+}
+template <typename T>
+constexpr int bwd_per_sm() {
+  return sizeof(T) == 2 ? 2 : 1;
+}
+
+template <typename T, bool TMA>
+__global__ void __launch_bounds__(32 * kWarps, fwd_per_sm<T>())
+    scan_tiles(const __grid_constant__ Args p, const __grid_constant__ Maps tm) {
+  extern __shared__ __align__(1024) uint8_t stages[];
+  __shared__ __align__(16) float4 maps[kWarps][32];
+  __shared__ __align__(16) float4 tiles[2][8][32];  // of the cluster's blocks
+  __shared__ __align__(8) uint64_t full[4];
+  constexpr int NS = fwd_stages<T>();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Lane<ADJ> ln(blockIdx.y * 64, p.D);
-  const int c = ln.c0, n = blockIdx.z;
   const int nblk = cluster_size(), rank = cluster_rank();
-  T* y = static_cast<T*>(p.y) + c;
-  if (n == p.nseq) {  // rows of no sequence, a row per warp of the cluster
+  const Lane ln(blockIdx.y * kCols, p.D);
+  const int n = blockIdx.z;
+  T* y = static_cast<T*>(p.y) + ln.c;
+  if (n == p.nseq) {  // rows of no sequence, in turn over the cluster's warps
     const int w = rank * kWarps + warp;
     for (long long t = rest_row(p, 0); t < p.T; t = rest_row(p, t + 1))
-      if (t % (nblk * kWarps) == w && ln.on0) store_pair<T, ADJ>(y + t * p.D, f2(0.f), ln.on1);
+      if (t % (nblk * kWarps) == w && ln.on) store_pair<T, false>(y + t * p.D, f2(0.f), ln.two);
     return;
   }
+  Ring<T, TMA, 3, NS> ring(stages, full);
+  if (nblk > 1) cluster_barrier();  // every block of the cluster runs before one writes to another
   const Seq q = sequence(p, n);
-  const T* x = static_cast<const T*>(p.x) + q.batch * p.xb + q.lo * p.xt + c;
-  const T* r = static_cast<const T*>(p.r) + q.batch * p.rb + q.lo * p.rt + c;
-  const T* i = static_cast<const T*>(p.i) + q.batch * p.ib + q.lo * p.it + c;
   y += (q.batch * p.T + q.lo) * p.D;
-  const float2 decay = limit_decay(ln.load(p.decay + c));
-  float2 carry = p.h0 != nullptr ? ln.load(p.h0 + (long long)n * p.D + c) : f2(0.f);
+  const float2 decay = limit_decay(ln.load(p.decay));
+  float2 carry = p.h0 != nullptr ? ln.load(p.h0 + (long long)n * p.D) : f2(0.f);
   const int ntiles = (q.len + kChunk - 1) / kChunk;
   const int rounds = (ntiles + nblk - 1) / nblk;
-  if (nblk > 1) cluster_barrier();  // every block of the cluster runs before one writes to another
-  Tile<T, ADJ> in;
-  in.load(x, r, i, p, rank * kChunk + warp * kRows, q.len, ln);
-  for (int round = 0; round < rounds; ++round) {
-    const int tile = round * nblk + rank, row0 = tile * kChunk + warp * kRows, par = round & 1;
+  auto ask = [&](int j) {
+    const int tile = j * nblk + rank;
+    if (tile < ntiles && ring.ok) ring.ask(tm.in, j, blockIdx.y * kCols, q.lo + tile * kChunk, (int)q.batch);
+  };
+  if (TMA && threadIdx.x == 0) {
+    ask(0);
+    ask(1);
+  }
+  const int own = (warp * kRows * kCols + 2 * lane) * (int)sizeof(T);
+  for (int j = 0; j < rounds; ++j) {
+    const int tile = j * nblk + rank, row0 = tile * kChunk + warp * kRows, par = j & 1;
+    uint8_t *xs = ring.slot(j, 0) + own, *rs = ring.slot(j, 1) + own, *is = ring.slot(j, 2) + own;
+    if constexpr (TMA) {
+      if (tile < ntiles) ring.wait(j, &g_status_scan);
+    } else if (ln.on) {
+      for (int k = 0; k < kRows && row0 + k < q.len; ++k) {
+        const long long t = q.lo + row0 + k;
+        put_pair<T>(xs, k, load_pair<T, false>(static_cast<const T*>(p.x) + q.batch * p.xb + t * p.xt + ln.c, ln.two).get());
+        put_pair<T>(rs, k, load_pair<T, false>(static_cast<const T*>(p.r) + q.batch * p.rb + t * p.rt + ln.c, ln.two).get());
+        put_pair<T>(is, k, load_pair<T, false>(static_cast<const T*>(p.i) + q.batch * p.ib + t * p.it + ln.c, ln.two).get());
+      }
+    }
+    if (row0 + kRows > q.len) {  // rows past the sequence's end hold the state
+      for (int k = 0; k < kRows; ++k)
+        if (row0 + k >= q.len) {
+          put_pair<T>(rs, k, f2(-INFINITY));
+          put_pair<T>(is, k, f2(0.f));
+          put_pair<T>(xs, k, f2(0.f));
+        }
+    }
     float2 A[kRows], S[kRows];
 #pragma unroll
     for (int k = 0; k < kRows; ++k) {
       float2 a, b;
-      token_pair<T>(in.x[k].get(), in.r[k].get(), in.i[k].get(), decay, a, b);
+      token_pair<T>(get_pair<T>(xs, k).get(), get_pair<T>(rs, k).get(), get_pair<T>(is, k).get(), decay, a, b);
       A[k] = k == 0 ? a : __fmul2_rn(a, A[k - 1]);
       S[k] = k == 0 ? b : __ffma2_rn(a, S[k - 1], b);
     }
-    in.load(x, r, i, p, row0 + nblk * kChunk, q.len, ln);
-    maps[par][warp][lane] = make_float4(A[kRows - 1].x, A[kRows - 1].y, S[kRows - 1].x, S[kRows - 1].y);
+    maps[warp][lane] = make_float4(A[kRows - 1].x, A[kRows - 1].y, S[kRows - 1].x, S[kRows - 1].y);
     __syncthreads();
     float2 h = carry;
     if (nblk > 1) {
@@ -363,7 +431,7 @@ __global__ void __launch_bounds__(32 * kWarps) scan_tiles(const Args p) {
         float2 ta = f2(1.f), ts = f2(0.f);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float4 m = maps[par][w][lane];
+          const float4 m = maps[w][lane];
           ta = __fmul2_rn(ta, make_float2(m.x, m.y));
           ts = apply(m, ts);
         }
@@ -375,89 +443,229 @@ __global__ void __launch_bounds__(32 * kWarps) scan_tiles(const Args p) {
         carry = apply(tiles[par][b][lane], carry);
       }
     }
-    if (p.states != nullptr && warp == 0 && tile < ntiles) ln.store(p.states + (q.slot + tile) * p.D + c, h);
+    if (p.states != nullptr && warp == 0 && tile < ntiles) ln.store(p.states + (q.slot + tile) * p.D, h);
     float2 hin = h;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       if (w == warp) hin = h;
-      h = apply(maps[par][w][lane], h);
+      h = apply(maps[w][lane], h);
     }
     if (nblk == 1) carry = h;
-    if (ln.on0) {
+    const bool whole = TMA && (tile + 1) * kChunk <= q.len;
+    if (whole) {
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) put_pair<T>(xs, k, __ffma2_rn(A[k], hin, S[k]));
+    } else if (ln.on) {
 #pragma unroll
       for (int k = 0; k < kRows; ++k)
-        if (row0 + k < q.len)
-          store_pair<T, ADJ>(y + (long long)(row0 + k) * p.D, __ffma2_rn(A[k], hin, S[k]), ln.on1);
+        if (row0 + k < q.len) store_pair<T, false>(y + (long long)(row0 + k) * p.D, __ffma2_rn(A[k], hin, S[k]), ln.two);
+    }
+    if constexpr (TMA) fence_proxy_async_smem();
+    __syncthreads();
+    if constexpr (TMA) {
+      if (threadIdx.x == 0) {
+        if (whole) tma_store_3d(&tm.out[0], ring.slot(j, 0), blockIdx.y * kCols, q.lo + tile * kChunk, (int)q.batch);
+        bulk_commit_group();
+        // Step j + 2 goes into the stage of step j + 2 - NS, whose tile must have left.
+        if constexpr (NS == 3)
+          bulk_wait_group_read1();
+        else
+          bulk_wait_group_read0();
+        if (j + 2 < rounds) ask(j + 2);
+      }
     }
   }
-  if (p.final_state != nullptr && rank == 0 && warp == 0) ln.store(p.final_state + (long long)n * p.D + c, carry);
+  if (TMA && threadIdx.x == 0) bulk_wait_group0();
+  if (p.final_state != nullptr && rank == 0 && warp == 0) ln.store(p.final_state + (long long)n * p.D, carry);
 }
 
-// One thread per channel, one token after another.
-struct Gate {
-  float s, L, a, p, m2;
-};
-template <typename T>
-__device__ __forceinline__ Gate gate(float r, float i, float decay) {
-  Gate g;
-  sigmoids<T>(r, i, g.s, g.p);
-  g.L = r < kHoldBelow ? 0.f : fminf(decay, kMaxDecay) * g.s;
-  float2 a, m2;
-  decay_pair(f2(g.L), a, m2);
-  g.a = a.x;
-  g.m2 = m2.x;
-  return g;
-}
-template <typename T>
-__global__ void __launch_bounds__(128) scan_bwd_direct(const Args p) {
-  const int c = blockIdx.x * 128 + threadIdx.x;
-  const int n = blockIdx.y;
-  if (c >= p.D) return;
-  T *dx = static_cast<T*>(p.dx), *dr = static_cast<T*>(p.dr), *di = static_cast<T*>(p.di);
+// --------------------------------------------------------------------------- backward
+// The same tiles from the back. A lane keeps s, p, t = a - 1 and the injected term of its 8
+// tokens; two maps a warp go through shared memory, the forward one (h, from the chunk's kept
+// state) and the backward one (G_t = a_t dh_t, from the tile behind), and the gradients leave
+// in the slots of x, r and i. Clusters exchange the backward maps only: every tile's entering
+// state is known.
+template <typename T, bool TMA>
+__global__ void __launch_bounds__(32 * kWarps, bwd_per_sm<T>())
+    scan_bwd_tiles(const __grid_constant__ Args p, const __grid_constant__ Maps tm) {
+  extern __shared__ __align__(1024) uint8_t stages[];
+  __shared__ __align__(16) float4 maps[kWarps][32];
+  __shared__ __align__(16) float2 back[kWarps][32];
+  __shared__ __align__(16) float4 tiles[2][8][32];
+  __shared__ __align__(8) uint64_t full[4];
+  constexpr int NS = bwd_stages<T>();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int nblk = cluster_size(), rank = cluster_rank();
+  const Lane ln(blockIdx.y * kCols, p.D);
+  const int n = blockIdx.z;
+  T *dx = static_cast<T*>(p.dx) + ln.c, *dr = static_cast<T*>(p.dr) + ln.c, *di = static_cast<T*>(p.di) + ln.c;
   if (n == p.nseq) {
+    const int w = rank * kWarps + warp;
     for (long long t = rest_row(p, 0); t < p.T; t = rest_row(p, t + 1))
-      dx[t * p.D + c] = dr[t * p.D + c] = di[t * p.D + c] = from_f32<T>(0.f);
+      if (t % (nblk * kWarps) == w && ln.on) {
+        store_pair<T, false>(dx + t * p.D, f2(0.f), ln.two);
+        store_pair<T, false>(dr + t * p.D, f2(0.f), ln.two);
+        store_pair<T, false>(di + t * p.D, f2(0.f), ln.two);
+      }
     return;
   }
+  Ring<T, TMA, 4, NS> ring(stages, full);
+  if (nblk > 1) cluster_barrier();
   const Seq q = sequence(p, n);
-  const T* x = static_cast<const T*>(p.x) + q.batch * p.xb + c;
-  const T* r = static_cast<const T*>(p.r) + q.batch * p.rb + c;
-  const T* i = static_cast<const T*>(p.i) + q.batch * p.ib + c;
-  const T* dy = static_cast<const T*>(p.dy) + q.batch * p.gb + c;
-  const long long o = q.batch * p.T * p.D + c;
-  const float decay = p.decay[c];
-  float dh = p.dfinal != nullptr ? p.dfinal[(long long)n * p.D + c] : 0.f;  // a_{t+1} dh_{t+1}
-  float ddecay = 0.f;
-  float prev[kChunk];
-  for (int ch = (q.len + kChunk - 1) / kChunk - 1; ch >= 0; --ch) {
-    const int rows = min(kChunk, q.len - ch * kChunk);
-    float h = p.states[(q.slot + ch) * p.D + c];
-    for (int k = 0; k < rows; ++k) {
-      const long long t = q.lo + ch * kChunk + k;
-      prev[k] = h;
-      const Gate g = gate<T>(to_f32<T>(r[t * p.rt]), to_f32<T>(i[t * p.it]), decay);
-      const float b = g.L != 0.f ? sqrtf(g.m2) * g.p * to_f32<T>(x[t * p.xt]) : 0.f;
-      h = fmaf(g.a, h, b);
+  const long long first = (q.batch * p.T + q.lo) * p.D;
+  const float2 decay = limit_decay(ln.load(p.decay));
+  float2 carry = p.dfinal != nullptr ? ln.load(p.dfinal + (long long)n * p.D) : f2(0.f);
+  float2 ddecay = f2(0.f);
+  const int ntiles = (q.len + kChunk - 1) / kChunk;
+  const int rounds = (ntiles + nblk - 1) / nblk;
+  auto ask = [&](int j) {
+    const int tile = ntiles - 1 - (j * nblk + rank);
+    if (tile >= 0 && ring.ok) ring.ask(tm.in, j, blockIdx.y * kCols, q.lo + tile * kChunk, (int)q.batch);
+  };
+  if (TMA && threadIdx.x == 0) {
+    ask(0);
+    ask(1);
+  }
+  const int own = (warp * kRows * kCols + 2 * lane) * (int)sizeof(T);
+  for (int j = 0; j < rounds; ++j) {
+    const int tile = ntiles - 1 - (j * nblk + rank), row0 = tile * kChunk + warp * kRows, par = j & 1;
+    uint8_t *xs = ring.slot(j, 0) + own, *rs = ring.slot(j, 1) + own, *is = ring.slot(j, 2) + own,
+            *gs = ring.slot(j, 3) + own;
+    const int have = tile < 0 ? 0 : min(max(q.len - row0, 0), kRows);  // rows of the lane's 8
+    float2 h = tile >= 0 ? ln.load(p.states + (q.slot + tile) * p.D) : f2(0.f);
+    if constexpr (TMA) {
+      if (tile >= 0) ring.wait(j, &g_status_scan);
+    } else if (ln.on) {
+      for (int k = 0; k < have; ++k) {
+        const long long t = q.lo + row0 + k;
+        put_pair<T>(xs, k, load_pair<T, false>(static_cast<const T*>(p.x) + q.batch * p.xb + t * p.xt + ln.c, ln.two).get());
+        put_pair<T>(rs, k, load_pair<T, false>(static_cast<const T*>(p.r) + q.batch * p.rb + t * p.rt + ln.c, ln.two).get());
+        put_pair<T>(is, k, load_pair<T, false>(static_cast<const T*>(p.i) + q.batch * p.ib + t * p.it + ln.c, ln.two).get());
+        put_pair<T>(gs, k, load_pair<T, false>(static_cast<const T*>(p.dy) + q.batch * p.gb + t * p.gt + ln.c, ln.two).get());
+      }
     }
-    for (int k = rows - 1; k >= 0; --k) {
-      const long long t = q.lo + ch * kChunk + k;
-      Gate g = gate<T>(to_f32<T>(r[t * p.rt]), to_f32<T>(i[t * p.it]), decay);
-      const bool held = g.L == 0.f;
-      const float xv = held ? 0.f : to_f32<T>(x[t * p.xt]);
-      const float pv = held ? 0.f : g.p;
-      const float im = held ? 0.f : rsqrtf(g.m2);
-      const float m = g.m2 * im;
-      dh += to_f32<T>(dy[t * p.gt]);
-      const float dLv = dh * fmaf(g.a * g.a * im, pv * xv, -g.a * prev[k]);
-      dx[o + t * p.D] = from_f32<T>(dh * m * pv);
-      di[o + t * p.D] = from_f32<T>(dh * m * xv * pv * (1.f - pv));
-      dr[o + t * p.D] = from_f32<T>(dLv * g.L * (1.f - g.s));
-      ddecay = fmaf(dLv, g.s, ddecay);
-      dh *= g.a;
+    for (int k = have; k < kRows; ++k) {
+      put_pair<T>(rs, k, f2(-INFINITY));
+      put_pair<T>(is, k, f2(0.f));
+      put_pair<T>(xs, k, f2(0.f));
+      put_pair<T>(gs, k, f2(0.f));
+    }
+    float2 t[kRows], hp[kRows], s[kRows], pi[kRows];
+    float2 A = f2(1.f), S = f2(0.f), P = f2(0.f);
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      const float2 r = get_pair<T>(rs, k).get();
+      float2 a;
+      sigmoids<T, true>(r, get_pair<T>(is, k).get(), s[k], pi[k]);
+      s[k] = make_float2(r.x < kHoldBelow ? 0.f : s[k].x, r.y < kHoldBelow ? 0.f : s[k].y);
+      decay_pair(__fmul2_rn(decay, s[k]), a, t[k]);
+      const float2 m2 = m2_of(t[k]), x = get_pair<T>(xs, k).get();
+      const float2 m = make_float2(sqrt_approx(m2.x), sqrt_approx(m2.y));
+      const float2 b = __fmul2_rn(__fmul2_rn(m, pi[k]), x);
+      hp[k] = make_float2(s[k].x == 0.f ? 0.f : b.x, s[k].y == 0.f ? 0.f : b.y);
+      A = __fmul2_rn(a, A);
+      S = __ffma2_rn(a, S, hp[k]);
+    }
+#pragma unroll
+    for (int k = kRows - 1; k >= 0; --k)
+      P = __fmul2_rn(__fadd2_rn(t[k], f2(1.f)), __fadd2_rn(P, get_pair<T>(gs, k).get()));
+    maps[warp][lane] = make_float4(A.x, A.y, S.x, S.y);
+    back[warp][lane] = P;
+    __syncthreads();
+    float2 G = carry;
+    if (nblk > 1) {
+      if (warp == 0) {
+        float2 ta = f2(1.f), tp = f2(0.f);
+#pragma unroll
+        for (int w = kWarps - 1; w >= 0; --w) {
+          const float4 m = maps[w][lane];
+          ta = __fmul2_rn(ta, make_float2(m.x, m.y));
+          tp = __ffma2_rn(make_float2(m.x, m.y), tp, back[w][lane]);
+        }
+        for (int b = 0; b < nblk; ++b) store_remote(&tiles[par][rank][lane], b, make_float4(ta.x, ta.y, tp.x, tp.y));
+      }
+      cluster_barrier();
+      for (int b = 0; b < nblk; ++b) {
+        if (b == rank) G = carry;
+        carry = apply(tiles[par][b][lane], carry);
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < kWarps - 1; ++w)
+      if (w < warp) h = apply(maps[w][lane], h);
+    float2 gin = G;
+#pragma unroll
+    for (int w = kWarps - 1; w >= 0; --w) {
+      if (w == warp) gin = G;
+      const float4 m = maps[w][lane];
+      G = __ffma2_rn(make_float2(m.x, m.y), G, back[w][lane]);
+    }
+    if (nblk == 1) carry = G;
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {  // the state before each token
+      const float2 b = hp[k];
+      hp[k] = h;
+      h = __ffma2_rn(__fadd2_rn(t[k], f2(1.f)), h, b);
+    }
+    const bool whole = TMA && tile >= 0 && (tile + 1) * kChunk <= q.len;
+#pragma unroll
+    for (int k = kRows - 1; k >= 0; --k) {
+      const float2 a = __fadd2_rn(t[k], f2(1.f)), m2 = m2_of(t[k]);
+      const float2 im = make_float2(m2.x > 0.f ? rsqrtf(m2.x) : 0.f, m2.y > 0.f ? rsqrtf(m2.y) : 0.f);
+      float2 x = get_pair<T>(xs, k).get();
+      x = make_float2(s[k].x == 0.f ? 0.f : x.x, s[k].y == 0.f ? 0.f : x.y);
+      const float2 dh = __fadd2_rn(get_pair<T>(gs, k).get(), gin);
+      gin = __fmul2_rn(a, dh);
+      const float2 gx = __fmul2_rn(dh, __fmul2_rn(__fmul2_rn(m2, im), pi[k]));  // dh m p
+      const float2 np = __fadd2_rn(f2(1.f), make_float2(-pi[k].x, -pi[k].y));
+      const float2 gi = __fmul2_rn(__fmul2_rn(gx, x), np);
+      // dL = a dh (a p x / m - h_{t-1})
+      const float2 u = __fmul2_rn(__fmul2_rn(__fmul2_rn(a, im), pi[k]), x);
+      const float2 dL = __fmul2_rn(gin, __fadd2_rn(u, make_float2(-hp[k].x, -hp[k].y)));
+      const float2 dLs = __fmul2_rn(dL, s[k]);
+      ddecay = __fadd2_rn(ddecay, dLs);
+      const float2 ns = __fadd2_rn(f2(1.f), make_float2(-s[k].x, -s[k].y));
+      const float2 gr = __fmul2_rn(__fmul2_rn(dLs, decay), ns);
+      if (whole) {
+        put_pair<T>(xs, k, gx);
+        put_pair<T>(rs, k, gr);
+        put_pair<T>(is, k, gi);
+      } else if (ln.on && k < have) {
+        const long long o = first + (long long)(row0 + k) * p.D;
+        store_pair<T, false>(dx + o, gx, ln.two);
+        store_pair<T, false>(dr + o, gr, ln.two);
+        store_pair<T, false>(di + o, gi, ln.two);
+      }
+    }
+    if constexpr (TMA) fence_proxy_async_smem();
+    __syncthreads();
+    if constexpr (TMA) {
+      if (threadIdx.x == 0) {
+        if (whole) {
+#pragma unroll
+          for (int k = 0; k < 3; ++k)
+            tma_store_3d(&tm.out[k], ring.slot(j, k), blockIdx.y * kCols, q.lo + tile * kChunk, (int)q.batch);
+        }
+        bulk_commit_group();
+        if constexpr (NS == 3)
+          bulk_wait_group_read1();
+        else
+          bulk_wait_group_read0();
+        if (j + 2 < rounds) ask(j + 2);
+      }
     }
   }
-  p.ddecay_part[(long long)n * p.D + c] = ddecay;
-  if (p.dh0 != nullptr) p.dh0[(long long)n * p.D + c] = dh;
+  if (TMA && threadIdx.x == 0) bulk_wait_group0();
+  // ddecay over the block's warps, in order.
+  back[warp][lane] = ddecay;
+  __syncthreads();
+  if (warp == 0) {
+    float2 d = f2(0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) d = __fadd2_rn(d, back[w][lane]);
+    ln.store(p.ddecay_part + ((long long)n * nblk + rank) * p.D, d);
+    if (p.dh0 != nullptr && rank == 0) ln.store(p.dh0 + (long long)n * p.D, carry);
+  }
 }
 
 struct StoreColumn {
@@ -465,63 +673,138 @@ struct StoreColumn {
   __device__ void operator()(int c, float v) const { out[c] = v; }
 };
 
-// Whether two neighbouring channels can be read as one access everywhere.
-bool pairs_fit(int elem, int D, std::initializer_list<const void*> ptrs, std::initializer_list<long long> strides) {
+// --------------------------------------------------------------------------- launches
+// Whether all of these are multiples of `unit` bytes.
+bool multiples(int unit, int elem, int D, std::initializer_list<const void*> ptrs,
+               std::initializer_list<long long> strides) {
   uintptr_t bits = (uintptr_t)D;
   for (long long s : strides) bits |= (uintptr_t)s;
   bits *= elem;
   for (const void* q : ptrs) bits |= reinterpret_cast<uintptr_t>(q);
-  return (bits & (2 * elem - 1)) == 0;
+  return (bits & (unit - 1)) == 0;
+}
+
+// A [B, T, D] tensor in 64 x 64 boxes. A dimension of one entry may have any stride.
+int encode(CUtensorMap* m, int dtype, const void* base, long long bs, long long ts, int B, int T, int D) {
+  const int elem = dtype == THM_BF16 ? 2 : 4;
+  const uint64_t dims[3] = {(uint64_t)D, (uint64_t)T, (uint64_t)B};
+  const uint64_t ts_b = (uint64_t)(T > 1 ? ts : (long long)(D * elem + 15) / 16 * 16 / elem) * elem;
+  const uint64_t bs_b = B > 1 ? (uint64_t)bs * elem : ts_b * (uint64_t)T;
+  const uint64_t strides[2] = {ts_b, bs_b};
+  const uint32_t box[3] = {(uint32_t)kCols, (uint32_t)kChunk, 1};
+  if (ts_b == 0 || bs_b == 0 || ts_b >= (1ull << 40) || bs_b >= (1ull << 40)) return THM_ERR_UNSUPPORTED;
+  return encode_tiled(m, dtype == THM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3,
+                      base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 // Up to this many tokens a lane's serial walk beats the tiles.
 constexpr int kDirectTokens = 16;
 
-// Blocks that share a sequence: doubled while the grid has fewer than four blocks an SM and a
-// block still has two tiles of an average sequence.
-int cluster_blocks(const Args& p) {
-  const long long base = (long long)p.nseq * ((p.D + 63) / 64);
-  const long long tiles = ((p.cu != nullptr ? (p.T + p.nseq - 1) / p.nseq : p.T) + kChunk - 1) / kChunk;
-  int n = 1;
-  while (n < 8 && base * n < 4ll * sm_count() && tiles >= 4 * n) n *= 2;
-  return n;
+// Blocks that share a sequence. All blocks of a launch take about the same time, so what counts
+// is how full the last of the rounds of resident blocks is; among equals the fewest, and never
+// more than an average sequence has pairs of tiles for.
+int cluster_blocks(int T, int D, int nseq, bool packed, int per_sm) {
+  const long long base = (long long)nseq * ((D + kCols - 1) / kCols);
+  const long long tiles = ((packed ? (T + nseq - 1) / nseq : T) + kChunk - 1) / kChunk;
+  const long long slots = (long long)sm_count() * per_sm;
+  int best = 1;
+  double best_fill = 0.;
+  for (int n = 1; n <= 8; n *= 2) {
+    if (n > 1 && tiles < 2 * n) break;
+    const long long blocks = base * n;
+    const double fill = (double)blocks / (double)((blocks + slots - 1) / slots * slots);
+    if (fill > best_fill * 1.05) {
+      best = n;
+      best_fill = fill;
+    }
+  }
+  return best;
 }
 
-template <typename T, bool ADJ>
-int launch_fwd(const Args& p, int seqs, cudaStream_t st) {
-  if (p.T <= kDirectTokens) {
-    const dim3 grid((p.D + 2 * kDirectThreads - 1) / (2 * kDirectThreads), seqs);
-    scan_direct<T, ADJ><<<grid, kDirectThreads, 0, st>>>(p);
-    return check_launch();
+int bwd_cluster(int T, int D, int nseq, bool packed, int dtype) {
+  return cluster_blocks(T, D, nseq, packed, dtype == THM_BF16 ? bwd_per_sm<__nv_bfloat16>() : bwd_per_sm<float>());
+}
+
+template <typename K>
+int launch_tiles(K kernel, const Args& p, const Maps& tm, int n, int seqs, int smem, cudaStream_t st) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+    cudaGetLastError();
+    return THM_ERR_CUDA;
   }
-  const int n = cluster_blocks(p);
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3(n, (p.D + 63) / 64, seqs);
+  cfg.gridDim = dim3(n, (p.D + kCols - 1) / kCols, seqs);
   cfg.blockDim = dim3(32 * kWarps);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = n;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, scan_tiles<T, ADJ>, p) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, kernel, p, tm) != cudaSuccess) {
     cudaGetLastError();
     return THM_ERR_CUDA;
   }
   return check_launch();
 }
 
+template <typename T>
+int run_fwd(const Args& p, int B, int seqs, int dtype, cudaStream_t st) {
+  constexpr int elem = sizeof(T);
+  const int per_sm = fwd_per_sm<T>();
+  if (p.T <= kDirectTokens) {
+    const dim3 grid((p.D + 2 * kDirectThreads - 1) / (2 * kDirectThreads), seqs);
+    if (multiples(2 * elem, elem, p.D, {p.x, p.r, p.i, p.y}, {p.xb, p.xt, p.rb, p.rt, p.ib, p.it}))
+      scan_direct<T, true><<<grid, kDirectThreads, 0, st>>>(p);
+    else
+      scan_direct<T, false><<<grid, kDirectThreads, 0, st>>>(p);
+    return check_launch();
+  }
+  const int n = cluster_blocks(p.T, p.D, p.nseq, p.cu != nullptr, per_sm);
+  Maps tm{};
+  const long long ys = p.D;
+  bool tma = multiples(16, elem, p.D, {p.x, p.r, p.i, p.y}, {B > 1 ? p.xb : 0, p.xt, B > 1 ? p.rb : 0, p.rt, B > 1 ? p.ib : 0, p.it});
+  tma = tma && encode(&tm.in[0], dtype, p.x, p.xb, p.xt, B, p.T, p.D) == THM_OK &&
+        encode(&tm.in[1], dtype, p.r, p.rb, p.rt, B, p.T, p.D) == THM_OK &&
+        encode(&tm.in[2], dtype, p.i, p.ib, p.it, B, p.T, p.D) == THM_OK &&
+        encode(&tm.out[0], dtype, p.y, ys * p.T, ys, B, p.T, p.D) == THM_OK;
+  const int smem = Ring<T, true, 3, fwd_stages<T>()>::kBytes;
+  return tma ? launch_tiles(scan_tiles<T, true>, p, tm, n, seqs, smem, st)
+             : launch_tiles(scan_tiles<T, false>, p, tm, n, seqs, smem, st);
+}
+
+template <typename T>
+int run_bwd(const Args& p, int B, int seqs, int dtype, int n, cudaStream_t st) {
+  constexpr int elem = sizeof(T);
+  Maps tm{};
+  const long long ys = p.D;
+  bool tma = multiples(16, elem, p.D, {p.x, p.r, p.i, p.dy, p.dx, p.dr, p.di},
+                       {B > 1 ? p.xb : 0, p.xt, B > 1 ? p.rb : 0, p.rt, B > 1 ? p.ib : 0, p.it, B > 1 ? p.gb : 0, p.gt});
+  tma = tma && p.T > 0 && encode(&tm.in[0], dtype, p.x, p.xb, p.xt, B, p.T, p.D) == THM_OK &&
+        encode(&tm.in[1], dtype, p.r, p.rb, p.rt, B, p.T, p.D) == THM_OK &&
+        encode(&tm.in[2], dtype, p.i, p.ib, p.it, B, p.T, p.D) == THM_OK &&
+        encode(&tm.in[3], dtype, p.dy, p.gb, p.gt, B, p.T, p.D) == THM_OK &&
+        encode(&tm.out[0], dtype, p.dx, ys * p.T, ys, B, p.T, p.D) == THM_OK &&
+        encode(&tm.out[1], dtype, p.dr, ys * p.T, ys, B, p.T, p.D) == THM_OK &&
+        encode(&tm.out[2], dtype, p.di, ys * p.T, ys, B, p.T, p.D) == THM_OK;
+  const int smem = Ring<T, true, 4, bwd_stages<T>()>::kBytes;
+  return tma ? launch_tiles(scan_bwd_tiles<T, true>, p, tm, n, seqs, smem, st)
+             : launch_tiles(scan_bwd_tiles<T, false>, p, tm, n, seqs, smem, st);
+}
+
 int check_sizes(int B, int T, int D, int nseq, const int* cu, int dtype) {
   if (B < 0 || T < 0 || D < 0 || nseq < 0) return THM_ERR_INVALID;
   if (dtype != THM_F32 && dtype != THM_BF16) return THM_ERR_INVALID;
   if (cu != nullptr ? B != 1 : nseq != B) return THM_ERR_INVALID;
-  if (nseq >= 65535) return THM_ERR_UNSUPPORTED;
+  if (nseq >= 65535 || (D + kCols - 1) / kCols > 65535) return THM_ERR_UNSUPPORTED;
   return THM_OK;
 }
 
 }  // namespace gscan
 }  // namespace thm
+
+THM_STATUS_READER(thm_internal_status_scan, g_status_scan)
 
 extern "C" int thm_gated_scan_fwd(const void* x, const void* r, const void* i, const float* decay, const float* h0,
                                   const int* cu_seqlens, void* y, float* final_state, float* states,
@@ -540,11 +823,14 @@ extern "C" int thm_gated_scan_fwd(const void* x, const void* r, const void* i, c
   p.T = T; p.D = D; p.nseq = nseq;
   const int seqs = nseq + (cu_seqlens != nullptr && zero_rest);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int elem = dtype == THM_BF16 ? 2 : 4;
-  const bool adj = gscan::pairs_fit(elem, D, {x, r, i, y}, {x_bs, x_ts, r_bs, r_ts, i_bs, i_ts});
-  if (dtype == THM_BF16)
-    return adj ? gscan::launch_fwd<__nv_bfloat16, true>(p, seqs, st) : gscan::launch_fwd<__nv_bfloat16, false>(p, seqs, st);
-  return adj ? gscan::launch_fwd<float, true>(p, seqs, st) : gscan::launch_fwd<float, false>(p, seqs, st);
+  return dtype == THM_BF16 ? gscan::run_fwd<__nv_bfloat16>(p, B, seqs, dtype, st)
+                           : gscan::run_fwd<float>(p, B, seqs, dtype, st);
+}
+
+extern "C" int thm_gated_scan_bwd_parts(int T, int D, int nseq, int packed, int dtype) {
+  using namespace thm;
+  if (T < 0 || D <= 0 || nseq <= 0) return 0;
+  return nseq * gscan::bwd_cluster(T, D, nseq, packed != 0, dtype);
 }
 
 extern "C" int thm_gated_scan_bwd(const void* x, const void* r, const void* i, const float* decay,
@@ -566,15 +852,15 @@ extern "C" int thm_gated_scan_bwd(const void* x, const void* r, const void* i, c
   p.xb = x_bs; p.xt = x_ts; p.rb = r_bs; p.rt = r_ts; p.ib = i_bs; p.it = i_ts; p.gb = dy_bs; p.gt = dy_ts;
   p.T = T; p.D = D; p.nseq = nseq;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  int parts = 0;
   if (nseq > 0) {
-    const dim3 grid((D + 127) / 128, nseq + (cu_seqlens != nullptr && zero_rest));
-    if (dtype == THM_BF16)
-      gscan::scan_bwd_direct<__nv_bfloat16><<<grid, 128, 0, st>>>(p);
-    else
-      gscan::scan_bwd_direct<float><<<grid, 128, 0, st>>>(p);
-    const int e = check_launch();
+    const int seqs = nseq + (cu_seqlens != nullptr && zero_rest);
+    const int n = gscan::bwd_cluster(T, D, nseq, cu_seqlens != nullptr, dtype);
+    parts = nseq * n;
+    const int e = dtype == THM_BF16 ? gscan::run_bwd<__nv_bfloat16>(p, B, seqs, dtype, n, st)
+                                    : gscan::run_bwd<float>(p, B, seqs, dtype, n, st);
     if (e != THM_OK) return e;
   }
-  sum_parts(workspace, nseq, D, gscan::StoreColumn{ddecay}, st);
+  sum_parts(workspace, parts, D, gscan::StoreColumn{ddecay}, st);
   return check_launch();
 }

@@ -447,7 +447,8 @@ def gated_scan_bwd(x, r, i, decay, states, dy, dfinal=None, cu_seqlens=None, dx=
         dx, dr, di = (torch.empty(B, T, D, device=x.device, dtype=x.dtype) for _ in range(3))
     ddecay = torch.empty(D, device=x.device, dtype=torch.float32)
     dh0 = torch.empty(n, D, device=x.device, dtype=torch.float32)
-    work = torch.empty(n, D, device=x.device, dtype=torch.float32)
+    parts = L.load().thm_gated_scan_bwd_parts(T, D, n, int(cu_seqlens is not None), L.dtype_code(x))
+    work = torch.empty(parts, D, device=x.device, dtype=torch.float32)
     L.check(L.load().thm_gated_scan_bwd(L.ptr(x), L.ptr(r), L.ptr(i), L.ptr(decay), L.ptr(states), L.ptr(dy),
                                         L.ptr(dfinal), L.ptr(cu_seqlens), L.ptr(dx), L.ptr(dr), L.ptr(di),
                                         L.ptr(ddecay), L.ptr(dh0), L.ptr(work), x.stride(0), x.stride(1), r.stride(0),
