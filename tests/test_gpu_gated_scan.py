@@ -62,6 +62,23 @@ def test_matches_oracle(B, T, D, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("T", [3, 300])
+def test_decays_past_the_plain_range(T, dtype):
+    """Decays over 1 and under 1e-6, in some warps' channels only and in all of one's."""
+    from theorem_b200 import ops
+    B, D = 2, 200
+    x, r, i, decay, h0, dy, df = _inputs(B, T, D, dtype, seed=T)
+    decay[:64] *= 20.0
+    decay[70] = 3.0
+    decay[130] = 1e-7
+    args = _d(x, r, i, decay)
+    out = ops.gated_scan(*args, h0=h0.to(DEV), want_states=True)
+    _check_fwd(x, r, i, decay, h0, out, dtype)
+    grads = ops.gated_scan_bwd(*args, out[2], dy.to(DEV), dfinal=df.to(DEV))
+    _check_bwd(x, r, i, decay, h0, dy, df, grads, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("T", [1, 100])
 def test_defaults_without_h0_and_dfinal(T, dtype):
     from theorem_b200 import ops

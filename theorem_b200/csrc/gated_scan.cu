@@ -134,6 +134,11 @@ __device__ __forceinline__ float sqrt_approx(float x) {
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+__device__ __forceinline__ float rsqrt_approx(float x) {
+  float r;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 __device__ __forceinline__ float min_nan(float a, float b) {  // NaN when either is
   float r;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -146,17 +151,23 @@ constexpr float kHoldBelow = -43.f;
 // e^-87 is the smallest decay of one token that stays a normal number.
 constexpr float kMaxDecay = 87.f;
 
+// A token of two channels is computed in one of two ways. PLAIN tokens have 1e-6 <= decay <= 1
+// on every channel of the warp and no held token among the warp's 8 (both checked once a tile,
+// which costs a bf16 minimum a row): no range reduction, no selects, a third fewer
+// instructions. Others take the general way.
+constexpr float kPlainDecayMin = 1e-6f, kPlainDecayMax = 1.f;
+
 // s = sigmoid(r), p = sigmoid(i). For bf16 inputs the two share a reciprocal,
 // 1 / ((1 + e^-r)(1 + e^-i)): three operations of the special-function unit, which runs at an
-// eighth of the FMA rate, instead of four. e^-i is kept under 2^62, so the product is finite
-// unless the token is held; there i (which may be NaN) is taken as 0 so that it does not reach
-// s, and p comes out as NaN unless FINITE asks for e^-r to be limited too.
-template <typename T, bool FINITE>
+// eighth of the FMA rate, instead of four. Both exponentials are kept under 2^62, so the product
+// is finite. A held token has s = 0, and its i (which may be NaN) is taken as 0 so that it does
+// not reach s.
+template <typename T, bool PLAIN>
 __device__ __forceinline__ void sigmoids(float2 r, float2 i, float2& s, float2& p) {
-  i = make_float2(r.x < kHoldBelow ? 0.f : i.x, r.y < kHoldBelow ? 0.f : i.y);
+  if constexpr (!PLAIN) i = make_float2(r.x < kHoldBelow ? 0.f : i.x, r.y < kHoldBelow ? 0.f : i.y);
   if constexpr (sizeof(T) == 2) {
     float2 nr = __fmul2_rn(r, f2(-1.4426950408889634f));
-    if constexpr (FINITE) nr = make_float2(min_nan(nr.x, 62.f), min_nan(nr.y, 62.f));
+    if constexpr (!PLAIN) nr = make_float2(min_nan(nr.x, 62.5f), min_nan(nr.y, 62.5f));
     const float2 ni = __fmul2_rn(i, f2(-1.4426950408889634f));
     const float2 A = __fadd2_rn(make_float2(ex2_approx(nr.x), ex2_approx(nr.y)), f2(1.f));
     const float2 B =
@@ -169,47 +180,85 @@ __device__ __forceinline__ void sigmoids(float2 r, float2 i, float2& s, float2& 
     s = make_float2(1.f / (1.f + expf(-r.x)), 1.f / (1.f + expf(-r.y)));
     p = make_float2(1.f / (1.f + expf(-i.x)), 1.f / (1.f + expf(-i.y)));
   }
+  if constexpr (!PLAIN) s = make_float2(r.x < kHoldBelow ? 0.f : s.x, r.y < kHoldBelow ? 0.f : s.y);
 }
 
-// a = e^-L and t = a - 1 for 0 <= L <= 87, both to fp32 accuracy and without the
-// special-function unit, whose exponential is off by up to 2^-22, always to the same side: in a
-// product over a memory of hundreds of tokens that adds up. -L = k ln 2 + f; e^f - 1 is a
-// polynomial fitted by reweighted least squares over |f| <= ln 2 / 2 (largest relative error
-// 1.3e-8); t = 2^k (e^f - 1) + (2^k - 1) does not cancel, and so neither does
-// m^2 = 1 - a^2 = -t (2 + t).
-__device__ __forceinline__ void decay_pair(float2 L, float2& a, float2& t) {
-  constexpr float kMagic = 12582912.f;  // 1.5 2^23: adding it rounds to an integer in the low bits
-  const float2 km = __ffma2_rn(L, f2(-1.4426950408889634f), f2(kMagic));
-  const float2 k = __fadd2_rn(km, f2(-kMagic));
-  const float2 scale = make_float2(__int_as_float((__float_as_int(km.x) << 23) + 0x3f800000),
-                                   __int_as_float((__float_as_int(km.y) << 23) + 0x3f800000));
-  const float2 f = __ffma2_rn(k, f2(-1.42860677e-6f), __ffma2_rn(k, f2(-0.693145752f), make_float2(-L.x, -L.y)));
-  float2 c = __ffma2_rn(f, f2(0.00138825101f), f2(0.00836658047f));
-  c = __ffma2_rn(f, c, f2(0.0416672018f));
-  c = __ffma2_rn(f, c, f2(0.166665432f));
-  c = __ffma2_rn(f, c, f2(0.499999981f));
-  const float2 q = __ffma2_rn(__fmul2_rn(f, f), c, f);
-  a = __ffma2_rn(scale, q, scale);
-  t = __ffma2_rn(scale, q, __fadd2_rn(scale, f2(-1.f)));
+// a = e^-L and t = a - 1 from nL = -L, 0 <= L <= 87 (PLAIN: 1), both to fp32 accuracy and
+// without the special-function unit, whose exponential is off by up to 2^-22, always to the same
+// side: in a product over a memory of hundreds of tokens that adds up. e^f - 1 is a polynomial
+// fitted by reweighted least squares, over -1 <= f <= 0 (largest relative error 2.7e-9) or, after
+// nL = k ln 2 + f, over |f| <= ln 2 / 2 (1.3e-8). t = 2^k (e^f - 1) + (2^k - 1) does not cancel,
+// and so neither does m^2 = 1 - a^2 = -t (2 + t).
+template <bool PLAIN>
+__device__ __forceinline__ void decay_pair(float2 nL, float2& a, float2& t) {
+  if constexpr (PLAIN) {
+    float2 c = __ffma2_rn(nL, f2(0.000129130927f), f2(0.00130112648f));
+    c = __ffma2_rn(nL, c, f2(0.00827620872f));
+    c = __ffma2_rn(nL, c, f2(0.0416474683f));
+    c = __ffma2_rn(nL, c, f2(0.166663656f));
+    c = __ffma2_rn(nL, c, f2(0.499999841f));
+    t = __ffma2_rn(__fmul2_rn(nL, nL), c, nL);
+    a = __fadd2_rn(t, f2(1.f));
+  } else {
+    constexpr float kMagic = 12582912.f;  // 1.5 2^23: adding it rounds to an integer in the low bits
+    const float2 km = __ffma2_rn(nL, f2(1.4426950408889634f), f2(kMagic));
+    const float2 k = __fadd2_rn(km, f2(-kMagic));
+    const float2 scale = make_float2(__int_as_float((__float_as_int(km.x) << 23) + 0x3f800000),
+                                     __int_as_float((__float_as_int(km.y) << 23) + 0x3f800000));
+    const float2 f = __ffma2_rn(k, f2(-1.42860677e-6f), __ffma2_rn(k, f2(-0.693145752f), nL));
+    float2 c = __ffma2_rn(f, f2(0.00138825101f), f2(0.00836658047f));
+    c = __ffma2_rn(f, c, f2(0.0416672018f));
+    c = __ffma2_rn(f, c, f2(0.166665432f));
+    c = __ffma2_rn(f, c, f2(0.499999981f));
+    const float2 q = __ffma2_rn(__fmul2_rn(f, f), c, f);
+    a = __ffma2_rn(scale, q, scale);
+    t = __ffma2_rn(scale, q, __fadd2_rn(scale, f2(-1.f)));
+  }
 }
-__device__ __forceinline__ float2 m2_of(float2 t) {
-  return __fmul2_rn(make_float2(-t.x, -t.y), __fadd2_rn(t, f2(2.f)));
-}
+__device__ __forceinline__ float2 m2_of(float2 t) { return __fmul2_rn(t, __ffma2_rn(t, f2(-1.f), f2(-2.f))); }
 
-// One token of two channels: h -> a h + b. `decay` is already limited to kMaxDecay.
-template <typename T>
-__device__ __forceinline__ void token_pair(float2 x, float2 r, float2 i, float2 decay, float2& a, float2& b) {
+// One token of two channels: h -> a h + b. `ndecay` is -decay, limited to kMaxDecay.
+template <typename T, bool PLAIN>
+__device__ __forceinline__ void token_pair(float2 x, float2 r, float2 i, float2 ndecay, float2& a, float2& b) {
   float2 s, p, t;
-  sigmoids<T, false>(r, i, s, p);
-  decay_pair(__fmul2_rn(decay, s), a, t);
+  sigmoids<T, PLAIN>(r, i, s, p);
+  decay_pair<PLAIN>(__fmul2_rn(ndecay, s), a, t);
   const float2 m2 = m2_of(t);
   const float2 m = make_float2(sqrt_approx(m2.x), sqrt_approx(m2.y));
-  const float2 v = __fmul2_rn(__fmul2_rn(m, p), x);
-  b = make_float2(r.x < kHoldBelow ? 0.f : v.x, r.y < kHoldBelow ? 0.f : v.y);
+  b = __fmul2_rn(__fmul2_rn(m, p), x);
+  if constexpr (!PLAIN) b = make_float2(s.x == 0.f ? 0.f : b.x, s.y == 0.f ? 0.f : b.y);
 }
 
-__device__ __forceinline__ float2 limit_decay(float2 d) {
-  return make_float2(min_nan(d.x, kMaxDecay), min_nan(d.y, kMaxDecay));
+// The smaller of two pairs, elementwise; a NaN gives way to the other.
+template <typename T>
+__device__ __forceinline__ RawPair<T> min_pair(RawPair<T> u, RawPair<T> v) {
+  if constexpr (sizeof(T) == 2) {
+    const __nv_bfloat162 m =
+        __hmin2(*reinterpret_cast<const __nv_bfloat162*>(&u.v), *reinterpret_cast<const __nv_bfloat162*>(&v.v));
+    return {*reinterpret_cast<const uint32_t*>(&m)};
+  } else {
+    return {make_float2(fminf(u.v.x, v.v.x), fminf(u.v.y, v.v.y))};
+  }
+}
+template <typename T>
+__device__ __forceinline__ RawPair<T> min_rows(const RawPair<T> (&r)[8]) {
+  return min_pair(min_pair(min_pair(r[0], r[1]), min_pair(r[2], r[3])),
+                  min_pair(min_pair(r[4], r[5]), min_pair(r[6], r[7])));
+}
+template <typename T>
+__device__ __forceinline__ bool any_held(RawPair<T> m) {
+  const float2 f = m.get();
+  return __any_sync(0xffffffffu, f.x < kHoldBelow || f.y < kHoldBelow);
+}
+
+// -decay of a lane's channels; channels that it does not have do not keep its warp from PLAIN.
+__device__ __forceinline__ float2 neg_decay(const Lane& ln, const float* decay) {
+  const float2 d = ln.load(decay);
+  return make_float2(ln.on ? -min_nan(d.x, kMaxDecay) : -1.f, ln.two ? -min_nan(d.y, kMaxDecay) : -1.f);
+}
+__device__ __forceinline__ bool plain_decays(float2 nd) {
+  return __all_sync(0xffffffffu, -nd.x >= kPlainDecayMin && -nd.x <= kPlainDecayMax && -nd.y >= kPlainDecayMin &&
+                                     -nd.y <= kPlainDecayMax);
 }
 
 // --------------------------------------------------------------------------- forward, few tokens
@@ -233,13 +282,14 @@ __global__ void __launch_bounds__(kDirectThreads) scan_direct(const Args p) {
   const T* r = static_cast<const T*>(p.r) + q.batch * p.rb + q.lo * p.rt + ln.c;
   const T* i = static_cast<const T*>(p.i) + q.batch * p.ib + q.lo * p.it + ln.c;
   y += (q.batch * p.T + q.lo) * p.D;
-  const float2 decay = limit_decay(ln.load(p.decay));
+  const float2 ndecay = neg_decay(ln, p.decay);
   float2 h = p.h0 != nullptr ? ln.load(p.h0 + (long long)n * p.D) : f2(0.f);
   for (int k = 0; k < q.len; ++k) {
     if (p.states != nullptr && k % kChunk == 0) ln.store(p.states + (q.slot + k / kChunk) * p.D, h);
     float2 a, b;
-    token_pair<T>(load_pair<T, PAIRED>(x + k * p.xt, ln.two).get(), load_pair<T, PAIRED>(r + k * p.rt, ln.two).get(),
-                  load_pair<T, PAIRED>(i + k * p.it, ln.two).get(), decay, a, b);
+    token_pair<T, false>(load_pair<T, PAIRED>(x + k * p.xt, ln.two).get(),
+                         load_pair<T, PAIRED>(r + k * p.rt, ln.two).get(),
+                         load_pair<T, PAIRED>(i + k * p.it, ln.two).get(), ndecay, a, b);
     h = __ffma2_rn(a, h, b);
     store_pair<T, PAIRED>(y + (long long)k * p.D, h, ln.two);
   }
@@ -252,20 +302,20 @@ __global__ void __launch_bounds__(kDirectThreads) scan_direct(const Args p) {
 // memory; after one barrier every lane composes the maps before its own with the state that
 // enters the tile, and its tokens' states are local + (product of a) x (entering state).
 //
-// Tiles come by TMA, up to two ahead, and leave by TMA from the slots they came in: neither
-// loads nor stores cost the warps an address. A sequence's last, partial tile leaves by plain
-// stores, because the rows behind it may be another sequence's. Where addresses or strides are
-// no multiples of 16 bytes (TMA false), the lanes fill their own slots with plain loads.
+// Tiles come by TMA, so loading costs the warps no addresses; the barrier that the maps need
+// also says that a tile has been read, and its stage is refilled there. Where addresses or
+// strides are no multiples of 16 bytes (TMA false), the lanes fill their own slots with plain
+// loads.
 //
 // Where there are too few channels to fill the GPU, a cluster of up to 8 blocks shares a
-// sequence: block k takes tiles k, k + n, ... . The blocks exchange their tiles' maps through
-// distributed shared memory once a round, so the chain along time costs one cluster barrier for
-// n tiles, and x, r, i are still read once.
+// sequence: block k takes tiles k, k + n, ... . Each round the blocks send their tiles' maps to
+// one another's shared memory, counted in by an mbarrier, so the chain along time costs one
+// such exchange for n tiles, and x, r, i are still read once.
 constexpr int kWarps = 8, kRows = 8, kCols = 64;
 static_assert(kWarps * kRows == kChunk, "a tile is a chunk");
 
-struct Maps {  // in place of the pointers where TMA carries the tiles
-  CUtensorMap in[4], out[3];
+struct Maps {  // of x, r, i, dy, where TMA carries the tiles
+  CUtensorMap in[4];
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -281,50 +331,88 @@ __device__ __forceinline__ uint32_t cluster_size() {
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// Store 16 bytes at the same shared-memory address in block `rank` of the cluster.
-__device__ __forceinline__ void store_remote(const void* local, uint32_t rank, float4 v) {
-  uint32_t addr;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(local)), "r"(rank));
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z),
-               "f"(v.w)
-               : "memory");
-}
 
 // The map (A, S) of two channels, h -> A h + S.
 __device__ __forceinline__ float2 apply(float4 m, float2 h) {
   return __ffma2_rn(make_float2(m.x, m.y), h, make_float2(m.z, m.w));
 }
 
+// What the blocks of a cluster tell each other about a round: a map each, double-buffered.
+// A block sends round j + 2 only after it has all of round j + 1, and each block sends round
+// j + 1 after a block barrier that follows its reads of round j: no map is overwritten unread.
+struct Exchange {
+  float4 (*slots)[8][32];
+  uint64_t* bar;
+  int nblk, rank;
+  bool ok;
+  __device__ __forceinline__ Exchange(float4 (*s)[8][32], uint64_t* b, int n, int r)
+      : slots(s), bar(b), nblk(n), rank(r), ok(true) {
+    if (nblk > 1) {
+      if (threadIdx.x == 0) {
+        mbar_init(&bar[0], 1);
+        mbar_init(&bar[1], 1);
+        fence_mbar_init();
+      }
+      cluster_barrier();  // every block of the cluster runs, its barriers set up, before one sends
+    }
+  }
+  // One warp: send this block's map of round j to every block.
+  __device__ __forceinline__ void send(int j, float4 m) {
+    const int lane = threadIdx.x & 31, par = j & 1;
+    if (lane == 0) mbar_arrive_expect_tx(&bar[par], nblk * 32 * (int)sizeof(float4));
+    const uint32_t slot = smem_u32(&slots[par][rank][lane]), b = smem_u32(&bar[par]);
+    for (int k = 0; k < nblk; ++k) {
+      uint32_t rs, rb;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(rs) : "r"(slot), "r"(k));
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(rb) : "r"(b), "r"(k));
+      asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(
+                       rs),
+                   "f"(m.x), "f"(m.y), "f"(m.z), "f"(m.w), "r"(rb)
+                   : "memory");
+    }
+  }
+  // All threads: the state that enters this block's tile of round j, and in `carry` the one
+  // that enters the next round.
+  __device__ __forceinline__ float2 receive(int j, float2& carry, unsigned* status) {
+    const int lane = threadIdx.x & 31, par = j & 1;
+    if (ok) ok = mbar_wait(&bar[par], (j >> 1) & 1, status);
+    float2 mine = carry;
+    for (int k = 0; k < nblk; ++k) {
+      if (k == rank) mine = carry;
+      carry = apply(slots[par][k][lane], carry);
+    }
+    return mine;
+  }
+};
+
 // The ring of stages that a block's tiles pass through: NIN input tiles a stage.
-template <typename T, bool TMA, int NIN, int NSTAGE>
+template <typename T, int NIN, int NSTAGE>
 struct Ring {
   static constexpr int kTile = kChunk * kCols * (int)sizeof(T);
   static constexpr int kStage = NIN * kTile;
   static constexpr int kBytes = NSTAGE * kStage;
   uint8_t* base;
   uint64_t* full;
-  int asked;  // loads issued (thread 0)
   bool ok;
 
-  __device__ __forceinline__ Ring(uint8_t* b, uint64_t* f) : base(b), full(f), asked(0), ok(true) {
-    if constexpr (TMA) {
-      if (threadIdx.x == 0) {
-        for (int k = 0; k < NSTAGE; ++k) mbar_init(&full[k], 1);
-        fence_mbar_init();
-      }
-      __syncthreads();
+  __device__ __forceinline__ Ring(uint8_t* b, uint64_t* f) : base(b), full(f), ok(true) {
+    if (threadIdx.x == 0) {
+      for (int k = 0; k < NSTAGE; ++k) mbar_init(&full[k], 1);
+      fence_mbar_init();
     }
+    __syncthreads();
   }
   __device__ __forceinline__ uint8_t* slot(int j, int in) const { return base + (j % NSTAGE) * kStage + in * kTile; }
-  // Thread 0: ask for the tile of step j, rows from `row` of batch entry `batch`.
+  // One thread: ask for the tiles of step j, rows from `row` of batch entry `batch`.
   __device__ __forceinline__ void ask(const CUtensorMap* in, int j, int col, int row, int batch) {
+    if (!ok) return;
     uint64_t* bar = &full[j % NSTAGE];
     mbar_arrive_expect_tx(bar, kStage);
 #pragma unroll
     for (int k = 0; k < NIN; ++k) tma_load_3d(slot(j, k), &in[k], bar, col, row, batch);
   }
-  // All threads: the tile of step j is there. After a wait that ran out no further one is
-  // entered: the kernel ends, and the device status says why.
+  // All threads: the tiles of step j are there. After a wait that ran out no further one is
+  // entered and nothing more is asked for: the kernel ends, and the device status says why.
   __device__ __forceinline__ void wait(int j, unsigned* status) {
     if (ok) ok = mbar_wait(&full[j % NSTAGE], (j / NSTAGE) & 1, status);
   }
@@ -338,35 +426,35 @@ template <typename T>
 __device__ __forceinline__ void put_pair(uint8_t* tile, int k, float2 f) {
   *reinterpret_cast<RawPair<T>*>(tile + k * kCols * sizeof(T)) = RawPair<T>::of(f);
 }
-
+// A lane's first `rows` rows of a tensor into its slots, without TMA.
 template <typename T>
-constexpr int fwd_stages() {
-  return sizeof(T) == 2 ? 2 : 2;
-}
-template <typename T>
-constexpr int bwd_stages() {
-  return sizeof(T) == 2 ? 3 : 2;
+__device__ __forceinline__ void fill(uint8_t* tile, const void* t, long long first, long long stride, int rows, bool two) {
+  const T* q = static_cast<const T*>(t) + first;
+  for (int k = 0; k < rows; ++k) put_pair<T>(tile, k, load_pair<T, false>(q + k * stride, two).get());
 }
 
-// Resident blocks an SM: bounded by registers (bf16) or shared memory (fp32).
+// Stages, and resident blocks an SM: three of 80 registers a thread forward and two of 128
+// backward for bf16; for fp32 shared memory holds fewer.
 template <typename T>
-constexpr int fwd_per_sm() {
-  return sizeof(T) == 2 ? 3 : 2;
-}
+struct Fwd {
+  static constexpr int kStages = 2, kPerSm = sizeof(T) == 2 ? 3 : 2;
+  using R = Ring<T, 3, kStages>;
+};
 template <typename T>
-constexpr int bwd_per_sm() {
-  return sizeof(T) == 2 ? 2 : 1;
-}
+struct Bwd {
+  static constexpr int kStages = sizeof(T) == 2 ? 2 : 1, kPerSm = 2;
+  using R = Ring<T, 4, kStages>;
+};
 
 template <typename T, bool TMA>
-__global__ void __launch_bounds__(32 * kWarps, fwd_per_sm<T>())
+__global__ void __launch_bounds__(32 * kWarps, Fwd<T>::kPerSm)
     scan_tiles(const __grid_constant__ Args p, const __grid_constant__ Maps tm) {
-  extern __shared__ __align__(1024) uint8_t stages[];
-  __shared__ __align__(16) float4 maps[kWarps][32];
-  __shared__ __align__(16) float4 tiles[2][8][32];  // of the cluster's blocks
-  __shared__ __align__(8) uint64_t full[4];
-  constexpr int NS = fwd_stages<T>();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  extern __shared__ __align__(128) uint8_t stages[];
+  __shared__ __align__(16) float4 maps[2][kWarps][32];
+  __shared__ __align__(16) float4 slots[2][8][32];
+  __shared__ __align__(8) uint64_t full[Fwd<T>::kStages], xbar[2];
+  constexpr int NS = Fwd<T>::kStages;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int nblk = cluster_size(), rank = cluster_rank();
   const Lane ln(blockIdx.y * kCols, p.D);
   const int n = blockIdx.z;
@@ -377,124 +465,117 @@ __global__ void __launch_bounds__(32 * kWarps, fwd_per_sm<T>())
       if (t % (nblk * kWarps) == w && ln.on) store_pair<T, false>(y + t * p.D, f2(0.f), ln.two);
     return;
   }
-  Ring<T, TMA, 3, NS> ring(stages, full);
-  if (nblk > 1) cluster_barrier();  // every block of the cluster runs before one writes to another
+  typename Fwd<T>::R ring(stages, full);
+  Exchange ex(slots, xbar, nblk, rank);
   const Seq q = sequence(p, n);
   y += (q.batch * p.T + q.lo) * p.D;
-  const float2 decay = limit_decay(ln.load(p.decay));
+  const float2 ndecay = neg_decay(ln, p.decay);
+  const bool plain = plain_decays(ndecay);
   float2 carry = p.h0 != nullptr ? ln.load(p.h0 + (long long)n * p.D) : f2(0.f);
   const int ntiles = (q.len + kChunk - 1) / kChunk;
   const int rounds = (ntiles + nblk - 1) / nblk;
   auto ask = [&](int j) {
     const int tile = j * nblk + rank;
-    if (tile < ntiles && ring.ok) ring.ask(tm.in, j, blockIdx.y * kCols, q.lo + tile * kChunk, (int)q.batch);
+    if (tile < ntiles) ring.ask(tm.in, j, blockIdx.y * kCols, q.lo + tile * kChunk, (int)q.batch);
   };
-  if (TMA && threadIdx.x == 0) {
-    ask(0);
-    ask(1);
-  }
+  if (TMA && threadIdx.x == 0)
+    for (int j = 0; j < NS; ++j) ask(j);
   const int own = (warp * kRows * kCols + 2 * lane) * (int)sizeof(T);
   for (int j = 0; j < rounds; ++j) {
     const int tile = j * nblk + rank, row0 = tile * kChunk + warp * kRows, par = j & 1;
+    const int have = min(max(q.len - row0, 0), kRows);  // rows of the lane's 8 that there are
     uint8_t *xs = ring.slot(j, 0) + own, *rs = ring.slot(j, 1) + own, *is = ring.slot(j, 2) + own;
     if constexpr (TMA) {
       if (tile < ntiles) ring.wait(j, &g_status_scan);
     } else if (ln.on) {
-      for (int k = 0; k < kRows && row0 + k < q.len; ++k) {
-        const long long t = q.lo + row0 + k;
-        put_pair<T>(xs, k, load_pair<T, false>(static_cast<const T*>(p.x) + q.batch * p.xb + t * p.xt + ln.c, ln.two).get());
-        put_pair<T>(rs, k, load_pair<T, false>(static_cast<const T*>(p.r) + q.batch * p.rb + t * p.rt + ln.c, ln.two).get());
-        put_pair<T>(is, k, load_pair<T, false>(static_cast<const T*>(p.i) + q.batch * p.ib + t * p.it + ln.c, ln.two).get());
-      }
+      const long long t = q.lo + row0;
+      fill<T>(xs, p.x, q.batch * p.xb + t * p.xt + ln.c, p.xt, have, ln.two);
+      fill<T>(rs, p.r, q.batch * p.rb + t * p.rt + ln.c, p.rt, have, ln.two);
+      fill<T>(is, p.i, q.batch * p.ib + t * p.it + ln.c, p.it, have, ln.two);
     }
-    if (row0 + kRows > q.len) {  // rows past the sequence's end hold the state
-      for (int k = 0; k < kRows; ++k)
-        if (row0 + k >= q.len) {
-          put_pair<T>(rs, k, f2(-INFINITY));
-          put_pair<T>(is, k, f2(0.f));
-          put_pair<T>(xs, k, f2(0.f));
-        }
+    for (int k = have; k < kRows; ++k) {  // rows past the sequence's end hold the state
+      put_pair<T>(rs, k, f2(-INFINITY));
+      put_pair<T>(is, k, f2(0.f));
+      put_pair<T>(xs, k, f2(0.f));
     }
+    if (TMA && have < kRows) fence_proxy_async_smem();  // before TMA writes there again
     float2 A[kRows], S[kRows];
+    RawPair<T> r[kRows];
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      float2 a, b;
-      token_pair<T>(get_pair<T>(xs, k).get(), get_pair<T>(rs, k).get(), get_pair<T>(is, k).get(), decay, a, b);
-      A[k] = k == 0 ? a : __fmul2_rn(a, A[k - 1]);
-      S[k] = k == 0 ? b : __ffma2_rn(a, S[k - 1], b);
-    }
-    maps[warp][lane] = make_float4(A[kRows - 1].x, A[kRows - 1].y, S[kRows - 1].x, S[kRows - 1].y);
+    for (int k = 0; k < kRows; ++k) r[k] = get_pair<T>(rs, k);
+    auto scan_rows = [&](auto is_plain) {
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        float2 a, b;
+        token_pair<T, decltype(is_plain)::value>(get_pair<T>(xs, k).get(), r[k].get(), get_pair<T>(is, k).get(), ndecay,
+                                                 a, b);
+        A[k] = k == 0 ? a : __fmul2_rn(a, A[k - 1]);
+        S[k] = k == 0 ? b : __ffma2_rn(a, S[k - 1], b);
+      }
+    };
+    if (plain && !any_held(min_rows(r)))
+      scan_rows(std::true_type());
+    else
+      scan_rows(std::false_type());
+    maps[par][warp][lane] = make_float4(A[kRows - 1].x, A[kRows - 1].y, S[kRows - 1].x, S[kRows - 1].y);
     __syncthreads();
-    float2 h = carry;
-    if (nblk > 1) {
-      if (warp == 0) {
+    if (TMA && threadIdx.x == 0) ask(j + NS);
+    float2 h = carry, hin;
+    if (nblk == 1) {
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w == warp) hin = carry;
+        carry = apply(maps[par][w][lane], carry);
+      }
+    } else {
+      if (warp == kWarps - 1) {
         float2 ta = f2(1.f), ts = f2(0.f);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float4 m = maps[w][lane];
+          const float4 m = maps[par][w][lane];
           ta = __fmul2_rn(ta, make_float2(m.x, m.y));
           ts = apply(m, ts);
         }
-        for (int b = 0; b < nblk; ++b) store_remote(&tiles[par][rank][lane], b, make_float4(ta.x, ta.y, ts.x, ts.y));
+        ex.send(j, make_float4(ta.x, ta.y, ts.x, ts.y));
       }
-      cluster_barrier();
-      for (int b = 0; b < nblk; ++b) {
-        if (b == rank) h = carry;
-        carry = apply(tiles[par][b][lane], carry);
-      }
+      h = ex.receive(j, carry, &g_status_scan);
+      hin = h;
+      for (int w = 0; w < warp; ++w) hin = apply(maps[par][w][lane], hin);
     }
     if (p.states != nullptr && warp == 0 && tile < ntiles) ln.store(p.states + (q.slot + tile) * p.D, h);
-    float2 hin = h;
+    if (ln.on) {
+      T* yr = y + (long long)row0 * p.D;
+      if (have == kRows) {
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w == warp) hin = h;
-      h = apply(maps[w][lane], h);
-    }
-    if (nblk == 1) carry = h;
-    const bool whole = TMA && (tile + 1) * kChunk <= q.len;
-    if (whole) {
+        for (int k = 0; k < kRows; ++k)
+          store_pair<T, TMA>(yr + (long long)k * p.D, __ffma2_rn(A[k], hin, S[k]), ln.two);
+      } else {
 #pragma unroll
-      for (int k = 0; k < kRows; ++k) put_pair<T>(xs, k, __ffma2_rn(A[k], hin, S[k]));
-    } else if (ln.on) {
-#pragma unroll
-      for (int k = 0; k < kRows; ++k)
-        if (row0 + k < q.len) store_pair<T, false>(y + (long long)(row0 + k) * p.D, __ffma2_rn(A[k], hin, S[k]), ln.two);
-    }
-    if constexpr (TMA) fence_proxy_async_smem();
-    __syncthreads();
-    if constexpr (TMA) {
-      if (threadIdx.x == 0) {
-        if (whole) tma_store_3d(&tm.out[0], ring.slot(j, 0), blockIdx.y * kCols, q.lo + tile * kChunk, (int)q.batch);
-        bulk_commit_group();
-        // Step j + 2 goes into the stage of step j + 2 - NS, whose tile must have left.
-        if constexpr (NS == 3)
-          bulk_wait_group_read1();
-        else
-          bulk_wait_group_read0();
-        if (j + 2 < rounds) ask(j + 2);
+        for (int k = 0; k < kRows; ++k)
+          if (k < have) store_pair<T, TMA>(yr + (long long)k * p.D, __ffma2_rn(A[k], hin, S[k]), ln.two);
       }
     }
   }
-  if (TMA && threadIdx.x == 0) bulk_wait_group0();
   if (p.final_state != nullptr && rank == 0 && warp == 0) ln.store(p.final_state + (long long)n * p.D, carry);
+  if (nblk > 1) cluster_barrier();  // no block leaves while another may still send to it
 }
 
 // --------------------------------------------------------------------------- backward
 // The same tiles from the back. A lane keeps s, p, t = a - 1 and the injected term of its 8
 // tokens; two maps a warp go through shared memory, the forward one (h, from the chunk's kept
-// state) and the backward one (G_t = a_t dh_t, from the tile behind), and the gradients leave
-// in the slots of x, r and i. Clusters exchange the backward maps only: every tile's entering
-// state is known.
+// state) and the backward one (G_t = a_t dh_t, from the tile behind). Clusters exchange the
+// backward maps only: every tile's entering state is known. x and dy are read again from the
+// tile after the barrier, so a stage is refilled at the next step's barrier.
 template <typename T, bool TMA>
-__global__ void __launch_bounds__(32 * kWarps, bwd_per_sm<T>())
+__global__ void __launch_bounds__(32 * kWarps, Bwd<T>::kPerSm)
     scan_bwd_tiles(const __grid_constant__ Args p, const __grid_constant__ Maps tm) {
-  extern __shared__ __align__(1024) uint8_t stages[];
-  __shared__ __align__(16) float4 maps[kWarps][32];
-  __shared__ __align__(16) float2 back[kWarps][32];
-  __shared__ __align__(16) float4 tiles[2][8][32];
-  __shared__ __align__(8) uint64_t full[4];
-  constexpr int NS = bwd_stages<T>();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  extern __shared__ __align__(128) uint8_t stages[];
+  __shared__ __align__(16) float4 maps[2][kWarps][32];
+  __shared__ __align__(16) float2 back[2][kWarps][32];
+  __shared__ __align__(16) float4 slots[2][8][32];
+  __shared__ __align__(8) uint64_t full[Bwd<T>::kStages], xbar[2];
+  constexpr int NS = Bwd<T>::kStages;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int nblk = cluster_size(), rank = cluster_rank();
   const Lane ln(blockIdx.y * kCols, p.D);
   const int n = blockIdx.z;
@@ -509,40 +590,43 @@ __global__ void __launch_bounds__(32 * kWarps, bwd_per_sm<T>())
       }
     return;
   }
-  Ring<T, TMA, 4, NS> ring(stages, full);
-  if (nblk > 1) cluster_barrier();
+  typename Bwd<T>::R ring(stages, full);
+  Exchange ex(slots, xbar, nblk, rank);
   const Seq q = sequence(p, n);
   const long long first = (q.batch * p.T + q.lo) * p.D;
-  const float2 decay = limit_decay(ln.load(p.decay));
+  const float2 ndecay = neg_decay(ln, p.decay);
+  const bool plain = plain_decays(ndecay);
   float2 carry = p.dfinal != nullptr ? ln.load(p.dfinal + (long long)n * p.D) : f2(0.f);
   float2 ddecay = f2(0.f);
   const int ntiles = (q.len + kChunk - 1) / kChunk;
   const int rounds = (ntiles + nblk - 1) / nblk;
   auto ask = [&](int j) {
     const int tile = ntiles - 1 - (j * nblk + rank);
-    if (tile >= 0 && ring.ok) ring.ask(tm.in, j, blockIdx.y * kCols, q.lo + tile * kChunk, (int)q.batch);
+    if (tile >= 0) ring.ask(tm.in, j, blockIdx.y * kCols, q.lo + tile * kChunk, (int)q.batch);
   };
-  if (TMA && threadIdx.x == 0) {
-    ask(0);
-    ask(1);
-  }
+  if (TMA && threadIdx.x == 0)
+    for (int j = 0; j < NS; ++j) ask(j);
   const int own = (warp * kRows * kCols + 2 * lane) * (int)sizeof(T);
   for (int j = 0; j < rounds; ++j) {
     const int tile = ntiles - 1 - (j * nblk + rank), row0 = tile * kChunk + warp * kRows, par = j & 1;
     uint8_t *xs = ring.slot(j, 0) + own, *rs = ring.slot(j, 1) + own, *is = ring.slot(j, 2) + own,
             *gs = ring.slot(j, 3) + own;
-    const int have = tile < 0 ? 0 : min(max(q.len - row0, 0), kRows);  // rows of the lane's 8
+    const int have = tile < 0 ? 0 : min(max(q.len - row0, 0), kRows);
     float2 h = tile >= 0 ? ln.load(p.states + (q.slot + tile) * p.D) : f2(0.f);
+    if constexpr (NS == 1) {
+      if (j > 0) {  // the one stage: refilled once every warp is through with it
+        __syncthreads();
+        if (TMA && threadIdx.x == 0) ask(j);
+      }
+    }
     if constexpr (TMA) {
       if (tile >= 0) ring.wait(j, &g_status_scan);
     } else if (ln.on) {
-      for (int k = 0; k < have; ++k) {
-        const long long t = q.lo + row0 + k;
-        put_pair<T>(xs, k, load_pair<T, false>(static_cast<const T*>(p.x) + q.batch * p.xb + t * p.xt + ln.c, ln.two).get());
-        put_pair<T>(rs, k, load_pair<T, false>(static_cast<const T*>(p.r) + q.batch * p.rb + t * p.rt + ln.c, ln.two).get());
-        put_pair<T>(is, k, load_pair<T, false>(static_cast<const T*>(p.i) + q.batch * p.ib + t * p.it + ln.c, ln.two).get());
-        put_pair<T>(gs, k, load_pair<T, false>(static_cast<const T*>(p.dy) + q.batch * p.gb + t * p.gt + ln.c, ln.two).get());
-      }
+      const long long t = q.lo + row0;
+      fill<T>(xs, p.x, q.batch * p.xb + t * p.xt + ln.c, p.xt, have, ln.two);
+      fill<T>(rs, p.r, q.batch * p.rb + t * p.rt + ln.c, p.rt, have, ln.two);
+      fill<T>(is, p.i, q.batch * p.ib + t * p.it + ln.c, p.it, have, ln.two);
+      fill<T>(gs, p.dy, q.batch * p.gb + t * p.gt + ln.c, p.gt, have, ln.two);
     }
     for (int k = have; k < kRows; ++k) {
       put_pair<T>(rs, k, f2(-INFINITY));
@@ -550,122 +634,119 @@ __global__ void __launch_bounds__(32 * kWarps, bwd_per_sm<T>())
       put_pair<T>(xs, k, f2(0.f));
       put_pair<T>(gs, k, f2(0.f));
     }
+    if (TMA && have < kRows) fence_proxy_async_smem();
     float2 t[kRows], hp[kRows], s[kRows], pi[kRows];
     float2 A = f2(1.f), S = f2(0.f), P = f2(0.f);
+    RawPair<T> r[kRows];
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      const float2 r = get_pair<T>(rs, k).get();
-      float2 a;
-      sigmoids<T, true>(r, get_pair<T>(is, k).get(), s[k], pi[k]);
-      s[k] = make_float2(r.x < kHoldBelow ? 0.f : s[k].x, r.y < kHoldBelow ? 0.f : s[k].y);
-      decay_pair(__fmul2_rn(decay, s[k]), a, t[k]);
-      const float2 m2 = m2_of(t[k]), x = get_pair<T>(xs, k).get();
-      const float2 m = make_float2(sqrt_approx(m2.x), sqrt_approx(m2.y));
-      const float2 b = __fmul2_rn(__fmul2_rn(m, pi[k]), x);
-      hp[k] = make_float2(s[k].x == 0.f ? 0.f : b.x, s[k].y == 0.f ? 0.f : b.y);
-      A = __fmul2_rn(a, A);
-      S = __ffma2_rn(a, S, hp[k]);
-    }
+    for (int k = 0; k < kRows; ++k) r[k] = get_pair<T>(rs, k);
+    auto scan_rows = [&](auto is_plain) {
+      constexpr bool kPlain = decltype(is_plain)::value;
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        float2 a;
+        sigmoids<T, kPlain>(r[k].get(), get_pair<T>(is, k).get(), s[k], pi[k]);
+        decay_pair<kPlain>(__fmul2_rn(ndecay, s[k]), a, t[k]);
+        const float2 m2 = m2_of(t[k]);
+        const float2 m = make_float2(sqrt_approx(m2.x), sqrt_approx(m2.y));
+        hp[k] = __fmul2_rn(__fmul2_rn(m, pi[k]), get_pair<T>(xs, k).get());
+        if constexpr (!kPlain) hp[k] = make_float2(s[k].x == 0.f ? 0.f : hp[k].x, s[k].y == 0.f ? 0.f : hp[k].y);
+        A = __fmul2_rn(a, A);
+        S = __ffma2_rn(a, S, hp[k]);
+      }
+    };
+    const bool plain_tile = plain && !any_held(min_rows(r));
+    if (plain_tile)
+      scan_rows(std::true_type());
+    else
+      scan_rows(std::false_type());
 #pragma unroll
     for (int k = kRows - 1; k >= 0; --k)
       P = __fmul2_rn(__fadd2_rn(t[k], f2(1.f)), __fadd2_rn(P, get_pair<T>(gs, k).get()));
-    maps[warp][lane] = make_float4(A.x, A.y, S.x, S.y);
-    back[warp][lane] = P;
+    maps[par][warp][lane] = make_float4(A.x, A.y, S.x, S.y);
+    back[par][warp][lane] = P;
     __syncthreads();
-    float2 G = carry;
-    if (nblk > 1) {
+    if (NS > 1 && TMA && threadIdx.x == 0 && j > 0) ask(j - 1 + NS);  // step j - 1's stage is free
+    float2 gin = carry;
+    if (nblk == 1) {
+#pragma unroll
+      for (int w = kWarps - 1; w >= 0; --w) {
+        if (w == warp) gin = carry;
+        const float4 m = maps[par][w][lane];
+        carry = __ffma2_rn(make_float2(m.x, m.y), carry, back[par][w][lane]);
+      }
+      for (int w = 0; w < warp; ++w) h = apply(maps[par][w][lane], h);
+    } else {
       if (warp == 0) {
         float2 ta = f2(1.f), tp = f2(0.f);
 #pragma unroll
         for (int w = kWarps - 1; w >= 0; --w) {
-          const float4 m = maps[w][lane];
+          const float4 m = maps[par][w][lane];
           ta = __fmul2_rn(ta, make_float2(m.x, m.y));
-          tp = __ffma2_rn(make_float2(m.x, m.y), tp, back[w][lane]);
+          tp = __ffma2_rn(make_float2(m.x, m.y), tp, back[par][w][lane]);
         }
-        for (int b = 0; b < nblk; ++b) store_remote(&tiles[par][rank][lane], b, make_float4(ta.x, ta.y, tp.x, tp.y));
+        ex.send(j, make_float4(ta.x, ta.y, tp.x, tp.y));
       }
-      cluster_barrier();
-      for (int b = 0; b < nblk; ++b) {
-        if (b == rank) G = carry;
-        carry = apply(tiles[par][b][lane], carry);
+      for (int w = 0; w < warp; ++w) h = apply(maps[par][w][lane], h);
+      gin = ex.receive(j, carry, &g_status_scan);
+      for (int w = kWarps - 1; w > warp; --w) {
+        const float4 m = maps[par][w][lane];
+        gin = __ffma2_rn(make_float2(m.x, m.y), gin, back[par][w][lane]);
       }
     }
-#pragma unroll
-    for (int w = 0; w < kWarps - 1; ++w)
-      if (w < warp) h = apply(maps[w][lane], h);
-    float2 gin = G;
-#pragma unroll
-    for (int w = kWarps - 1; w >= 0; --w) {
-      if (w == warp) gin = G;
-      const float4 m = maps[w][lane];
-      G = __ffma2_rn(make_float2(m.x, m.y), G, back[w][lane]);
-    }
-    if (nblk == 1) carry = G;
 #pragma unroll
     for (int k = 0; k < kRows; ++k) {  // the state before each token
       const float2 b = hp[k];
       hp[k] = h;
       h = __ffma2_rn(__fadd2_rn(t[k], f2(1.f)), h, b);
     }
-    const bool whole = TMA && tile >= 0 && (tile + 1) * kChunk <= q.len;
+    const long long o = first + (long long)row0 * p.D;
+    T *dxr = dx + o, *drr = dr + o, *dir = di + o;
+    auto grad_rows = [&](auto is_plain) {
+      constexpr bool kPlain = decltype(is_plain)::value;
 #pragma unroll
-    for (int k = kRows - 1; k >= 0; --k) {
-      const float2 a = __fadd2_rn(t[k], f2(1.f)), m2 = m2_of(t[k]);
-      const float2 im = make_float2(m2.x > 0.f ? rsqrtf(m2.x) : 0.f, m2.y > 0.f ? rsqrtf(m2.y) : 0.f);
-      float2 x = get_pair<T>(xs, k).get();
-      x = make_float2(s[k].x == 0.f ? 0.f : x.x, s[k].y == 0.f ? 0.f : x.y);
-      const float2 dh = __fadd2_rn(get_pair<T>(gs, k).get(), gin);
-      gin = __fmul2_rn(a, dh);
-      const float2 gx = __fmul2_rn(dh, __fmul2_rn(__fmul2_rn(m2, im), pi[k]));  // dh m p
-      const float2 np = __fadd2_rn(f2(1.f), make_float2(-pi[k].x, -pi[k].y));
-      const float2 gi = __fmul2_rn(__fmul2_rn(gx, x), np);
-      // dL = a dh (a p x / m - h_{t-1})
-      const float2 u = __fmul2_rn(__fmul2_rn(__fmul2_rn(a, im), pi[k]), x);
-      const float2 dL = __fmul2_rn(gin, __fadd2_rn(u, make_float2(-hp[k].x, -hp[k].y)));
-      const float2 dLs = __fmul2_rn(dL, s[k]);
-      ddecay = __fadd2_rn(ddecay, dLs);
-      const float2 ns = __fadd2_rn(f2(1.f), make_float2(-s[k].x, -s[k].y));
-      const float2 gr = __fmul2_rn(__fmul2_rn(dLs, decay), ns);
-      if (whole) {
-        put_pair<T>(xs, k, gx);
-        put_pair<T>(rs, k, gr);
-        put_pair<T>(is, k, gi);
-      } else if (ln.on && k < have) {
-        const long long o = first + (long long)(row0 + k) * p.D;
-        store_pair<T, false>(dx + o, gx, ln.two);
-        store_pair<T, false>(dr + o, gr, ln.two);
-        store_pair<T, false>(di + o, gi, ln.two);
-      }
-    }
-    if constexpr (TMA) fence_proxy_async_smem();
-    __syncthreads();
-    if constexpr (TMA) {
-      if (threadIdx.x == 0) {
-        if (whole) {
-#pragma unroll
-          for (int k = 0; k < 3; ++k)
-            tma_store_3d(&tm.out[k], ring.slot(j, k), blockIdx.y * kCols, q.lo + tile * kChunk, (int)q.batch);
+      for (int k = kRows - 1; k >= 0; --k) {
+        const float2 a = __fadd2_rn(t[k], f2(1.f)), m2 = m2_of(t[k]);
+        float2 im = make_float2(rsqrt_approx(m2.x), rsqrt_approx(m2.y));
+        float2 x = get_pair<T>(xs, k).get();
+        if constexpr (!kPlain) {  // no gradient through m where it is 0, none at all where the token held
+          im = make_float2(m2.x > 0.f ? im.x : 0.f, m2.y > 0.f ? im.y : 0.f);
+          x = make_float2(s[k].x == 0.f ? 0.f : x.x, s[k].y == 0.f ? 0.f : x.y);
         }
-        bulk_commit_group();
-        if constexpr (NS == 3)
-          bulk_wait_group_read1();
-        else
-          bulk_wait_group_read0();
-        if (j + 2 < rounds) ask(j + 2);
+        const float2 dh = __fadd2_rn(get_pair<T>(gs, k).get(), gin);
+        gin = __fmul2_rn(a, dh);
+        const float2 w = __fmul2_rn(im, pi[k]);                // p / m
+        const float2 gx = __fmul2_rn(dh, __fmul2_rn(m2, w));   // dh m p
+        const float2 gi = __fmul2_rn(__fmul2_rn(gx, x), __ffma2_rn(pi[k], f2(-1.f), f2(1.f)));
+        // dL = a dh (a p x / m - h_{t-1})
+        const float2 u = __ffma2_rn(hp[k], f2(-1.f), __fmul2_rn(__fmul2_rn(a, w), x));
+        const float2 dLs = __fmul2_rn(__fmul2_rn(gin, u), s[k]);
+        ddecay = __fadd2_rn(ddecay, dLs);
+        const float2 gr = __fmul2_rn(__fmul2_rn(dLs, ndecay), __fadd2_rn(s[k], f2(-1.f)));
+        if (ln.on && k < have) {
+          store_pair<T, TMA>(dxr + (long long)k * p.D, gx, ln.two);
+          store_pair<T, TMA>(drr + (long long)k * p.D, gr, ln.two);
+          store_pair<T, TMA>(dir + (long long)k * p.D, gi, ln.two);
+        }
       }
-    }
+    };
+    if (plain_tile)
+      grad_rows(std::true_type());
+    else
+      grad_rows(std::false_type());
   }
-  if (TMA && threadIdx.x == 0) bulk_wait_group0();
   // ddecay over the block's warps, in order.
-  back[warp][lane] = ddecay;
+  __syncthreads();
+  back[0][warp][lane] = ddecay;
   __syncthreads();
   if (warp == 0) {
     float2 d = f2(0.f);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) d = __fadd2_rn(d, back[w][lane]);
+    for (int w = 0; w < kWarps; ++w) d = __fadd2_rn(d, back[0][w][lane]);
     ln.store(p.ddecay_part + ((long long)n * nblk + rank) * p.D, d);
     if (p.dh0 != nullptr && rank == 0) ln.store(p.dh0 + (long long)n * p.D, carry);
   }
+  if (nblk > 1) cluster_barrier();
 }
 
 struct StoreColumn {
@@ -722,7 +803,7 @@ int cluster_blocks(int T, int D, int nseq, bool packed, int per_sm) {
 }
 
 int bwd_cluster(int T, int D, int nseq, bool packed, int dtype) {
-  return cluster_blocks(T, D, nseq, packed, dtype == THM_BF16 ? bwd_per_sm<__nv_bfloat16>() : bwd_per_sm<float>());
+  return cluster_blocks(T, D, nseq, packed, dtype == THM_BF16 ? Bwd<__nv_bfloat16>::kPerSm : Bwd<float>::kPerSm);
 }
 
 template <typename K>
@@ -752,7 +833,7 @@ int launch_tiles(K kernel, const Args& p, const Maps& tm, int n, int seqs, int s
 template <typename T>
 int run_fwd(const Args& p, int B, int seqs, int dtype, cudaStream_t st) {
   constexpr int elem = sizeof(T);
-  const int per_sm = fwd_per_sm<T>();
+  const int per_sm = Fwd<T>::kPerSm;
   if (p.T <= kDirectTokens) {
     const dim3 grid((p.D + 2 * kDirectThreads - 1) / (2 * kDirectThreads), seqs);
     if (multiples(2 * elem, elem, p.D, {p.x, p.r, p.i, p.y}, {p.xb, p.xt, p.rb, p.rt, p.ib, p.it}))
@@ -763,13 +844,11 @@ int run_fwd(const Args& p, int B, int seqs, int dtype, cudaStream_t st) {
   }
   const int n = cluster_blocks(p.T, p.D, p.nseq, p.cu != nullptr, per_sm);
   Maps tm{};
-  const long long ys = p.D;
   bool tma = multiples(16, elem, p.D, {p.x, p.r, p.i, p.y}, {B > 1 ? p.xb : 0, p.xt, B > 1 ? p.rb : 0, p.rt, B > 1 ? p.ib : 0, p.it});
   tma = tma && encode(&tm.in[0], dtype, p.x, p.xb, p.xt, B, p.T, p.D) == THM_OK &&
         encode(&tm.in[1], dtype, p.r, p.rb, p.rt, B, p.T, p.D) == THM_OK &&
-        encode(&tm.in[2], dtype, p.i, p.ib, p.it, B, p.T, p.D) == THM_OK &&
-        encode(&tm.out[0], dtype, p.y, ys * p.T, ys, B, p.T, p.D) == THM_OK;
-  const int smem = Ring<T, true, 3, fwd_stages<T>()>::kBytes;
+        encode(&tm.in[2], dtype, p.i, p.ib, p.it, B, p.T, p.D) == THM_OK;
+  const int smem = Fwd<T>::R::kBytes;
   return tma ? launch_tiles(scan_tiles<T, true>, p, tm, n, seqs, smem, st)
              : launch_tiles(scan_tiles<T, false>, p, tm, n, seqs, smem, st);
 }
@@ -778,17 +857,13 @@ template <typename T>
 int run_bwd(const Args& p, int B, int seqs, int dtype, int n, cudaStream_t st) {
   constexpr int elem = sizeof(T);
   Maps tm{};
-  const long long ys = p.D;
   bool tma = multiples(16, elem, p.D, {p.x, p.r, p.i, p.dy, p.dx, p.dr, p.di},
                        {B > 1 ? p.xb : 0, p.xt, B > 1 ? p.rb : 0, p.rt, B > 1 ? p.ib : 0, p.it, B > 1 ? p.gb : 0, p.gt});
   tma = tma && p.T > 0 && encode(&tm.in[0], dtype, p.x, p.xb, p.xt, B, p.T, p.D) == THM_OK &&
         encode(&tm.in[1], dtype, p.r, p.rb, p.rt, B, p.T, p.D) == THM_OK &&
         encode(&tm.in[2], dtype, p.i, p.ib, p.it, B, p.T, p.D) == THM_OK &&
-        encode(&tm.in[3], dtype, p.dy, p.gb, p.gt, B, p.T, p.D) == THM_OK &&
-        encode(&tm.out[0], dtype, p.dx, ys * p.T, ys, B, p.T, p.D) == THM_OK &&
-        encode(&tm.out[1], dtype, p.dr, ys * p.T, ys, B, p.T, p.D) == THM_OK &&
-        encode(&tm.out[2], dtype, p.di, ys * p.T, ys, B, p.T, p.D) == THM_OK;
-  const int smem = Ring<T, true, 4, bwd_stages<T>()>::kBytes;
+        encode(&tm.in[3], dtype, p.dy, p.gb, p.gt, B, p.T, p.D) == THM_OK;
+  const int smem = Bwd<T>::R::kBytes;
   return tma ? launch_tiles(scan_bwd_tiles<T, true>, p, tm, n, seqs, smem, st)
              : launch_tiles(scan_bwd_tiles<T, false>, p, tm, n, seqs, smem, st);
 }
