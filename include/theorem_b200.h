@@ -255,7 +255,8 @@ int thm_gated_scan_bwd_parts(int T, int D, int nseq, int packed, int dtype);
  *
  * x, gate, dy [R, C] in `dtype`, unit stride over C, row strides *_rs in
  * elements; y, dx, dgate [R, C] contiguous; weight, bias [C] fp32 or NULL (1 and
- * 0); dweight, dbias [C] fp32 or NULL, summed in a fixed order. C % G == 0,
+ * 0); dweight, dbias [C] fp32 or NULL (dbias only with bias), summed in a fixed
+ * order. C % G == 0,
  * G <= 4096. workspace: [thm_group_norm_bwd_parts(R, C, G), 2, C] fp32, needed
  * when dweight or dbias is given.
  * ------------------------------------------------------------------------- */

@@ -76,15 +76,67 @@ struct BwdArgs {
   int S, D, act, rows;  // rows: of a warp's strip
 };
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 8, kBlockRows = 4;
+
+__device__ __forceinline__ float2 f2(float v) { return make_float2(v, v); }
+
+// VEC channels as fp32 pairs (one channel: an empty second half).
+template <typename T, int VEC>
+__device__ __forceinline__ void widen(const Pack<T, VEC>& q, float2 (&f)[(VEC + 1) / 2]) {
+  if constexpr (VEC == 1) {
+    f[0] = make_float2(to_f32<T>(q.v[0]), 0.f);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC / 2; ++e) {
+      if constexpr (sizeof(T) == 2) {
+        const uint32_t w = reinterpret_cast<const uint32_t*>(&q)[e];
+        f[e] = make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+      } else {
+        f[e] = make_float2(q.v[2 * e], q.v[2 * e + 1]);
+      }
+    }
+  }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_pairs(T* p, const float2 (&f)[(VEC + 1) / 2]) {
+  if constexpr (VEC == 1) {
+    *p = from_f32<T>(f[0].x);
+  } else {
+    Pack<T, VEC> q;
+#pragma unroll
+    for (int e = 0; e < VEC / 2; ++e) {
+      if constexpr (sizeof(T) == 2)
+        reinterpret_cast<uint32_t*>(&q)[e] = pack_bf16x2(f[e].x, f[e].y);
+      else
+        reinterpret_cast<float2*>(&q)[e] = f[e];
+    }
+    *reinterpret_cast<Pack<T, VEC>*>(p) = q;
+  }
+}
+
+// g silu'(u) = g s (1 + u (1 - s)), s = sigmoid(u).
+template <typename T>
+__device__ __forceinline__ float2 through_silu(float2 g, float2 u) {
+  float2 s;
+  if constexpr (sizeof(T) == 2) {
+    const float2 e = __fmul2_rn(u, f2(-1.4426950408889634f));
+    const float2 d = __fadd2_rn(make_float2(ex2_approx(e.x), ex2_approx(e.y)), f2(1.f));
+    s = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+  } else {
+    s = make_float2(sigmoid<T>(u.x), sigmoid<T>(u.y));
+  }
+  return __fmul2_rn(g, __fmul2_rn(s, __ffma2_rn(u, __ffma2_rn(s, f2(-1.f), f2(1.f)), f2(1.f))));
+}
 
 // A block has 32 * VEC channels and kWarps strips of rows of one sequence, a strip per
-// warp. A thread walks its strip and W - 1 rows past its end: du of row t needs x of
-// rows t - W + 1 .. t, and dx of row t du of rows t .. t + W - 1, so windows of both stay
-// in registers and every row is read once but for the halo. Rows past the strip count
-// for dx only, not for dw and db.
-template <typename T, int VEC, int W>
-__global__ void __launch_bounds__(32 * kWarps) conv_bwd(const BwdArgs p) {
+// warp. A lane walks its strip and W - 1 rows past its end, four rows at a time, the next four
+// in flight: du of row t needs x of rows t - W + 1 .. t, and dx of row t du of rows t .. t + W - 1,
+// so windows of both stay in registers and every row is read once but for the halo. Rows past
+// the strip count for dx only, not for dw and db; rows past the sequence are zeros, whose du is 0.
+template <typename T, int VEC, int W, bool ACT>
+__global__ void __launch_bounds__(32 * kWarps, W <= 4 ? 2 : 1) conv_bwd(const BwdArgs p) {
+  constexpr int NP = (VEC + 1) / 2, RB = kBlockRows;
+  using Raw = Pack<T, VEC>;
   __shared__ float fold[kWarps][32 * VEC];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = (blockIdx.x * 32 + lane) * VEC;
@@ -94,64 +146,90 @@ __global__ void __launch_bounds__(32 * kWarps) conv_bwd(const BwdArgs p) {
   const T* x = static_cast<const T*>(p.x) + (long long)blockIdx.z * p.xb + c;
   const T* dy = static_cast<const T*>(p.dy) + (long long)blockIdx.z * p.gb + c;
   T* dx = static_cast<T*>(p.dx) + (long long)blockIdx.z * p.S * p.D + c;
-  float w[W][VEC], dw[W][VEC], b[VEC], db[VEC], xw[W][VEC], du[W][VEC];
+  float2 w[W][NP], dw[W][NP], b[NP], db[NP], xw[W - 1 + RB][NP], du[W - 1 + RB][NP];
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    b[e] = on ? p.b[c + e] : 0.f;
-    db[e] = 0.f;
+  for (int e = 0; e < NP; ++e) {
+    const bool two = VEC > 1;
+    b[e] = on ? make_float2(p.b[c + 2 * e], two ? p.b[c + 2 * e + 1] : 0.f) : f2(0.f);
+    db[e] = f2(0.f);
 #pragma unroll
     for (int k = 0; k < W; ++k) {
-      w[k][e] = on ? p.w[(long long)(c + e) * W + k] : 0.f;
-      dw[k][e] = du[k][e] = xw[k][e] = 0.f;
+      w[k][e] = on ? make_float2(p.w[(long long)(c + 2 * e) * W + k], two ? p.w[(long long)(c + 2 * e + 1) * W + k] : 0.f)
+                   : f2(0.f);
+      dw[k][e] = f2(0.f);
     }
   }
   if (on && t0 < t1) {
+    const int end = min(t1 + W - 1, p.S);  // rows that there are and that count
 #pragma unroll
-    for (int k = 1; k < W; ++k)  // rows t0 - W + k, in xw[k]
-      if (t0 - W + k >= 0) load_vec<T, VEC>(x + (long long)(t0 - W + k) * p.xt, xw[k]);
-    for (int t = t0; t < t1 + W - 1; ++t) {
+    for (int k = 0; k + 1 < W; ++k) {  // the rows before the strip
+      const int t = t0 - (W - 1) + k;
+      Raw q{};
+      if (t >= 0) q = *reinterpret_cast<const Raw*>(x + t * p.xt);
+      widen<T, VEC>(q, xw[k]);
+#pragma unroll
+      for (int e = 0; e < NP; ++e) du[k][e] = f2(0.f);
+    }
+    Raw xr[RB], gr[RB];
+    auto load = [&](int t) {
+#pragma unroll
+      for (int k = 0; k < RB; ++k) {
+        xr[k] = gr[k] = Raw{};
+        if (t + k < end) {
+          xr[k] = *reinterpret_cast<const Raw*>(x + (t + k) * p.xt);
+          gr[k] = *reinterpret_cast<const Raw*>(dy + (t + k) * p.gt);
+        }
+      }
+    };
+    load(t0);
+    for (int t = t0; t < t1 + W - 1; t += RB) {
+#pragma unroll
+      for (int k = 0; k < RB; ++k) {
+        widen<T, VEC>(xr[k], xw[W - 1 + k]);
+        widen<T, VEC>(gr[k], du[W - 1 + k]);
+      }
+      load(t + RB);
+      if constexpr (ACT) {
+#pragma unroll
+        for (int k = 0; k < RB; ++k)
+#pragma unroll
+          for (int e = 0; e < NP; ++e) {
+            float2 u = b[e];
+#pragma unroll
+            for (int j = 0; j < W; ++j) u = __ffma2_rn(w[j][e], xw[k + j][e], u);
+            du[W - 1 + k][e] = through_silu<T>(du[W - 1 + k][e], u);
+          }
+      }
+      if (t < t1) {  // strips are whole blocks of rows, but for the sequence's end
+#pragma unroll
+        for (int k = 0; k < RB; ++k)
+#pragma unroll
+          for (int e = 0; e < NP; ++e) {
+            db[e] = __fadd2_rn(db[e], du[W - 1 + k][e]);
+#pragma unroll
+            for (int j = 0; j < W; ++j) dw[j][e] = __ffma2_rn(du[W - 1 + k][e], xw[k + j][e], dw[j][e]);
+          }
+      }
+#pragma unroll
+      for (int k = 0; k < RB; ++k) {  // dx of row t + k - (W - 1)
+        const int row = t + k - (W - 1);
+        if (row < t0 || row >= t1) continue;
+        float2 g[NP];
+#pragma unroll
+        for (int e = 0; e < NP; ++e) {
+          g[e] = __fmul2_rn(w[0][e], du[k + W - 1][e]);
+#pragma unroll
+          for (int j = 1; j < W; ++j) g[e] = __ffma2_rn(w[j][e], du[k + W - 1 - j][e], g[e]);
+        }
+        store_pairs<T, VEC>(dx + (long long)row * p.D, g);
+      }
 #pragma unroll
       for (int k = 0; k + 1 < W; ++k)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          xw[k][e] = xw[k + 1][e];
-          du[k][e] = du[k + 1][e];
+        for (int e = 0; e < NP; ++e) {
+          xw[k][e] = xw[k + RB][e];
+          du[k][e] = du[k + RB][e];
         }
-      if (t < p.S) {
-        load_vec<T, VEC>(x + t * p.xt, xw[W - 1]);
-        load_vec<T, VEC>(dy + t * p.gt, du[W - 1]);
-        if (p.act) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            float u = b[e], f, df;
-#pragma unroll
-            for (int k = 0; k < W; ++k) u = fmaf(w[k][e], xw[k][e], u);
-            silu_grad<T>(u, f, df);
-            du[W - 1][e] *= df;
-          }
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) du[W - 1][e] = 0.f;
-      }
-      if (t < t1) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          db[e] += du[W - 1][e];
-#pragma unroll
-          for (int k = 0; k < W; ++k) dw[k][e] = fmaf(du[W - 1][e], xw[k][e], dw[k][e]);
-        }
-      }
-      if (t - (W - 1) >= t0) {  // dx of row t - W + 1: du of rows t - W + 1 .. t are du[0 .. W - 1]
-        float g[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          g[e] = 0.f;
-#pragma unroll
-          for (int k = 0; k < W; ++k) g[e] = fmaf(w[k][e], du[W - 1 - k][e], g[e]);
-        }
-        store_vec<T, VEC>(dx + (long long)(t - W + 1) * p.D, g);
-      }
     }
   }
   // The strips' sums, added in the order of the rows.
@@ -160,7 +238,11 @@ __global__ void __launch_bounds__(32 * kWarps) conv_bwd(const BwdArgs p) {
   for (int k = 0; k <= W; ++k) {
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) fold[warp][lane * VEC + e] = k < W ? dw[k < W ? k : 0][e] : db[e];
+    for (int e = 0; e < NP; ++e) {
+      const float2 v = k < W ? dw[k < W ? k : 0][e] : db[e];
+      fold[warp][lane * VEC + 2 * e] = v.x;
+      if constexpr (VEC > 1) fold[warp][lane * VEC + 2 * e + 1] = v.y;
+    }
     __syncthreads();
     for (int j = threadIdx.x; j < 32 * VEC; j += 32 * kWarps) {
       const int col = blockIdx.x * 32 * VEC + j;
@@ -233,14 +315,17 @@ void launch_step(const StepArgs& p, int W, int vec, cudaStream_t st) {
   });
 }
 
+// Channels a lane of the backward kernel takes where vectors fit: its windows and sums of more
+// than 4 taps do not fit the registers for 4.
+constexpr int bwd_vec(int W) { return W <= 4 ? 4 : 2; }
+
 template <typename T>
 void launch_bwd(const BwdArgs& p, dim3 grid, int W, int vec, cudaStream_t st) {
   with_width(W, [&](auto w) {
-    constexpr int kW = decltype(w)::value;
-    if (vec == 4)
-      conv_bwd<T, 4, kW><<<grid, 32 * kWarps, 0, st>>>(p);
-    else
-      conv_bwd<T, 1, kW><<<grid, 32 * kWarps, 0, st>>>(p);
+    constexpr int kW = decltype(w)::value, kVec = bwd_vec(kW);
+    auto k = vec > 1 ? (p.act ? conv_bwd<T, kVec, kW, true> : conv_bwd<T, kVec, kW, false>)
+                     : (p.act ? conv_bwd<T, 1, kW, true> : conv_bwd<T, 1, kW, false>);
+    k<<<grid, 32 * kWarps, 0, st>>>(p);
   });
 }
 
@@ -296,7 +381,7 @@ extern "C" int thm_causal_conv1d_bwd(const void* x, const float* weight, const f
     const uintptr_t bits = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(dy) |
                            reinterpret_cast<uintptr_t>(dx) | (uintptr_t)(D * elem) | (uintptr_t)(x_bs * elem) |
                            (uintptr_t)(x_ts * elem) | (uintptr_t)(dy_bs * elem) | (uintptr_t)(dy_ts * elem);
-    const int vec = convg::vector_of(bits, elem);
+    const int vec = convg::vector_of(bits, elem) > 1 ? convg::bwd_vec(W) : 1;
     const int rows = convg::strip_rows(B, S, D);
     const int blocks_y = parts / B;
     if (blocks_y > 65535) return THM_ERR_UNSUPPORTED;

@@ -119,16 +119,6 @@ struct Lane {
 
 __device__ __forceinline__ float2 f2(float v) { return make_float2(v, v); }
 
-__device__ __forceinline__ float ex2_approx(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ float rcp_approx(float x) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 __device__ __forceinline__ float sqrt_approx(float x) {
   float r;
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -781,27 +771,21 @@ int encode(CUtensorMap* m, int dtype, const void* base, long long bs, long long 
 // Up to this many tokens a lane's serial walk beats the tiles.
 constexpr int kDirectTokens = 16;
 
-// Blocks that share a sequence. All blocks of a launch take about the same time, so what counts
-// is how full the last of the rounds of resident blocks is; among equals the fewest, and never
-// more than an average sequence has pairs of tiles for.
+// Blocks that share a sequence: as many as fit the GPU at once, and no more than a sequence (an
+// average one when packed) has pairs of tiles for. Measured on bf16, forward: B8 T4096 D2048
+// (256 sequences of channels) 127 us alone, 141 with two blocks each, 158 with eight; B1 T131072
+// D2048 2473 us alone, 618 with eight. Where a grid of single blocks leaves less than a second
+// round to fill and sequences are long, halves of them fill it better (B16 T8192: 446 us
+// alone, 426 with two, 476 with four; backward 846, 803, 858).
 int cluster_blocks(int T, int D, int nseq, bool packed, int per_sm) {
   const long long base = (long long)nseq * ((D + kCols - 1) / kCols);
   const long long tiles = ((packed ? (T + nseq - 1) / nseq : T) + kChunk - 1) / kChunk;
   const long long slots = (long long)sm_count() * per_sm;
-  int best = 1;
-  double best_fill = 0.;
-  for (int n = 1; n <= 8; n *= 2) {
-    if (n > 1 && tiles < 2 * n) break;
-    const long long blocks = base * n;
-    const double fill = (double)blocks / (double)((blocks + slots - 1) / slots * slots);
-    if (fill > best_fill * 1.05) {
-      best = n;
-      best_fill = fill;
-    }
-  }
-  return best;
+  if (base > slots) return base < 2 * slots && tiles >= 96 ? 2 : 1;
+  int n = 1;
+  while (n < 8 && base * n * 2 <= slots && tiles >= 4 * n) n *= 2;
+  return n;
 }
-
 int bwd_cluster(int T, int D, int nseq, bool packed, int dtype) {
   return cluster_blocks(T, D, nseq, packed, dtype == THM_BF16 ? Bwd<__nv_bfloat16>::kPerSm : Bwd<float>::kPerSm);
 }

@@ -24,13 +24,13 @@ struct Args {
   const void *x, *z, *dy;
   const float *w, *b;
   void *y, *dx, *dz;
-  float* part;             // backward: [blocks in y, 2, C] sums of dw and db, or null
+  float* part;             // backward: [blocks in y, 1 or 2, C] sums of dw and db, or null
   long long xs, zs, gs;    // row strides of x, z, dy
   long long R;
   int C, G, groups;
   int tl;                  // lanes of a team; 0: the whole block
   int gpc, rpi;            // groups and rows that a block works on at a time
-  int center, act;
+  int center, flags;
   float eps;
 };
 
@@ -50,7 +50,7 @@ __device__ __forceinline__ float team_sum(float v, int tl, float* sh) {
 }
 
 // Where a thread stands: its team's group and row offset in the block, and whether the
-// team has work. Channel of vector j: c0 + j * step.
+// team has work.
 struct Place {
   int group, sub, lane, width;
   bool on;
@@ -68,176 +68,266 @@ __device__ __forceinline__ Place place(const Args& p) {
 
 constexpr int max_threads(int vec) { return vec == 1 ? 1024 : vec == 2 ? 512 : 256; }
 
-// Mean (if centred) and scale of the group in v; masked vectors hold zeros. v is centred.
-template <int VEC, int NV>
-__device__ __forceinline__ float normalise(float (&v)[NV][VEC], const bool (&have)[NV], const Args& p, float* sh) {
-  const float inv = 1.f / (float)p.G;
-  if (p.center) {
-    float s = 0.f;
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) s += v[j][e];
-    const float mu = team_sum(s, p.tl, sh) * inv;
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[j][e] = have[j] ? v[j][e] - mu : 0.f;
-  }
-  float s2 = 0.f;
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) s2 = fmaf(v[j][e], v[j][e], s2);
-  return rsqrtf(fmaf(team_sum(s2, p.tl, sh), inv, p.eps));
+// What a call does besides the norm. The kernels for whole 16-byte vectors have it as a
+// template argument, the narrow ones (FLAGS < 0) look at p.flags.
+constexpr int kGate = 1, kAct = 2, kBias = 4;
+template <int FLAGS>
+__device__ __forceinline__ bool flag(const Args& p, int bit) {
+  return FLAGS >= 0 ? (FLAGS & bit) != 0 : (p.flags & bit) != 0;
 }
 
+__device__ __forceinline__ float2 f2(float v) { return make_float2(v, v); }
+
+// sigmoid of a pair; bf16 outputs take the hardware exponential and reciprocal.
+template <typename T>
+__device__ __forceinline__ float2 sigmoid2(float2 x) {
+  if constexpr (sizeof(T) == 2) {
+    const float2 e = __fmul2_rn(x, f2(-1.4426950408889634f));
+    const float2 d = __fadd2_rn(make_float2(ex2_approx(e.x), ex2_approx(e.y)), f2(1.f));
+    return make_float2(rcp_approx(d.x), rcp_approx(d.y));
+  } else {
+    return make_float2(sigmoid<T>(x.x), sigmoid<T>(x.y));
+  }
+}
+
+// A thread's share of a group: NV vectors of VEC channels as fp32 pairs (a single channel has
+// an empty second half).
 template <typename T, int VEC, int NV>
+struct Share {
+  static constexpr int kPairs = (VEC * NV + 1) / 2;
+  using Vec = Pack<T, VEC>;
+  int ch[NV];
+  bool have[NV];
+
+  __device__ __forceinline__ Share(const Args& p, const Place& q) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int k = (q.lane + j * q.width) * VEC;
+      have[j] = q.on && k < p.G;
+      ch[j] = have[j] ? q.group * p.G + k : 0;
+    }
+  }
+  __device__ __forceinline__ void load(const void* t, long long row, long long stride, bool ok, Vec (&raw)[NV]) const {
+    const T* r = static_cast<const T*>(t) + row * stride;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (have[j] && ok)
+        raw[j] = *reinterpret_cast<const Vec*>(r + ch[j]);
+      else
+        raw[j] = Vec{};
+    }
+  }
+  static __device__ __forceinline__ void widen(const Vec (&raw)[NV], float2 (&f)[kPairs]) {
+    if constexpr (VEC == 1) {
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j)
+        f[j] = make_float2(to_f32<T>(raw[2 * j].v[0]), 2 * j + 1 < NV ? to_f32<T>(raw[2 * j + 1 < NV ? 2 * j + 1 : 0].v[0]) : 0.f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < VEC / 2; ++e) {
+          if constexpr (sizeof(T) == 2) {
+            const uint32_t w = reinterpret_cast<const uint32_t*>(&raw[j])[e];
+            f[j * VEC / 2 + e] = make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+          } else {
+            f[j * VEC / 2 + e] = make_float2(raw[j].v[2 * e], raw[j].v[2 * e + 1]);
+          }
+        }
+    }
+  }
+  __device__ __forceinline__ void store(void* t, long long row, int C, bool ok, const float2 (&f)[kPairs]) const {
+    T* r = static_cast<T*>(t) + row * C;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (!(have[j] && ok)) continue;
+      if constexpr (VEC == 1) {
+        r[ch[j]] = from_f32<T>(j & 1 ? f[j / 2].y : f[j / 2].x);
+      } else {
+        Vec v;
+#pragma unroll
+        for (int e = 0; e < VEC / 2; ++e) {
+          const float2 w = f[j * VEC / 2 + e];
+          if constexpr (sizeof(T) == 2)
+            reinterpret_cast<uint32_t*>(&v)[e] = pack_bf16x2(w.x, w.y);
+          else
+            reinterpret_cast<float2*>(&v)[e] = w;
+        }
+        *reinterpret_cast<Vec*>(r + ch[j]) = v;
+      }
+    }
+  }
+  // Element e of vector j in pairs, for the parameters and their gradients.
+  static __device__ __forceinline__ float& at(float2 (&f)[kPairs], int j, int e) {
+    const int k = j * VEC + e;
+    return k & 1 ? f[k / 2].y : f[k / 2].x;
+  }
+  __device__ __forceinline__ void params(const float* t, float absent, float2 (&f)[kPairs]) const {
+#pragma unroll
+    for (int k = 0; k < kPairs; ++k) f[k] = f2(0.f);
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) at(f, j, e) = have[j] ? (t != nullptr ? t[ch[j] + e] : absent) : 0.f;
+  }
+  // Sum of a over the thread's channels.
+  static __device__ __forceinline__ float sum(const float2 (&a)[kPairs]) {
+    float2 s = a[0];
+#pragma unroll
+    for (int k = 1; k < kPairs; ++k) s = __fadd2_rn(s, a[k]);
+    return s.x + s.y;
+  }
+  static __device__ __forceinline__ float dot(const float2 (&a)[kPairs], const float2 (&b)[kPairs]) {
+    float2 s = __fmul2_rn(a[0], b[0]);
+#pragma unroll
+    for (int k = 1; k < kPairs; ++k) s = __ffma2_rn(a[k], b[k], s);
+    return s.x + s.y;
+  }
+  // Take the mean off v where the group is centred (absent channels stay 0); 1 / sqrt(mean of
+  // squares + eps).
+  __device__ __forceinline__ float normalise(float2 (&v)[kPairs], const Args& p, float* sh) const {
+    const float inv = 1.f / (float)p.G;
+    if (p.center) {
+      const float mu = team_sum(sum(v), p.tl, sh) * inv;
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) v[k] = __fadd2_rn(v[k], f2(-mu));
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (!have[j])
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) at(v, j, e) = 0.f;
+      if constexpr (VEC * NV == 1) v[0].y = 0.f;
+    }
+    return rsqrtf(fmaf(team_sum(dot(v, v), p.tl, sh), inv, p.eps));
+  }
+};
+
+// The next row's loads are issued before a row is worked on: a row's arithmetic hides them, and
+// with 16 bytes a thread and tensor in flight three blocks an SM keep HBM busy.
+template <typename T, int VEC, int NV, int FLAGS>
 __global__ void __launch_bounds__(max_threads(VEC)) norm_fwd(const Args p) {
   __shared__ float sh[32];
+  using S = Share<T, VEC, NV>;
+  constexpr int N = S::kPairs;
   const Place q = place(p);
-  int ch[NV];
-  bool have[NV];
-  float w[NV][VEC], b[NV][VEC];
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int k = (q.lane + j * q.width) * VEC;
-    have[j] = q.on && k < p.G;
-    ch[j] = have[j] ? q.group * p.G + k : 0;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      w[j][e] = have[j] && p.w != nullptr ? p.w[ch[j] + e] : 1.f;
-      b[j][e] = have[j] && p.b != nullptr ? p.b[ch[j] + e] : 0.f;
-    }
-  }
+  const S me(p, q);
+  float2 w[N], b[N];
+  me.params(p.w, 1.f, w);
+  me.params(p.b, 0.f, b);
   const long long step = (long long)gridDim.y * p.rpi;
-  for (long long base = (long long)blockIdx.y * p.rpi; base < p.R; base += step) {
-    const long long row = base + q.sub;
-    const bool rowok = row < p.R;
-    float v[NV][VEC], z[NV][VEC];
+  long long row = (long long)blockIdx.y * p.rpi + q.sub;
+  typename S::Vec xr[NV], zr[NV];
+  me.load(p.x, row, p.xs, row < p.R, xr);
+  if (flag<FLAGS>(p, kGate)) me.load(p.z, row, p.zs, row < p.R, zr);
+  for (; row - q.sub < p.R; row += step) {
+    float2 v[N], z[N];
+    S::widen(xr, v);
+    if (flag<FLAGS>(p, kGate)) S::widen(zr, z);
+    const bool more = row + step < p.R;
+    me.load(p.x, row + step, p.xs, more, xr);
+    if (flag<FLAGS>(p, kGate)) me.load(p.z, row + step, p.zs, more, zr);
+    const float rs = me.normalise(v, p, sh);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[j][e] = z[j][e] = 0.f;
-      if (have[j] && rowok) {
-        load_vec<T, VEC>(static_cast<const T*>(p.x) + row * p.xs + ch[j], v[j]);
-        if (p.z != nullptr) load_vec<T, VEC>(static_cast<const T*>(p.z) + row * p.zs + ch[j], z[j]);
+    for (int k = 0; k < N; ++k) {
+      float2 u = __fmul2_rn(v[k], f2(rs));
+      u = flag<FLAGS>(p, kBias) ? __ffma2_rn(u, w[k], b[k]) : __fmul2_rn(u, w[k]);
+      if (flag<FLAGS>(p, kGate)) {
+        if (flag<FLAGS>(p, kAct)) u = __fmul2_rn(u, sigmoid2<T>(z[k]));
+        u = __fmul2_rn(u, z[k]);
+      } else if (flag<FLAGS>(p, kAct)) {
+        u = __fmul2_rn(u, sigmoid2<T>(u));
       }
+      v[k] = u;
     }
-    const float rs = normalise<VEC, NV>(v, have, p, sh);
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if (!(have[j] && rowok)) continue;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        float u = fmaf(v[j][e] * rs, w[j][e], b[j][e]);
-        if (p.z != nullptr)
-          u *= p.act ? silu_of<T>(z[j][e]) : z[j][e];
-        else if (p.act)
-          u = silu_of<T>(u);
-        v[j][e] = u;
-      }
-      store_vec<T, VEC>(static_cast<T*>(p.y) + row * p.C + ch[j], v[j]);
-    }
+    me.store(p.y, row, p.C, row < p.R, v);
   }
 }
 
-template <typename T, int VEC, int NV>
-__global__ void __launch_bounds__(max_threads(VEC)) norm_bwd(const Args p) {
+template <typename T, int VEC, int NV, int FLAGS>
+__global__ void __launch_bounds__(max_threads(VEC), VEC * NV == 8 && sizeof(T) == 2 ? 3 : 1) norm_bwd(const Args p) {
   __shared__ float sh[32];
   extern __shared__ float fold[];  // [rpi][gpc * G] when a block works on several rows
+  using S = Share<T, VEC, NV>;
+  constexpr int N = S::kPairs;
   const Place q = place(p);
+  const S me(p, q);
   const float inv = 1.f / (float)p.G;
-  int ch[NV];
-  bool have[NV];
-  float w[NV][VEC], dw[NV][VEC], db[NV][VEC];
+  float2 w[N], dw[N], db[N];
+  me.params(p.w, 1.f, w);
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int k = (q.lane + j * q.width) * VEC;
-    have[j] = q.on && k < p.G;
-    ch[j] = have[j] ? q.group * p.G + k : 0;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      w[j][e] = have[j] && p.w != nullptr ? p.w[ch[j] + e] : 1.f;
-      dw[j][e] = db[j][e] = 0.f;
-    }
-  }
+  for (int k = 0; k < N; ++k) dw[k] = db[k] = f2(0.f);
   const long long step = (long long)gridDim.y * p.rpi;
-  for (long long base = (long long)blockIdx.y * p.rpi; base < p.R; base += step) {
-    const long long row = base + q.sub;
-    const bool rowok = row < p.R;
-    float v[NV][VEC], d[NV][VEC];
+  long long row = (long long)blockIdx.y * p.rpi + q.sub;
+  typename S::Vec xr[NV], gr[NV], zr[NV];
+  me.load(p.x, row, p.xs, row < p.R, xr);
+  me.load(p.dy, row, p.gs, row < p.R, gr);
+  if (flag<FLAGS>(p, kGate)) me.load(p.z, row, p.zs, row < p.R, zr);
+  for (; row - q.sub < p.R; row += step) {
+    float2 v[N], d[N], z[N];
+    S::widen(xr, v);
+    S::widen(gr, d);
+    if (flag<FLAGS>(p, kGate)) S::widen(zr, z);
+    const bool more = row + step < p.R;
+    me.load(p.x, row + step, p.xs, more, xr);
+    me.load(p.dy, row + step, p.gs, more, gr);
+    if (flag<FLAGS>(p, kGate)) me.load(p.z, row + step, p.zs, more, zr);
+    const float rs = me.normalise(v, p, sh);
+    float2 b[N];
+    if (flag<FLAGS>(p, kBias)) me.params(p.b, 0.f, b);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[j][e] = d[j][e] = 0.f;
-      if (have[j] && rowok) {
-        load_vec<T, VEC>(static_cast<const T*>(p.x) + row * p.xs + ch[j], v[j]);
-        load_vec<T, VEC>(static_cast<const T*>(p.dy) + row * p.gs + ch[j], d[j]);
-      }
-    }
-    const float rs = normalise<VEC, NV>(v, have, p, sh);
-    float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if (!(have[j] && rowok)) continue;
-      float z[VEC];
-      if (p.z != nullptr) load_vec<T, VEC>(static_cast<const T*>(p.z) + row * p.zs + ch[j], z);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float xh = v[j][e] * rs;
-        const float u = fmaf(xh, w[j][e], p.b != nullptr ? p.b[ch[j] + e] : 0.f);
-        float du = d[j][e];
-        if (p.z != nullptr) {
-          float f = z[e], df = 1.f;
-          if (p.act) silu_grad<T>(z[e], f, df);
-          z[e] = du * u * df;
-          du *= f;
-        } else if (p.act) {
-          float f, df;
-          silu_grad<T>(u, f, df);
-          du *= df;
+    for (int k = 0; k < N; ++k) {
+      v[k] = __fmul2_rn(v[k], f2(rs));  // xh
+      const float2 u = flag<FLAGS>(p, kBias) ? __ffma2_rn(v[k], w[k], b[k]) : __fmul2_rn(v[k], w[k]);
+      // du and, with a gate, dz = dy u act'(z); silu'(x) = s (1 + x (1 - s)).
+      float2 du = d[k];
+      if (flag<FLAGS>(p, kGate)) {
+        float2 f = z[k], dz = __fmul2_rn(du, u);
+        if (flag<FLAGS>(p, kAct)) {
+          const float2 s = sigmoid2<T>(f);
+          dz = __fmul2_rn(dz, __fmul2_rn(s, __ffma2_rn(f, __ffma2_rn(s, f2(-1.f), f2(1.f)), f2(1.f))));
+          f = __fmul2_rn(f, s);
         }
-        dw[j][e] = fmaf(du, xh, dw[j][e]);
-        db[j][e] += du;
-        const float dxh = du * w[j][e];
-        s1 += dxh;
-        s2 = fmaf(dxh, xh, s2);
-        v[j][e] = xh;
-        d[j][e] = dxh;
+        z[k] = dz;
+        du = __fmul2_rn(du, f);
+      } else if (flag<FLAGS>(p, kAct)) {
+        const float2 s = sigmoid2<T>(u);
+        du = __fmul2_rn(du, __fmul2_rn(s, __ffma2_rn(u, __ffma2_rn(s, f2(-1.f), f2(1.f)), f2(1.f))));
       }
-      if (p.z != nullptr) store_vec<T, VEC>(static_cast<T*>(p.dz) + row * p.C + ch[j], z);
+      dw[k] = __ffma2_rn(du, v[k], dw[k]);
+      if (flag<FLAGS>(p, kBias)) db[k] = __fadd2_rn(db[k], du);
+      d[k] = __fmul2_rn(du, w[k]);  // dxh
     }
-    const float m1 = p.center ? team_sum(s1, p.tl, sh) * inv : 0.f;
-    const float m2 = team_sum(s2, p.tl, sh) * inv;
+    if (flag<FLAGS>(p, kGate)) me.store(p.dz, row, p.C, row < p.R, z);
+    const float m1 = p.center ? team_sum(S::sum(d), p.tl, sh) * inv : 0.f;
+    const float m2 = team_sum(S::dot(d, v), p.tl, sh) * inv;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if (!(have[j] && rowok)) continue;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) d[j][e] = rs * (d[j][e] - m1 - v[j][e] * m2);
-      store_vec<T, VEC>(static_cast<T*>(p.dx) + row * p.C + ch[j], d[j]);
-    }
+    for (int k = 0; k < N; ++k)
+      d[k] = __fmul2_rn(f2(rs), __ffma2_rn(v[k], f2(-m2), __fadd2_rn(d[k], f2(-m1))));
+    me.store(p.dx, row, p.C, row < p.R, d);
   }
   if (p.part == nullptr) return;
-  // One row of dw and db sums for the block: the block's rows are added in order.
-  const int span = p.gpc * p.G;
-  const int first = blockIdx.x * span;
-  for (int pass = 0; pass < 2; ++pass) {
-    float* out = p.part + ((long long)blockIdx.y * 2 + pass) * p.C;
+  // One row of dw (and db) sums for the block: the block's rows are added in order.
+  const int span = p.gpc * p.G, first = blockIdx.x * span;
+  const int npass = flag<FLAGS>(p, kBias) ? 2 : 1;
+  for (int pass = 0; pass < npass; ++pass) {
+    float* out = p.part + ((long long)blockIdx.y * npass + pass) * p.C;
+    if (pass == 1)
+#pragma unroll
+      for (int k = 0; k < N; ++k) dw[k] = db[k];
     if (p.rpi == 1) {
 #pragma unroll
       for (int j = 0; j < NV; ++j)
-        if (have[j])
+        if (me.have[j])
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) out[ch[j] + e] = pass == 0 ? dw[j][e] : db[j][e];
+          for (int e = 0; e < VEC; ++e) out[me.ch[j] + e] = S::at(dw, j, e);
       continue;
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < NV; ++j)
-      if (have[j])
+      if (me.have[j])
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) fold[q.sub * span + ch[j] - first + e] = pass == 0 ? dw[j][e] : db[j][e];
+        for (int e = 0; e < VEC; ++e) fold[q.sub * span + me.ch[j] - first + e] = S::at(dw, j, e);
     __syncthreads();
     for (int k = threadIdx.x; k < span && first + k < p.C; k += blockDim.x) {
       float acc = 0.f;
@@ -275,6 +365,7 @@ Plan make_plan(Args& p, int elem, const void* const* ptrs, int nptr, int blocks_
   bits |= (uintptr_t)(p.xs * elem) | (uintptr_t)(p.zs * elem) | (uintptr_t)(p.gs * elem);
   for (int k = 0; k < nptr; ++k) bits |= reinterpret_cast<uintptr_t>(ptrs[k]);
   while (q.vec > 1 && (bits & (q.vec * elem - 1)) != 0) q.vec >>= 1;
+  if (q.vec == 4 && elem == 2) q.vec = 2;  // built for 16 bytes, two elements and one
   const int nvec = (p.G + q.vec - 1) / q.vec;
   q.threads = 256;
   if (nvec <= 128) {
@@ -303,17 +394,17 @@ Plan make_plan(Args& p, int elem, const void* const* ptrs, int nptr, int blocks_
   return q;
 }
 
-constexpr int kFwdBlocks = 8, kBwdBlocks = 4;
+constexpr int kFwdBlocks = 4, kBwdBlocks = 3;
 
-template <typename T, int VEC>
+template <typename T, int VEC, int FLAGS>
 void launch(const Plan& q, const Args& p, bool bwd, cudaStream_t st) {
   const size_t fold = bwd && p.part != nullptr && p.rpi > 1 ? sizeof(float) * p.rpi * p.gpc * p.G : 0;
   auto go = [&](auto nv) {
     constexpr int NV = decltype(nv)::value;
     if (bwd)
-      norm_bwd<T, VEC, NV><<<q.grid, q.threads, fold, st>>>(p);
+      norm_bwd<T, VEC, NV, FLAGS><<<q.grid, q.threads, fold, st>>>(p);
     else
-      norm_fwd<T, VEC, NV><<<q.grid, q.threads, 0, st>>>(p);
+      norm_fwd<T, VEC, NV, FLAGS><<<q.grid, q.threads, 0, st>>>(p);
   };
   if (q.nv == 1)
     go(std::integral_constant<int, 1>());
@@ -323,17 +414,30 @@ void launch(const Plan& q, const Args& p, bool bwd, cudaStream_t st) {
     go(std::integral_constant<int, 4>());
 }
 
+template <typename T, int VEC>
+void launch_flags(const Plan& q, const Args& p, bool bwd, cudaStream_t st) {
+  switch (p.flags) {
+    case 0: launch<T, VEC, 0>(q, p, bwd, st); break;
+    case 1: launch<T, VEC, 1>(q, p, bwd, st); break;
+    case 2: launch<T, VEC, 2>(q, p, bwd, st); break;
+    case 3: launch<T, VEC, 3>(q, p, bwd, st); break;
+    case 4: launch<T, VEC, 4>(q, p, bwd, st); break;
+    case 5: launch<T, VEC, 5>(q, p, bwd, st); break;
+    case 6: launch<T, VEC, 6>(q, p, bwd, st); break;
+    default: launch<T, VEC, 7>(q, p, bwd, st); break;
+  }
+}
+
 int dispatch(const Plan& q, const Args& p, int dtype, bool bwd, cudaStream_t st) {
   if (dtype == THM_BF16) {
     using T = __nv_bfloat16;
-    if (q.vec == 8) launch<T, 8>(q, p, bwd, st);
-    else if (q.vec == 4) launch<T, 4>(q, p, bwd, st);
-    else if (q.vec == 2) launch<T, 2>(q, p, bwd, st);
-    else launch<T, 1>(q, p, bwd, st);
+    if (q.vec == 8) launch_flags<T, 8>(q, p, bwd, st);
+    else if (q.vec >= 2) launch<T, 2, -1>(q, p, bwd, st);
+    else launch<T, 1, -1>(q, p, bwd, st);
   } else {
-    if (q.vec == 4) launch<float, 4>(q, p, bwd, st);
-    else if (q.vec == 2) launch<float, 2>(q, p, bwd, st);
-    else launch<float, 1>(q, p, bwd, st);
+    if (q.vec == 4) launch_flags<float, 4>(q, p, bwd, st);
+    else if (q.vec == 2) launch<float, 2, -1>(q, p, bwd, st);
+    else launch<float, 1, -1>(q, p, bwd, st);
   }
   return check_launch();
 }
@@ -349,7 +453,7 @@ int check_sizes(long long R, int C, int G, int act, int dtype) {
 Args make_args(long long R, int C, int G, int center, int act, float eps) {
   Args p{};
   p.R = R; p.C = C; p.G = G; p.groups = C / G;
-  p.center = center != 0; p.act = act == THM_ACT_SILU; p.eps = eps;
+  p.center = center != 0; p.flags = act == THM_ACT_SILU ? kAct : 0; p.eps = eps;
   return p;
 }
 
@@ -366,6 +470,7 @@ extern "C" int thm_group_norm_fwd(const void* x, const void* gate, const float* 
   if (!x || !y) return THM_ERR_INVALID;
   gnorm::Args p = gnorm::make_args(R, C, G, center, activation, eps);
   p.x = x; p.z = gate; p.w = weight; p.b = bias; p.y = y;
+  p.flags |= (gate != nullptr ? gnorm::kGate : 0) | (bias != nullptr ? gnorm::kBias : 0);
   p.xs = x_rs; p.zs = gate != nullptr ? gate_rs : 0;
   const void* ptrs[] = {x, gate, y};
   const gnorm::Plan q = gnorm::make_plan(p, dtype == THM_BF16 ? 2 : 4, ptrs, 3, gnorm::kFwdBlocks);
@@ -390,7 +495,7 @@ extern "C" int thm_group_norm_bwd(const void* x, const void* gate, const float* 
   if (bad != THM_OK) return bad;
   if (C == 0) return THM_OK;
   const bool params = dweight != nullptr || dbias != nullptr;
-  if (params && !workspace) return THM_ERR_INVALID;
+  if ((params && !workspace) || (dbias != nullptr && bias == nullptr)) return THM_ERR_INVALID;
   if (R > 0 && (!x || !dy || !dx || (gate != nullptr) != (dgate != nullptr))) return THM_ERR_INVALID;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   int rows = 0;
@@ -398,6 +503,7 @@ extern "C" int thm_group_norm_bwd(const void* x, const void* gate, const float* 
     gnorm::Args p = gnorm::make_args(R, C, G, center, activation, eps);
     p.x = x; p.z = gate; p.w = weight; p.b = bias; p.dy = dy; p.dx = dx; p.dz = dgate;
     p.part = params ? workspace : nullptr;
+    p.flags |= (gate != nullptr ? gnorm::kGate : 0) | (bias != nullptr ? gnorm::kBias : 0);
     p.xs = x_rs; p.zs = gate != nullptr ? gate_rs : 0; p.gs = dy_rs;
     const void* ptrs[] = {x, gate, dy, dx, dgate};
     const gnorm::Plan q = gnorm::make_plan(p, dtype == THM_BF16 ? 2 : 4, ptrs, 5, gnorm::kBwdBlocks);
@@ -406,7 +512,7 @@ extern "C" int thm_group_norm_bwd(const void* x, const void* gate, const float* 
     rows = (int)q.grid.y;
   }
   if (params) {
-    sum_parts(workspace, rows, 2 * C, gnorm::StoreParams{dweight, dbias, C}, st);
+    sum_parts(workspace, rows, bias != nullptr ? 2 * C : C, gnorm::StoreParams{dweight, dbias, C}, st);
     return check_launch();
   }
   return THM_OK;

@@ -35,6 +35,17 @@ __device__ __forceinline__ void store_vec(T* p, const float* f) {
   *reinterpret_cast<Pack<T, VEC>*>(p) = q;
 }
 
+__device__ __forceinline__ float ex2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // e^x: the hardware exponential where the result is rounded to 16 bits (its error
 // grows as |x| 2^-24), expf where fp32 leaves the kernel.
 template <typename T>
@@ -68,31 +79,31 @@ __device__ __forceinline__ void silu_grad(float x, float& y, float& dy) {
 }
 
 // out[map(c)] = sum over the n rows of part [n, M], column c: the second half of a
-// reduction over all tokens whose first half left one row per block. 8 threads share a
-// column (rows k, k + 8, ... each) and are added in a fixed order, so the result does not
+// reduction over all tokens whose first half left one row per block. 32 threads share a
+// column (rows k, k + 32, ... each) and are added in a fixed order, so the result does not
 // depend on the order in which blocks ran.
 template <typename Map>
-__global__ void __launch_bounds__(256) sum_parts_kernel(const float* __restrict__ part, int n, int M, Map map) {
-  __shared__ float sh[8][33];
+__global__ void __launch_bounds__(1024) sum_parts_kernel(const float* __restrict__ part, int n, int M, Map map) {
+  __shared__ float sh[32][33];
   const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   float acc = 0.f;
   if (c < M) {
-#pragma unroll 4
-    for (int j = k; j < n; j += 8) acc += part[(long long)j * M + c];
+#pragma unroll 8
+    for (int j = k; j < n; j += 32) acc += part[(long long)j * M + c];
   }
   sh[k][lane] = acc;
   __syncthreads();
-  if (k == 0 && c < M) {
+  // Column k's 32 sums, one a lane of warp k.
+  acc = sh[lane][k];
 #pragma unroll
-    for (int j = 1; j < 8; ++j) acc += sh[j][lane];
-    map(c, acc);
-  }
+  for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+  if (lane == 0 && blockIdx.x * 32 + k < M) map(blockIdx.x * 32 + k, acc);
 }
 
 template <typename Map>
 inline void sum_parts(const float* part, int n, int M, Map map, cudaStream_t st) {
-  sum_parts_kernel<<<(M + 31) / 32, 256, 0, st>>>(part, n, M, map);
+  sum_parts_kernel<<<(M + 31) / 32, 1024, 0, st>>>(part, n, M, map);
 }
 
 }  // namespace thm
