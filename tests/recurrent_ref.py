@@ -34,12 +34,12 @@ def assert_within(got, ref, bound, what):
 
 def sigmoid_rel(x, dtype):
     """Relative error of sigmoid(x) = 1 / (1 + e^-x): the exponential's, times 1 - s <= 1 of
-    it that reaches the sum, the sum's and the division's."""
+    it that reaches the sum, the sum's and the reciprocal's (rcp.approx: 1 ulp)."""
     x = np.abs(orc._f64(x))
     x = np.where(np.isfinite(x), x, 0.0)  # sigmoid(+-inf) is exact; NaN stands only where it is not used
     if dtype == torch.bfloat16:
         return (2 * (2 + 1.173 * x) + 1 + 4) * U
-    return np.full(x.shape, 2 + 1 + 1) * U
+    return np.full(x.shape, 2 + 1 + 2) * U
 
 
 def p_floor(dtype):

@@ -113,7 +113,8 @@ def ptr(t) -> int | None:
 def stream_of(t) -> int:
     """Raw cudaStream_t of torch's current stream on the tensor's device."""
     import torch
-    return torch.cuda.current_stream(t.device).cuda_stream
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # 0.2 us; a Stream object costs 2.4
+    return raw(t.device.index) if raw is not None else torch.cuda.current_stream(t.device).cuda_stream
 
 
 def dtype_code(t) -> int:

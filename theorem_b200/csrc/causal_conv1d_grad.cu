@@ -9,6 +9,8 @@
 #include "host_util.h"
 #include "rowops.cuh"
 
+THM_DEFINE_STATUS(g_status_conv_grad)
+
 namespace thm {
 namespace convg {
 
@@ -73,44 +75,42 @@ struct BwdArgs {
   void* dx;
   float* part;  // [blocks, W + 1, D]
   long long xb, xt, gb, gt;
-  int S, D, act, rows;  // rows: of a warp's strip
+  int S, D, rows;  // rows: of a warp's strip, a multiple of kBlockRows
+};
+struct BwdMaps {
+  CUtensorMap x, dy;
 };
 
-constexpr int kWarps = 8, kBlockRows = 4;
+constexpr int kWarps = 8, kBlockRows = 4, kCols = 64;
 
 __device__ __forceinline__ float2 f2(float v) { return make_float2(v, v); }
 
-// VEC channels as fp32 pairs (one channel: an empty second half).
-template <typename T, int VEC>
-__device__ __forceinline__ void widen(const Pack<T, VEC>& q, float2 (&f)[(VEC + 1) / 2]) {
-  if constexpr (VEC == 1) {
-    f[0] = make_float2(to_f32<T>(q.v[0]), 0.f);
+// Two neighbouring channels in shared memory.
+template <typename T>
+__device__ __forceinline__ float2 get_pair(const uint8_t* p) {
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   } else {
-#pragma unroll
-    for (int e = 0; e < VEC / 2; ++e) {
-      if constexpr (sizeof(T) == 2) {
-        const uint32_t w = reinterpret_cast<const uint32_t*>(&q)[e];
-        f[e] = make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-      } else {
-        f[e] = make_float2(q.v[2 * e], q.v[2 * e + 1]);
-      }
-    }
+    return *reinterpret_cast<const float2*>(p);
   }
 }
-template <typename T, int VEC>
-__device__ __forceinline__ void store_pairs(T* p, const float2 (&f)[(VEC + 1) / 2]) {
-  if constexpr (VEC == 1) {
-    *p = from_f32<T>(f[0].x);
+// ... and in global memory, as one access (PAIRED) or as two.
+template <typename T, bool PAIRED>
+__device__ __forceinline__ float2 load_pair(const T* p, bool two) {
+  if constexpr (PAIRED) return get_pair<T>(reinterpret_cast<const uint8_t*>(p));
+  return make_float2(to_f32<T>(p[0]), two ? to_f32<T>(p[1]) : 0.f);
+}
+template <typename T, bool PAIRED>
+__device__ __forceinline__ void store_pair(T* p, float2 f, bool two) {
+  if constexpr (PAIRED) {
+    if constexpr (sizeof(T) == 2)
+      *reinterpret_cast<uint32_t*>(p) = pack_bf16x2(f.x, f.y);
+    else
+      *reinterpret_cast<float2*>(p) = f;
   } else {
-    Pack<T, VEC> q;
-#pragma unroll
-    for (int e = 0; e < VEC / 2; ++e) {
-      if constexpr (sizeof(T) == 2)
-        reinterpret_cast<uint32_t*>(&q)[e] = pack_bf16x2(f[e].x, f[e].y);
-      else
-        reinterpret_cast<float2*>(&q)[e] = f[e];
-    }
-    *reinterpret_cast<Pack<T, VEC>*>(p) = q;
+    p[0] = from_f32<T>(f.x);
+    if (two) p[1] = from_f32<T>(f.y);
   }
 }
 
@@ -128,130 +128,153 @@ __device__ __forceinline__ float2 through_silu(float2 g, float2 u) {
   return __fmul2_rn(g, __fmul2_rn(s, __ffma2_rn(u, __ffma2_rn(s, f2(-1.f), f2(1.f)), f2(1.f))));
 }
 
-// A block has 32 * VEC channels and kWarps strips of rows of one sequence, a strip per
-// warp. A lane walks its strip and W - 1 rows past its end, four rows at a time, the next four
-// in flight: du of row t needs x of rows t - W + 1 .. t, and dx of row t du of rows t .. t + W - 1,
-// so windows of both stay in registers and every row is read once but for the halo. Rows past
-// the strip count for dx only, not for dw and db; rows past the sequence are zeros, whose du is 0.
-template <typename T, int VEC, int W, bool ACT>
-__global__ void __launch_bounds__(32 * kWarps, W <= 4 ? 2 : 1) conv_bwd(const BwdArgs p) {
-  constexpr int NP = (VEC + 1) / 2, RB = kBlockRows;
-  using Raw = Pack<T, VEC>;
-  __shared__ float fold[kWarps][32 * VEC];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = (blockIdx.x * 32 + lane) * VEC;
-  const bool on = c < p.D;
+// A block has 64 channels and 8 strips of rows of one sequence, a strip per warp and two channels
+// a lane. A warp walks its strip and W - 1 rows past its end: du of row t needs x of rows
+// t - W + 1 .. t, and dx of row t du of rows t .. t + W - 1, so windows of both stay in registers, as
+// rings that the unrolled loop indexes, and every row is read once but for the halo. Rows past
+// the strip count for dx only, not for dw and db; rows past the sequence come as zeros, whose du
+// is 0.
+//
+// The rows come by TMA, a ring's worth (8 or 12) of both tensors at a time, into a ring of
+// stages of the warp's own: no block barrier, no address arithmetic, and the bytes in flight
+// take no registers (loads of 4 rows ahead into registers left HBM at a third of its rate).
+// Where addresses or strides are no multiples of 16 bytes (TMA false), the lanes fill their own
+// slots.
+template <typename T, int W>
+struct Bwd {
+  static constexpr int kNB = (W - 1 + 2 * kBlockRows - 1) / kBlockRows;  // blocks of rows in a ring
+  static constexpr int kRing = kNB * kBlockRows;
+  static constexpr int kTile = kRing * kCols * (int)sizeof(T);
+  static constexpr int kStages = sizeof(T) == 2 ? 4 : 2;
+  static constexpr int kBytes = kWarps * kStages * 2 * kTile;
+};
+
+template <typename T, int W, bool ACT, bool TMA>
+__global__ void __launch_bounds__(32 * kWarps, W <= 5 ? 3 : 2)
+    conv_bwd(const __grid_constant__ BwdArgs p, const __grid_constant__ BwdMaps tm) {
+  using C = Bwd<T, W>;
+  constexpr int RB = kBlockRows, RING = C::kRing, NS = C::kStages;
+  extern __shared__ __align__(128) uint8_t stages[];
+  __shared__ float2 fold[kWarps][32];
+  __shared__ __align__(8) uint64_t full[kWarps][NS];
+  const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+  const int c = blockIdx.x * kCols + 2 * lane;
+  const bool on = c < p.D, two = c + 1 < p.D;
   const int t0 = (blockIdx.y * kWarps + warp) * p.rows;
   const int t1 = min(t0 + p.rows, p.S);
+  uint8_t* ring = stages + warp * NS * 2 * C::kTile;
+  if (lane == 0) {
+    for (int k = 0; k < NS; ++k) mbar_init(&full[warp][k], 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
+  const int steps = t0 < t1 ? (t1 - t0 + W - 1 + RING - 1) / RING : 0;
+  bool ok = true;
+  auto ask = [&](int j) {
+    if (j >= steps || !ok) return;
+    uint64_t* bar = &full[warp][j % NS];
+    uint8_t* slot = ring + (j % NS) * 2 * C::kTile;
+    mbar_arrive_expect_tx(bar, 2 * C::kTile);
+    tma_load_3d(slot, &tm.x, bar, blockIdx.x * kCols, t0 + j * RING, blockIdx.z);
+    tma_load_3d(slot + C::kTile, &tm.dy, bar, blockIdx.x * kCols, t0 + j * RING, blockIdx.z);
+  };
+  if (TMA && lane == 0)
+    for (int j = 0; j < NS; ++j) ask(j);
+  float2 w[W], dw[W], b = f2(0.f), db = f2(0.f);
+  if (on) b = make_float2(p.b[c], two ? p.b[c + 1] : 0.f);
+#pragma unroll
+  for (int k = 0; k < W; ++k) {
+    w[k] = on ? make_float2(p.w[(long long)c * W + k], two ? p.w[(long long)(c + 1) * W + k] : 0.f) : f2(0.f);
+    dw[k] = f2(0.f);
+  }
   const T* x = static_cast<const T*>(p.x) + (long long)blockIdx.z * p.xb + c;
   const T* dy = static_cast<const T*>(p.dy) + (long long)blockIdx.z * p.gb + c;
-  T* dx = static_cast<T*>(p.dx) + (long long)blockIdx.z * p.S * p.D + c;
-  float2 w[W][NP], dw[W][NP], b[NP], db[NP], xw[W - 1 + RB][NP], du[W - 1 + RB][NP];
+  T* dx = static_cast<T*>(p.dx) + ((long long)blockIdx.z * p.S + t0 - (W - 1)) * p.D + c;
+  float2 xw[RING], du[RING];  // row t0 + k at k % RING
 #pragma unroll
-  for (int e = 0; e < NP; ++e) {
-    const bool two = VEC > 1;
-    b[e] = on ? make_float2(p.b[c + 2 * e], two ? p.b[c + 2 * e + 1] : 0.f) : f2(0.f);
-    db[e] = f2(0.f);
+  for (int k = 0; k < RING; ++k) xw[k] = du[k] = f2(0.f);
 #pragma unroll
-    for (int k = 0; k < W; ++k) {
-      w[k][e] = on ? make_float2(p.w[(long long)(c + 2 * e) * W + k], two ? p.w[(long long)(c + 2 * e + 1) * W + k] : 0.f)
-                   : f2(0.f);
-      dw[k][e] = f2(0.f);
-    }
-  }
-  if (on && t0 < t1) {
-    const int end = min(t1 + W - 1, p.S);  // rows that there are and that count
-#pragma unroll
-    for (int k = 0; k + 1 < W; ++k) {  // the rows before the strip
-      const int t = t0 - (W - 1) + k;
-      Raw q{};
-      if (t >= 0) q = *reinterpret_cast<const Raw*>(x + t * p.xt);
-      widen<T, VEC>(q, xw[k]);
-#pragma unroll
-      for (int e = 0; e < NP; ++e) du[k][e] = f2(0.f);
-    }
-    Raw xr[RB], gr[RB];
-    auto load = [&](int t) {
-#pragma unroll
-      for (int k = 0; k < RB; ++k) {
-        xr[k] = gr[k] = Raw{};
-        if (t + k < end) {
-          xr[k] = *reinterpret_cast<const Raw*>(x + (t + k) * p.xt);
-          gr[k] = *reinterpret_cast<const Raw*>(dy + (t + k) * p.gt);
+  for (int k = 1; k < W; ++k)  // the rows before the strip
+    if (on && t0 < t1 && t0 - k >= 0) xw[RING - k] = load_pair<T, TMA>(x + (t0 - k) * p.xt, two);
+  for (int j = 0; j < steps; ++j) {
+    const int tb = t0 + j * RING;
+    uint8_t* slot = ring + (j % NS) * 2 * C::kTile + 2 * lane * (int)sizeof(T);
+    if constexpr (TMA) {
+      if (ok) ok = mbar_wait(&full[warp][j % NS], (j / NS) & 1, &g_status_conv_grad);
+    } else {
+      for (int k = 0; k < RING; ++k) {
+        const bool there = on && tb + k < p.S;
+        float2 xv = f2(0.f), gv = f2(0.f);
+        if (there) {
+          xv = load_pair<T, false>(x + (tb + k) * p.xt, two);
+          gv = load_pair<T, false>(dy + (tb + k) * p.gt, two);
         }
+        store_pair<T, true>(reinterpret_cast<T*>(slot + k * kCols * sizeof(T)), xv, true);
+        store_pair<T, true>(reinterpret_cast<T*>(slot + C::kTile + k * kCols * sizeof(T)), gv, true);
       }
-    };
-    load(t0);
-    for (int t = t0; t < t1 + W - 1; t += RB) {
+    }
+#pragma unroll
+    for (int i = 0; i < C::kNB; ++i) {
+      const int t = tb + i * RB, r0 = i * RB + RING;  // ring index of row t
 #pragma unroll
       for (int k = 0; k < RB; ++k) {
-        widen<T, VEC>(xr[k], xw[W - 1 + k]);
-        widen<T, VEC>(gr[k], du[W - 1 + k]);
+        xw[(r0 + k) % RING] = get_pair<T>(slot + (i * RB + k) * kCols * sizeof(T));
+        du[(r0 + k) % RING] = get_pair<T>(slot + C::kTile + (i * RB + k) * kCols * sizeof(T));
       }
-      load(t + RB);
       if constexpr (ACT) {
 #pragma unroll
-        for (int k = 0; k < RB; ++k)
+        for (int k = 0; k < RB; ++k) {
+          float2 u = b;
 #pragma unroll
-          for (int e = 0; e < NP; ++e) {
-            float2 u = b[e];
-#pragma unroll
-            for (int j = 0; j < W; ++j) u = __ffma2_rn(w[j][e], xw[k + j][e], u);
-            du[W - 1 + k][e] = through_silu<T>(du[W - 1 + k][e], u);
-          }
+          for (int l = 0; l < W; ++l) u = __ffma2_rn(w[l], xw[(r0 + k - (W - 1) + l) % RING], u);
+          du[(r0 + k) % RING] = through_silu<T>(du[(r0 + k) % RING], u);
+        }
       }
       if (t < t1) {  // strips are whole blocks of rows, but for the sequence's end
 #pragma unroll
-        for (int k = 0; k < RB; ++k)
+        for (int k = 0; k < RB; ++k) {
+          const float2 g = du[(r0 + k) % RING];
+          db = __fadd2_rn(db, g);
 #pragma unroll
-          for (int e = 0; e < NP; ++e) {
-            db[e] = __fadd2_rn(db[e], du[W - 1 + k][e]);
-#pragma unroll
-            for (int j = 0; j < W; ++j) dw[j][e] = __ffma2_rn(du[W - 1 + k][e], xw[k + j][e], dw[j][e]);
-          }
-      }
-#pragma unroll
-      for (int k = 0; k < RB; ++k) {  // dx of row t + k - (W - 1)
-        const int row = t + k - (W - 1);
-        if (row < t0 || row >= t1) continue;
-        float2 g[NP];
-#pragma unroll
-        for (int e = 0; e < NP; ++e) {
-          g[e] = __fmul2_rn(w[0][e], du[k + W - 1][e]);
-#pragma unroll
-          for (int j = 1; j < W; ++j) g[e] = __ffma2_rn(w[j][e], du[k + W - 1 - j][e], g[e]);
+          for (int l = 0; l < W; ++l) dw[l] = __ffma2_rn(g, xw[(r0 + k - (W - 1) + l) % RING], dw[l]);
         }
-        store_pairs<T, VEC>(dx + (long long)row * p.D, g);
       }
+      float2 g[RB];  // dx of rows t + k - (W - 1)
 #pragma unroll
-      for (int k = 0; k + 1 < W; ++k)
+      for (int k = 0; k < RB; ++k) {
+        g[k] = __fmul2_rn(w[0], du[(r0 + k) % RING]);
 #pragma unroll
-        for (int e = 0; e < NP; ++e) {
-          xw[k][e] = xw[k + RB][e];
-          du[k][e] = du[k + RB][e];
+        for (int l = 1; l < W; ++l) g[k] = __ffma2_rn(w[l], du[(r0 + k - l) % RING], g[k]);
+      }
+      const int row = t - (W - 1);
+      if (on) {
+        if (row >= t0 && row + RB <= t1) {
+#pragma unroll
+          for (int k = 0; k < RB; ++k) store_pair<T, TMA>(dx + (long long)(i * RB + k) * p.D, g[k], two);
+        } else {
+#pragma unroll
+          for (int k = 0; k < RB; ++k)
+            if (row + k >= t0 && row + k < t1) store_pair<T, TMA>(dx + (long long)(i * RB + k) * p.D, g[k], two);
         }
+      }
     }
+    dx += (long long)RING * p.D;
+    __syncwarp();  // the stage has been read
+    if (TMA && lane == 0) ask(j + NS);
   }
   // The strips' sums, added in the order of the rows.
   float* part = p.part + ((long long)blockIdx.z * gridDim.y + blockIdx.y) * (W + 1) * p.D;
 #pragma unroll
   for (int k = 0; k <= W; ++k) {
     __syncthreads();
-#pragma unroll
-    for (int e = 0; e < NP; ++e) {
-      const float2 v = k < W ? dw[k < W ? k : 0][e] : db[e];
-      fold[warp][lane * VEC + 2 * e] = v.x;
-      if constexpr (VEC > 1) fold[warp][lane * VEC + 2 * e + 1] = v.y;
-    }
+    fold[warp][lane] = k < W ? dw[k < W ? k : 0] : db;
     __syncthreads();
-    for (int j = threadIdx.x; j < 32 * VEC; j += 32 * kWarps) {
-      const int col = blockIdx.x * 32 * VEC + j;
-      if (col < p.D) {
-        float acc = 0.f;
+    if (warp == 0 && on) {
+      float2 acc = fold[0][lane];
 #pragma unroll
-        for (int s = 0; s < kWarps; ++s) acc += fold[s][j];
-        part[(long long)k * p.D + col] = acc;
-      }
+      for (int s = 1; s < kWarps; ++s) acc = __fadd2_rn(acc, fold[s][lane]);
+      part[(long long)k * p.D + c] = acc.x;
+      if (two) part[(long long)k * p.D + c + 1] = acc.y;
     }
   }
 }
@@ -268,11 +291,12 @@ struct StoreGrads {
   }
 };
 
-// Rows of a warp's strip.
+// Rows of a warp's strip: long ones, of which the halo is little, where there are enough.
 int strip_rows(int B, int S, int D) {
-  (void)B;
-  (void)D;
-  return S >= 1024 ? 64 : 16;
+  const long long cols = (long long)B * ((D + kCols - 1) / kCols);
+  int rows = 128;
+  while (rows > 16 && cols * ((S + kWarps * rows - 1) / (kWarps * rows)) < 2ll * sm_count()) rows /= 2;
+  return rows;
 }
 
 template <typename F>
@@ -315,22 +339,48 @@ void launch_step(const StepArgs& p, int W, int vec, cudaStream_t st) {
   });
 }
 
-// Channels a lane of the backward kernel takes where vectors fit: its windows and sums of more
-// than 4 taps do not fit the registers for 4.
-constexpr int bwd_vec(int W) { return W <= 4 ? 4 : 2; }
+// x or dy [B, S, D] in boxes of `rows` x 64. A dimension of one entry may have any stride.
+int encode(CUtensorMap* m, int dtype, const void* base, long long bs, long long ts, int B, int S, int D, int rows) {
+  const int elem = dtype == THM_BF16 ? 2 : 4;
+  const uint64_t dims[3] = {(uint64_t)D, (uint64_t)S, (uint64_t)B};
+  const uint64_t ts_b = S > 1 ? (uint64_t)ts * elem : (uint64_t)(D * elem + 15) / 16 * 16;
+  const uint64_t strides[2] = {ts_b, B > 1 ? (uint64_t)bs * elem : ts_b * (uint64_t)S};
+  const uint32_t box[3] = {(uint32_t)kCols, (uint32_t)rows, 1};
+  if (strides[0] == 0 || strides[1] == 0 || strides[0] >= (1ull << 40) || strides[1] >= (1ull << 40))
+    return THM_ERR_UNSUPPORTED;
+  return encode_tiled(m, dtype == THM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3,
+                      base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
 
 template <typename T>
-void launch_bwd(const BwdArgs& p, dim3 grid, int W, int vec, cudaStream_t st) {
+int launch_bwd(const BwdArgs& p, dim3 grid, int B, int W, bool act, int dtype, cudaStream_t st) {
+  const int elem = sizeof(T);
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.dy) |
+                         reinterpret_cast<uintptr_t>(p.dx) | (uintptr_t)(p.D * elem) |
+                         (uintptr_t)((B > 1 ? p.xb | p.gb : 0) * elem) | (uintptr_t)((p.xt | p.gt) * elem);
+  int status = THM_OK;
   with_width(W, [&](auto w) {
-    constexpr int kW = decltype(w)::value, kVec = bwd_vec(kW);
-    auto k = vec > 1 ? (p.act ? conv_bwd<T, kVec, kW, true> : conv_bwd<T, kVec, kW, false>)
-                     : (p.act ? conv_bwd<T, 1, kW, true> : conv_bwd<T, 1, kW, false>);
-    k<<<grid, 32 * kWarps, 0, st>>>(p);
+    constexpr int kW = decltype(w)::value;
+    using C = Bwd<T, kW>;
+    BwdMaps tm{};
+    const bool tma = (bits & 15) == 0 && encode(&tm.x, dtype, p.x, p.xb, p.xt, B, p.S, p.D, C::kRing) == THM_OK &&
+                     encode(&tm.dy, dtype, p.dy, p.gb, p.gt, B, p.S, p.D, C::kRing) == THM_OK;
+    auto k = tma ? (act ? conv_bwd<T, kW, true, true> : conv_bwd<T, kW, false, true>)
+                 : (act ? conv_bwd<T, kW, true, false> : conv_bwd<T, kW, false, false>);
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes) != cudaSuccess) {
+      cudaGetLastError();
+      status = THM_ERR_CUDA;
+      return;
+    }
+    k<<<grid, 32 * kWarps, C::kBytes, st>>>(p, tm);
   });
+  return status != THM_OK ? status : check_launch();
 }
 
 }  // namespace convg
 }  // namespace thm
+
+THM_STATUS_READER(thm_internal_status_conv_grad, g_status_conv_grad)
 
 extern "C" int thm_causal_conv1d_step(const void* x, const void* state, const float* weight, const float* bias,
                                       void* out, void* state_out, long long x_bs, long long x_ts, int B, int S,
@@ -377,22 +427,13 @@ extern "C" int thm_causal_conv1d_bwd(const void* x, const float* weight, const f
   if (parts > 0 && (!x || !dy || !dx || !workspace)) return THM_ERR_INVALID;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (parts > 0) {
-    const int elem = dtype == THM_BF16 ? 2 : 4;
-    const uintptr_t bits = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(dy) |
-                           reinterpret_cast<uintptr_t>(dx) | (uintptr_t)(D * elem) | (uintptr_t)(x_bs * elem) |
-                           (uintptr_t)(x_ts * elem) | (uintptr_t)(dy_bs * elem) | (uintptr_t)(dy_ts * elem);
-    const int vec = convg::vector_of(bits, elem) > 1 ? convg::bwd_vec(W) : 1;
-    const int rows = convg::strip_rows(B, S, D);
     const int blocks_y = parts / B;
     if (blocks_y > 65535) return THM_ERR_UNSUPPORTED;
-    const dim3 grid((D + 32 * vec - 1) / (32 * vec), blocks_y, B);
-    const convg::BwdArgs p{x,     dy,    weight, bias, dx, workspace, x_bs, x_ts, dy_bs, dy_ts, S, D,
-                           activation == THM_ACT_SILU, rows};
-    if (dtype == THM_BF16)
-      convg::launch_bwd<__nv_bfloat16>(p, grid, W, vec, st);
-    else
-      convg::launch_bwd<float>(p, grid, W, vec, st);
-    const int e = check_launch();
+    const dim3 grid((D + convg::kCols - 1) / convg::kCols, blocks_y, B);
+    const convg::BwdArgs p{x, dy, weight, bias, dx, workspace, x_bs, x_ts, dy_bs, dy_ts, S, D, convg::strip_rows(B, S, D)};
+    const bool act = activation == THM_ACT_SILU;
+    const int e = dtype == THM_BF16 ? convg::launch_bwd<__nv_bfloat16>(p, grid, B, W, act, dtype, st)
+                                    : convg::launch_bwd<float>(p, grid, B, W, act, dtype, st);
     if (e != THM_OK) return e;
   }
   sum_parts(workspace, parts, (W + 1) * D, convg::StoreGrads{dweight, dbias, D, W}, st);

@@ -13,6 +13,7 @@
 //   dh0 = a_1 dh_1
 // h_{t-1} is recomputed in fp32 from the state that entered each 64-row chunk, which the
 // forward pass keeps (4 / 64 bytes an element), not read back from the rounded y.
+#include <cmath>
 #include <initializer_list>
 
 #include "host_util.h"
@@ -167,8 +168,8 @@ __device__ __forceinline__ void sigmoids(float2 r, float2 i, float2& s, float2& 
     s = __fmul2_rn(q, B);
     p = __fmul2_rn(q, A);
   } else {
-    s = make_float2(1.f / (1.f + expf(-r.x)), 1.f / (1.f + expf(-r.y)));
-    p = make_float2(1.f / (1.f + expf(-i.x)), 1.f / (1.f + expf(-i.y)));
+    s = make_float2(sigmoid<T>(r.x), sigmoid<T>(r.y));
+    p = make_float2(sigmoid<T>(i.x), sigmoid<T>(i.y));
   }
   if constexpr (!PLAIN) s = make_float2(r.x < kHoldBelow ? 0.f : s.x, r.y < kHoldBelow ? 0.f : s.y);
 }
@@ -771,21 +772,25 @@ int encode(CUtensorMap* m, int dtype, const void* base, long long bs, long long 
 // Up to this many tokens a lane's serial walk beats the tiles.
 constexpr int kDirectTokens = 16;
 
-// Blocks that share a sequence: as many as fit the GPU at once, and no more than a sequence (an
-// average one when packed) has pairs of tiles for. Measured on bf16, forward: B8 T4096 D2048
-// (256 sequences of channels) 127 us alone, 141 with two blocks each, 158 with eight; B1 T131072
-// D2048 2473 us alone, 618 with eight. Where a grid of single blocks leaves less than a second
-// round to fill and sequences are long, halves of them fill it better (B16 T8192: 446 us
-// alone, 426 with two, 476 with four; backward 846, 803, 858).
+// Blocks that share a sequence: as many as fit the GPU at once, and no more than a sequence has
+// pairs of tiles for. Measured on bf16, forward: B8 T4096 D2048 (256 sequences of channels)
+// 127 us alone, 141 with two blocks each, 158 with eight; B1 T131072 D2048 2473 us alone, 618
+// with eight. Where a grid of single blocks leaves less than a second round to fill and sequences
+// are long, halves of them fill it better (B16 T8192: 446 us alone, 426 with two, 476 with four;
+// backward 846, 803, 858). Packed lengths are not known here: the longest of n random pieces
+// has about (1 + ln n) / n of the rows, and the rest of the work fits beside it (65537 rows in 5
+// pieces backward: 902 us alone, 622, 506 and 517 with two, four, eight; 20011 rows in 37 pieces
+// forward fp32: 80, 86, 111, 164).
 int cluster_blocks(int T, int D, int nseq, bool packed, int per_sm) {
-  const long long base = (long long)nseq * ((D + kCols - 1) / kCols);
-  const long long tiles = ((packed ? (T + nseq - 1) / nseq : T) + kChunk - 1) / kChunk;
-  const long long slots = (long long)sm_count() * per_sm;
+  const double cols = (D + kCols - 1) / kCols, longest = packed ? (1. + std::log((double)nseq)) / nseq : 1.;
+  const double base = packed ? cols / longest : cols * nseq, tiles = T * longest / kChunk;
+  const double slots = (double)sm_count() * per_sm;
   if (base > slots) return base < 2 * slots && tiles >= 96 ? 2 : 1;
   int n = 1;
   while (n < 8 && base * n * 2 <= slots && tiles >= 4 * n) n *= 2;
   return n;
 }
+
 int bwd_cluster(int T, int D, int nseq, bool packed, int dtype) {
   return cluster_blocks(T, D, nseq, packed, dtype == THM_BF16 ? Bwd<__nv_bfloat16>::kPerSm : Bwd<float>::kPerSm);
 }

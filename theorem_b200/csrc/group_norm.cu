@@ -37,15 +37,37 @@ struct Args {
 // Sum over the team, the same value in each of its threads.
 __device__ __forceinline__ float team_sum(float v, int tl, float* sh) {
   if (tl != 0) {
-    for (int o = tl >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      if (tl > o) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
   }
+#pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   __syncthreads();  // the previous sum has been read
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
   __syncthreads();
   float s = 0.f;
   for (int k = 0; k < (int)(blockDim.x >> 5); ++k) s += sh[k];
+  return s;
+}
+// Two at a time: their steps overlap, and a block needs one exchange for both.
+__device__ __forceinline__ float2 team_sum2(float2 v, int tl, float2* sh) {
+  if (tl != 0) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      if (tl > o)
+        v = __fadd2_rn(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o)));
+    return v;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    v = __fadd2_rn(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o)));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float2 s = make_float2(0.f, 0.f);
+  for (int k = 0; k < (int)(blockDim.x >> 5); ++k) s = __fadd2_rn(s, sh[k]);
   return s;
 }
 
@@ -66,15 +88,11 @@ __device__ __forceinline__ Place place(const Args& p) {
   return q;
 }
 
-constexpr int max_threads(int vec) { return vec == 1 ? 1024 : vec == 2 ? 512 : 256; }
+// Threads of a block at most: 4096 channels of single elements take 512 threads with eight each.
+constexpr int max_threads(int vec, int nv) { return (vec == 1 && nv == 8) || vec == 2 ? 512 : 256; }
 
-// What a call does besides the norm. The kernels for whole 16-byte vectors have it as a
-// template argument, the narrow ones (FLAGS < 0) look at p.flags.
+// What a call does besides the norm: template arguments of the kernels.
 constexpr int kGate = 1, kAct = 2, kBias = 4;
-template <int FLAGS>
-__device__ __forceinline__ bool flag(const Args& p, int bit) {
-  return FLAGS >= 0 ? (FLAGS & bit) != 0 : (p.flags & bit) != 0;
-}
 
 __device__ __forceinline__ float2 f2(float v) { return make_float2(v, v); }
 
@@ -96,25 +114,21 @@ template <typename T, int VEC, int NV>
 struct Share {
   static constexpr int kPairs = (VEC * NV + 1) / 2;
   using Vec = Pack<T, VEC>;
-  int ch[NV];
+  int c0, step;    // channel of vector j: c0 + j step
   bool have[NV];
 
   __device__ __forceinline__ Share(const Args& p, const Place& q) {
+    c0 = q.on ? q.group * p.G + q.lane * VEC : 0;
+    step = q.width * VEC;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int k = (q.lane + j * q.width) * VEC;
-      have[j] = q.on && k < p.G;
-      ch[j] = have[j] ? q.group * p.G + k : 0;
-    }
+    for (int j = 0; j < NV; ++j) have[j] = q.on && (q.lane + j * q.width) * VEC < p.G;
   }
-  __device__ __forceinline__ void load(const void* t, long long row, long long stride, bool ok, Vec (&raw)[NV]) const {
-    const T* r = static_cast<const T*>(t) + row * stride;
+  // The vectors at t (channel c0 of a row); absent ones, and all where there is no row, are 0.
+  __device__ __forceinline__ void load(const T* t, bool ok, Vec (&raw)[NV]) const {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (have[j] && ok)
-        raw[j] = *reinterpret_cast<const Vec*>(r + ch[j]);
-      else
-        raw[j] = Vec{};
+      raw[j] = Vec{};
+      if (have[j] && ok) raw[j] = *reinterpret_cast<const Vec*>(t + j * step);
     }
   }
   static __device__ __forceinline__ void widen(const Vec (&raw)[NV], float2 (&f)[kPairs]) {
@@ -136,13 +150,12 @@ struct Share {
         }
     }
   }
-  __device__ __forceinline__ void store(void* t, long long row, int C, bool ok, const float2 (&f)[kPairs]) const {
-    T* r = static_cast<T*>(t) + row * C;
+  __device__ __forceinline__ void store(T* r, bool ok, const float2 (&f)[kPairs]) const {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       if (!(have[j] && ok)) continue;
       if constexpr (VEC == 1) {
-        r[ch[j]] = from_f32<T>(j & 1 ? f[j / 2].y : f[j / 2].x);
+        r[j * step] = from_f32<T>(j & 1 ? f[j / 2].y : f[j / 2].x);
       } else {
         Vec v;
 #pragma unroll
@@ -153,7 +166,7 @@ struct Share {
           else
             reinterpret_cast<float2*>(&v)[e] = w;
         }
-        *reinterpret_cast<Vec*>(r + ch[j]) = v;
+        *reinterpret_cast<Vec*>(r + j * step) = v;
       }
     }
   }
@@ -168,7 +181,7 @@ struct Share {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) at(f, j, e) = have[j] ? (t != nullptr ? t[ch[j] + e] : absent) : 0.f;
+      for (int e = 0; e < VEC; ++e) at(f, j, e) = have[j] ? (t != nullptr ? t[c0 + j * step + e] : absent) : 0.f;
   }
   // Sum of a over the thread's channels.
   static __device__ __forceinline__ float sum(const float2 (&a)[kPairs]) {
@@ -205,7 +218,7 @@ struct Share {
 // The next row's loads are issued before a row is worked on: a row's arithmetic hides them, and
 // with 16 bytes a thread and tensor in flight three blocks an SM keep HBM busy.
 template <typename T, int VEC, int NV, int FLAGS>
-__global__ void __launch_bounds__(max_threads(VEC)) norm_fwd(const Args p) {
+__global__ void __launch_bounds__(max_threads(VEC, NV)) norm_fwd(const Args p) {
   __shared__ float sh[32];
   using S = Share<T, VEC, NV>;
   constexpr int N = S::kPairs;
@@ -216,99 +229,114 @@ __global__ void __launch_bounds__(max_threads(VEC)) norm_fwd(const Args p) {
   me.params(p.b, 0.f, b);
   const long long step = (long long)gridDim.y * p.rpi;
   long long row = (long long)blockIdx.y * p.rpi + q.sub;
+  const T *x = static_cast<const T*>(p.x) + row * p.xs + me.c0, *zp = static_cast<const T*>(p.z) + row * p.zs + me.c0;
+  T* y = static_cast<T*>(p.y) + row * p.C + me.c0;
+  const long long xstep = step * p.xs, zstep = step * p.zs, ystep = step * p.C;
   typename S::Vec xr[NV], zr[NV];
-  me.load(p.x, row, p.xs, row < p.R, xr);
-  if (flag<FLAGS>(p, kGate)) me.load(p.z, row, p.zs, row < p.R, zr);
+  me.load(x, row < p.R, xr);
+  if constexpr ((FLAGS & kGate) != 0) me.load(zp, row < p.R, zr);
   for (; row - q.sub < p.R; row += step) {
     float2 v[N], z[N];
     S::widen(xr, v);
-    if (flag<FLAGS>(p, kGate)) S::widen(zr, z);
+    if constexpr ((FLAGS & kGate) != 0) S::widen(zr, z);
     const bool more = row + step < p.R;
-    me.load(p.x, row + step, p.xs, more, xr);
-    if (flag<FLAGS>(p, kGate)) me.load(p.z, row + step, p.zs, more, zr);
+    me.load(x += xstep, more, xr);
+    if constexpr ((FLAGS & kGate) != 0) me.load(zp += zstep, more, zr);
     const float rs = me.normalise(v, p, sh);
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       float2 u = __fmul2_rn(v[k], f2(rs));
-      u = flag<FLAGS>(p, kBias) ? __ffma2_rn(u, w[k], b[k]) : __fmul2_rn(u, w[k]);
-      if (flag<FLAGS>(p, kGate)) {
-        if (flag<FLAGS>(p, kAct)) u = __fmul2_rn(u, sigmoid2<T>(z[k]));
+      u = (FLAGS & kBias) != 0 ? __ffma2_rn(u, w[k], b[k]) : __fmul2_rn(u, w[k]);
+      if constexpr ((FLAGS & kGate) != 0) {
+        if constexpr ((FLAGS & kAct) != 0) u = __fmul2_rn(u, sigmoid2<T>(z[k]));
         u = __fmul2_rn(u, z[k]);
-      } else if (flag<FLAGS>(p, kAct)) {
+      } else if constexpr ((FLAGS & kAct) != 0) {
         u = __fmul2_rn(u, sigmoid2<T>(u));
       }
       v[k] = u;
     }
-    me.store(p.y, row, p.C, row < p.R, v);
+    me.store(y, row < p.R, v);
+    y += ystep;
   }
 }
 
 template <typename T, int VEC, int NV, int FLAGS>
-__global__ void __launch_bounds__(max_threads(VEC), VEC * NV == 8 && sizeof(T) == 2 ? 3 : 1) norm_bwd(const Args p) {
+__global__ void __launch_bounds__(max_threads(VEC, NV), (VEC * NV == 8 && sizeof(T) == 2) || VEC * NV == 4 ? 3 : 1) norm_bwd(const Args p) {
   __shared__ float sh[32];
+  __shared__ float2 sh2[32];
   extern __shared__ float fold[];  // [rpi][gpc * G] when a block works on several rows
   using S = Share<T, VEC, NV>;
   constexpr int N = S::kPairs;
   const Place q = place(p);
   const S me(p, q);
   const float inv = 1.f / (float)p.G;
-  float2 w[N], dw[N], db[N];
+  float2 w[N], b[N], dw[N], db[N];
   me.params(p.w, 1.f, w);
+  if constexpr ((FLAGS & kBias) != 0) me.params(p.b, 0.f, b);
 #pragma unroll
   for (int k = 0; k < N; ++k) dw[k] = db[k] = f2(0.f);
   const long long step = (long long)gridDim.y * p.rpi;
   long long row = (long long)blockIdx.y * p.rpi + q.sub;
+  const T *x = static_cast<const T*>(p.x) + row * p.xs + me.c0, *dy = static_cast<const T*>(p.dy) + row * p.gs + me.c0,
+          *zp = static_cast<const T*>(p.z) + row * p.zs + me.c0;
+  T *dx = static_cast<T*>(p.dx) + row * p.C + me.c0, *dz = static_cast<T*>(p.dz) + row * p.C + me.c0;
+  const long long xstep = step * p.xs, gstep = step * p.gs, zstep = step * p.zs, ostep = step * p.C;
   typename S::Vec xr[NV], gr[NV], zr[NV];
-  me.load(p.x, row, p.xs, row < p.R, xr);
-  me.load(p.dy, row, p.gs, row < p.R, gr);
-  if (flag<FLAGS>(p, kGate)) me.load(p.z, row, p.zs, row < p.R, zr);
+  me.load(x, row < p.R, xr);
+  me.load(dy, row < p.R, gr);
+  if constexpr ((FLAGS & kGate) != 0) me.load(zp, row < p.R, zr);
   for (; row - q.sub < p.R; row += step) {
     float2 v[N], d[N], z[N];
     S::widen(xr, v);
     S::widen(gr, d);
-    if (flag<FLAGS>(p, kGate)) S::widen(zr, z);
+    if constexpr ((FLAGS & kGate) != 0) S::widen(zr, z);
     const bool more = row + step < p.R;
-    me.load(p.x, row + step, p.xs, more, xr);
-    me.load(p.dy, row + step, p.gs, more, gr);
-    if (flag<FLAGS>(p, kGate)) me.load(p.z, row + step, p.zs, more, zr);
+    me.load(x += xstep, more, xr);
+    me.load(dy += gstep, more, gr);
+    if constexpr ((FLAGS & kGate) != 0) me.load(zp += zstep, more, zr);
     const float rs = me.normalise(v, p, sh);
-    float2 b[N];
-    if (flag<FLAGS>(p, kBias)) me.params(p.b, 0.f, b);
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       v[k] = __fmul2_rn(v[k], f2(rs));  // xh
-      const float2 u = flag<FLAGS>(p, kBias) ? __ffma2_rn(v[k], w[k], b[k]) : __fmul2_rn(v[k], w[k]);
+      const float2 u = (FLAGS & kBias) != 0 ? __ffma2_rn(v[k], w[k], b[k]) : __fmul2_rn(v[k], w[k]);
       // du and, with a gate, dz = dy u act'(z); silu'(x) = s (1 + x (1 - s)).
       float2 du = d[k];
-      if (flag<FLAGS>(p, kGate)) {
+      if constexpr ((FLAGS & kGate) != 0) {
         float2 f = z[k], dz = __fmul2_rn(du, u);
-        if (flag<FLAGS>(p, kAct)) {
+        if constexpr ((FLAGS & kAct) != 0) {
           const float2 s = sigmoid2<T>(f);
           dz = __fmul2_rn(dz, __fmul2_rn(s, __ffma2_rn(f, __ffma2_rn(s, f2(-1.f), f2(1.f)), f2(1.f))));
           f = __fmul2_rn(f, s);
         }
         z[k] = dz;
         du = __fmul2_rn(du, f);
-      } else if (flag<FLAGS>(p, kAct)) {
+      } else if constexpr ((FLAGS & kAct) != 0) {
         const float2 s = sigmoid2<T>(u);
         du = __fmul2_rn(du, __fmul2_rn(s, __ffma2_rn(u, __ffma2_rn(s, f2(-1.f), f2(1.f)), f2(1.f))));
       }
       dw[k] = __ffma2_rn(du, v[k], dw[k]);
-      if (flag<FLAGS>(p, kBias)) db[k] = __fadd2_rn(db[k], du);
+      if constexpr ((FLAGS & kBias) != 0) db[k] = __fadd2_rn(db[k], du);
       d[k] = __fmul2_rn(du, w[k]);  // dxh
     }
-    if (flag<FLAGS>(p, kGate)) me.store(p.dz, row, p.C, row < p.R, z);
-    const float m1 = p.center ? team_sum(S::sum(d), p.tl, sh) * inv : 0.f;
-    const float m2 = team_sum(S::dot(d, v), p.tl, sh) * inv;
+    if constexpr ((FLAGS & kGate) != 0) me.store(dz, row < p.R, z);
+    if (p.center) {
+      const float2 m = team_sum2(make_float2(S::sum(d), S::dot(d, v)), p.tl, sh2);
 #pragma unroll
-    for (int k = 0; k < N; ++k)
-      d[k] = __fmul2_rn(f2(rs), __ffma2_rn(v[k], f2(-m2), __fadd2_rn(d[k], f2(-m1))));
-    me.store(p.dx, row, p.C, row < p.R, d);
+      for (int k = 0; k < N; ++k)
+        d[k] = __fmul2_rn(f2(rs), __ffma2_rn(v[k], f2(-m.y * inv), __fadd2_rn(d[k], f2(-m.x * inv))));
+    } else {
+      const float m2 = team_sum(S::dot(d, v), p.tl, sh) * inv;
+#pragma unroll
+      for (int k = 0; k < N; ++k) d[k] = __fmul2_rn(f2(rs), __ffma2_rn(v[k], f2(-m2), d[k]));
+    }
+    me.store(dx, row < p.R, d);
+    dx += ostep;
+    dz += ostep;
   }
   if (p.part == nullptr) return;
   // One row of dw (and db) sums for the block: the block's rows are added in order.
   const int span = p.gpc * p.G, first = blockIdx.x * span;
-  const int npass = flag<FLAGS>(p, kBias) ? 2 : 1;
+  const int npass = (FLAGS & kBias) != 0 ? 2 : 1;
   for (int pass = 0; pass < npass; ++pass) {
     float* out = p.part + ((long long)blockIdx.y * npass + pass) * p.C;
     if (pass == 1)
@@ -319,7 +347,7 @@ __global__ void __launch_bounds__(max_threads(VEC), VEC * NV == 8 && sizeof(T) =
       for (int j = 0; j < NV; ++j)
         if (me.have[j])
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) out[me.ch[j] + e] = S::at(dw, j, e);
+          for (int e = 0; e < VEC; ++e) out[me.c0 + j * me.step + e] = S::at(dw, j, e);
       continue;
     }
     __syncthreads();
@@ -327,7 +355,7 @@ __global__ void __launch_bounds__(max_threads(VEC), VEC * NV == 8 && sizeof(T) =
     for (int j = 0; j < NV; ++j)
       if (me.have[j])
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) fold[q.sub * span + me.ch[j] - first + e] = S::at(dw, j, e);
+        for (int e = 0; e < VEC; ++e) fold[q.sub * span + me.c0 + j * me.step - first + e] = S::at(dw, j, e);
     __syncthreads();
     for (int k = threadIdx.x; k < span && first + k < p.C; k += blockDim.x) {
       float acc = 0.f;
@@ -365,25 +393,28 @@ Plan make_plan(Args& p, int elem, const void* const* ptrs, int nptr, int blocks_
   bits |= (uintptr_t)(p.xs * elem) | (uintptr_t)(p.zs * elem) | (uintptr_t)(p.gs * elem);
   for (int k = 0; k < nptr; ++k) bits |= reinterpret_cast<uintptr_t>(ptrs[k]);
   while (q.vec > 1 && (bits & (q.vec * elem - 1)) != 0) q.vec >>= 1;
-  if (q.vec == 4 && elem == 2) q.vec = 2;  // built for 16 bytes, two elements and one
+  if (q.vec * elem < 16 && q.vec > 2) q.vec = 2;  // built for 16 bytes, two elements and one
   const int nvec = (p.G + q.vec - 1) / q.vec;
+  // Whole 16-byte vectors: a lane has one, so that more lanes have loads in flight, and never more
+  // than 16 channels, whose sums and parameters fit its registers. Narrow ones: a lane has four,
+  // because their sums across lanes cost more than their loads.
+  const bool wide = q.vec * elem == 16;
+  const int most = wide ? 16 / q.vec : 4;  // vectors of a lane
   q.threads = 256;
-  if (nvec <= 128) {
+  if (nvec <= 32 * most) {
     p.tl = 1;
-    while (p.tl < 32 && p.tl < nvec) p.tl <<= 1;
+    while (p.tl < 32 && p.tl * (wide ? 1 : 4) < nvec) p.tl <<= 1;
     q.nv = (nvec + p.tl - 1) / p.tl;
-    q.nv = q.nv > 2 ? 4 : q.nv;
+    q.nv = !wide || q.nv > 2 ? 4 : q.nv;
     const int teams = q.threads / p.tl;
     p.gpc = teams < p.groups ? teams : p.groups;
     p.rpi = teams / p.gpc;
   } else {
     p.tl = 0;
     p.gpc = p.rpi = 1;
-    const int cap = max_threads(q.vec);
-    q.nv = 1;
-    while (q.nv < 4 && nvec > 256 * q.nv) q.nv <<= 1;
+    q.nv = wide ? 1 : q.vec == 2 ? 4 : 8;
+    while (wide && nvec > 256 * q.nv) q.nv <<= 1;
     q.threads = ((nvec + q.nv - 1) / q.nv + 31) / 32 * 32;
-    if (q.threads > cap) q.threads = cap;
   }
   const int gx = (p.groups + p.gpc - 1) / p.gpc;
   const long long need = (p.R + p.rpi - 1) / p.rpi;
@@ -396,48 +427,42 @@ Plan make_plan(Args& p, int elem, const void* const* ptrs, int nptr, int blocks_
 
 constexpr int kFwdBlocks = 4, kBwdBlocks = 3;
 
-template <typename T, int VEC, int FLAGS>
+template <typename T, int VEC, int NV, int FLAGS>
 void launch(const Plan& q, const Args& p, bool bwd, cudaStream_t st) {
   const size_t fold = bwd && p.part != nullptr && p.rpi > 1 ? sizeof(float) * p.rpi * p.gpc * p.G : 0;
-  auto go = [&](auto nv) {
-    constexpr int NV = decltype(nv)::value;
-    if (bwd)
-      norm_bwd<T, VEC, NV, FLAGS><<<q.grid, q.threads, fold, st>>>(p);
-    else
-      norm_fwd<T, VEC, NV, FLAGS><<<q.grid, q.threads, 0, st>>>(p);
-  };
-  if (q.nv == 1)
-    go(std::integral_constant<int, 1>());
-  else if (q.nv == 2)
-    go(std::integral_constant<int, 2>());
+  if (bwd)
+    norm_bwd<T, VEC, NV, FLAGS><<<q.grid, q.threads, fold, st>>>(p);
   else
-    go(std::integral_constant<int, 4>());
+    norm_fwd<T, VEC, NV, FLAGS><<<q.grid, q.threads, 0, st>>>(p);
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, int NV>
 void launch_flags(const Plan& q, const Args& p, bool bwd, cudaStream_t st) {
   switch (p.flags) {
-    case 0: launch<T, VEC, 0>(q, p, bwd, st); break;
-    case 1: launch<T, VEC, 1>(q, p, bwd, st); break;
-    case 2: launch<T, VEC, 2>(q, p, bwd, st); break;
-    case 3: launch<T, VEC, 3>(q, p, bwd, st); break;
-    case 4: launch<T, VEC, 4>(q, p, bwd, st); break;
-    case 5: launch<T, VEC, 5>(q, p, bwd, st); break;
-    case 6: launch<T, VEC, 6>(q, p, bwd, st); break;
-    default: launch<T, VEC, 7>(q, p, bwd, st); break;
+    case 0: launch<T, VEC, NV, 0>(q, p, bwd, st); break;
+    case 1: launch<T, VEC, NV, 1>(q, p, bwd, st); break;
+    case 2: launch<T, VEC, NV, 2>(q, p, bwd, st); break;
+    case 3: launch<T, VEC, NV, 3>(q, p, bwd, st); break;
+    case 4: launch<T, VEC, NV, 4>(q, p, bwd, st); break;
+    case 5: launch<T, VEC, NV, 5>(q, p, bwd, st); break;
+    case 6: launch<T, VEC, NV, 6>(q, p, bwd, st); break;
+    default: launch<T, VEC, NV, 7>(q, p, bwd, st); break;
   }
 }
 
-int dispatch(const Plan& q, const Args& p, int dtype, bool bwd, cudaStream_t st) {
-  if (dtype == THM_BF16) {
-    using T = __nv_bfloat16;
-    if (q.vec == 8) launch_flags<T, 8>(q, p, bwd, st);
-    else if (q.vec >= 2) launch<T, 2, -1>(q, p, bwd, st);
-    else launch<T, 1, -1>(q, p, bwd, st);
+template <typename T>
+int dispatch(const Plan& q, const Args& p, bool bwd, cudaStream_t st) {
+  constexpr int kWide = 16 / sizeof(T);
+  if (q.vec == kWide) {
+    if (q.nv == 1) launch_flags<T, kWide, 1>(q, p, bwd, st);
+    else if (q.nv == 2) launch_flags<T, kWide, 2>(q, p, bwd, st);
+    else if constexpr (sizeof(T) == 4) launch_flags<T, kWide, 4>(q, p, bwd, st);
+  } else if (q.vec == 2) {
+    launch_flags<T, 2, 4>(q, p, bwd, st);
+  } else if (q.nv == 4) {
+    launch_flags<T, 1, 4>(q, p, bwd, st);
   } else {
-    if (q.vec == 4) launch_flags<float, 4>(q, p, bwd, st);
-    else if (q.vec == 2) launch<float, 2, -1>(q, p, bwd, st);
-    else launch<float, 1, -1>(q, p, bwd, st);
+    launch_flags<T, 1, 8>(q, p, bwd, st);
   }
   return check_launch();
 }
@@ -474,7 +499,8 @@ extern "C" int thm_group_norm_fwd(const void* x, const void* gate, const float* 
   p.xs = x_rs; p.zs = gate != nullptr ? gate_rs : 0;
   const void* ptrs[] = {x, gate, y};
   const gnorm::Plan q = gnorm::make_plan(p, dtype == THM_BF16 ? 2 : 4, ptrs, 3, gnorm::kFwdBlocks);
-  return gnorm::dispatch(q, p, dtype, false, reinterpret_cast<cudaStream_t>(stream));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return dtype == THM_BF16 ? gnorm::dispatch<__nv_bfloat16>(q, p, false, st) : gnorm::dispatch<float>(q, p, false, st);
 }
 
 // Rows of the workspace [rows, 2, C] that thm_group_norm_bwd may use at most.
@@ -507,7 +533,7 @@ extern "C" int thm_group_norm_bwd(const void* x, const void* gate, const float* 
     p.xs = x_rs; p.zs = gate != nullptr ? gate_rs : 0; p.gs = dy_rs;
     const void* ptrs[] = {x, gate, dy, dx, dgate};
     const gnorm::Plan q = gnorm::make_plan(p, dtype == THM_BF16 ? 2 : 4, ptrs, 5, gnorm::kBwdBlocks);
-    const int e = gnorm::dispatch(q, p, dtype, true, st);
+    const int e = dtype == THM_BF16 ? gnorm::dispatch<__nv_bfloat16>(q, p, true, st) : gnorm::dispatch<float>(q, p, true, st);
     if (e != THM_OK) return e;
     rows = (int)q.grid.y;
   }

@@ -36,6 +36,7 @@ int thm_internal_status_h(unsigned* s, int reset);
 int thm_internal_status_o(unsigned* s, int reset);
 int thm_internal_status_ho(unsigned* s, int reset);
 int thm_internal_status_scan(unsigned* s, int reset);
+int thm_internal_status_conv_grad(unsigned* s, int reset);
 int thm_internal_status_selftest(unsigned* s, int reset);
 
 // Reads (optionally clears) a TU's status symbol.

@@ -56,14 +56,10 @@ __device__ __forceinline__ float exp_for(float x) {
     return expf(x);
 }
 
-// 1 / (1 + e^-x): 0 at -inf, 1 at +inf, NaN for NaN.
+// 1 / (1 + e^-x): 0 at -inf, 1 at +inf, NaN for NaN. The reciprocal is off by 1 ulp at most.
 template <typename T>
 __device__ __forceinline__ float sigmoid(float x) {
-  const float d = 1.f + exp_for<T>(-x);
-  if constexpr (sizeof(T) == 2)
-    return __fdividef(1.f, d);
-  else
-    return 1.f / d;
+  return rcp_approx(1.f + exp_for<T>(-x));
 }
 
 // silu(x) = x s and silu'(x) = s (1 + x (1 - s)), s = sigmoid(x).

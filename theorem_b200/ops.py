@@ -23,7 +23,9 @@ def _on_input_device(fn):
     the caller's current device is another GPU."""
     @functools.wraps(fn)
     def wrapped(*args, **kw):
-        t = next((a for a in args if torch.is_tensor(a)), None)
+        t = args[0] if args else None
+        if not isinstance(t, torch.Tensor):
+            t = next((a for a in (*args, *kw.values()) if torch.is_tensor(a)), None)
         if t is not None and t.is_cuda and t.device.index != torch.cuda.current_device():
             with torch.cuda.device(t.device):
                 return fn(*args, **kw)
@@ -340,48 +342,49 @@ def chunk_local_cumsum(g_inc, scale: float = 1.0, out=None):
 # ---------------------------------------------------------------------------
 # Recurrent block: gated scan, group norm, the conv's carried-state form and gradients
 # ---------------------------------------------------------------------------
-def _same(ref, **ts):
-    """Each given tensor has ref's shape, dtype and device."""
-    for name, t in ts.items():
-        if t is not None:
-            assert t.shape == ref.shape and t.dtype == ref.dtype and t.device == ref.device, \
-                f"{name} must be {tuple(ref.shape)} {ref.dtype} on {ref.device}"
+# These calls serve single tokens too, where the launch takes 2 to 3 us on the GPU and the host
+# sets the pace: the checks are plain comparisons, and messages are only formed on failure.
+def _like(name, t, ref):
+    """t has ref's shape, dtype and device, and unit stride over channels."""
+    assert t.shape == ref.shape and t.dtype == ref.dtype and t.device == ref.device, \
+        f"{name} must be {tuple(ref.shape)} {ref.dtype} on {ref.device}"
+    assert t.shape[-1] <= 1 or t.stride(-1) == 1, f"{name} must have unit stride over channels"
 
 
-def _dense(ref, shape, dtype, **ts):
-    """Each given tensor is a contiguous ``shape`` of ``dtype`` on ref's device."""
-    for name, t in ts.items():
-        if t is not None:
-            assert t.shape == tuple(shape) and t.dtype == dtype and t.device == ref.device and t.is_contiguous(), \
-                f"{name} must be a contiguous {tuple(shape)} {dtype} on {ref.device}"
+def _dense(name, t, ref, shape, dtype):
+    """t is a contiguous ``shape`` of ``dtype`` on ref's device."""
+    assert t.shape == shape and t.dtype == dtype and t.device == ref.device and t.is_contiguous(), \
+        f"{name} must be a contiguous {tuple(shape)} {dtype} on {ref.device}"
 
 
-def _unit_channels(**ts):
-    for name, t in ts.items():
-        if t is not None:
-            assert t.shape[-1] <= 1 or t.stride(-1) == 1, f"{name} must have unit stride over channels"
+def _empty(ref, shape, dtype):
+    """An uninitialised contiguous tensor on ref's device (empty_like is the cheaper call)."""
+    if ref.shape == shape and ref.dtype == dtype and ref.is_contiguous():
+        return torch.empty_like(ref)
+    return torch.empty(shape, dtype=dtype, device=ref.device)
 
 
-def _float_in(x):
+def _channel_last(x, what):
     assert x.dtype in (torch.float32, torch.bfloat16), f"unsupported dtype {x.dtype} (float32 or bfloat16)"
+    assert x.shape[-1] <= 1 or x.stride(-1) == 1, f"{what} must have unit stride over channels"
 
 
 def _scan_args(x, r, i, decay, cu_seqlens):
+    """(B, T, D, sequences, shape of the chunk states)."""
     _cuda(x, r, i, decay, cu_seqlens)
     assert x.dim() == 3, "x must be [B, T, D]"
-    _float_in(x)
-    _same(x, r=r, i=i)
-    _unit_channels(x=x, r=r, i=i)
+    _channel_last(x, "x")
+    _like("r", r, x)
+    _like("i", i, x)
     B, T, D = x.shape
-    _dense(x, (D,), torch.float32, decay=decay)
-    n = B
-    if cu_seqlens is not None:
-        assert B == 1, "packed sequences share one batch entry: x must be [1, T, D]"
-        assert cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 2, "cu_seqlens must hold N + 1 >= 2 row offsets"
-        n = cu_seqlens.numel() - 1
-        _dense(x, (n + 1,), torch.int32, cu_seqlens=cu_seqlens)
-    slots = T // BT + n if cu_seqlens is not None else (T + BT - 1) // BT
-    return B, T, D, n, (B, slots, D)
+    _dense("decay", decay, x, (D,), torch.float32)
+    if cu_seqlens is None:
+        return B, T, D, B, (B, (T + BT - 1) // BT, D)
+    assert B == 1, "packed sequences share one batch entry: x must be [1, T, D]"
+    assert cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 2, "cu_seqlens must hold N + 1 >= 2 row offsets"
+    n = cu_seqlens.numel() - 1
+    _dense("cu_seqlens", cu_seqlens, x, (n + 1,), torch.int32)
+    return B, T, D, n, (B, T // BT + n, D)
 
 
 @_on_input_device
@@ -406,12 +409,19 @@ def gated_scan(x, r, i, decay, h0=None, cu_seqlens=None, want_states: bool = Fal
     [1, T // 64 + N, D] and unused slots are 0.
     """
     B, T, D, n, sshape = _scan_args(x, r, i, decay, cu_seqlens)
-    _dense(x, (n, D), torch.float32, h0=h0, final=final)
-    _dense(x, x.shape, x.dtype, y=y)
+    if h0 is not None:
+        _cuda(h0)
+        _dense("h0", h0, x, (n, D), torch.float32)
     fresh = y is None
     if fresh:
-        y = torch.empty(B, T, D, device=x.device, dtype=x.dtype)
-    if final is None:
+        y = _empty(x, x.shape, x.dtype)
+    else:
+        _dense("y", y, x, x.shape, x.dtype)
+    if final is not None:
+        _dense("final", final, x, (n, D), torch.float32)
+    elif h0 is not None:
+        final = torch.empty_like(h0)
+    else:
         final = torch.empty(n, D, device=x.device, dtype=torch.float32)
     states = None
     if want_states:
@@ -436,15 +446,18 @@ def gated_scan_bwd(x, r, i, decay, states, dy, dfinal=None, cu_seqlens=None, dx=
     """
     B, T, D, n, sshape = _scan_args(x, r, i, decay, cu_seqlens)
     _cuda(states, dy, dfinal)
-    _same(x, dy=dy)
-    _unit_channels(dy=dy)
-    _dense(x, sshape, torch.float32, states=states)
-    _dense(x, (n, D), torch.float32, dfinal=dfinal)
-    _dense(x, x.shape, x.dtype, dx=dx, dr=dr, di=di)
-    given = [t is not None for t in (dx, dr, di)]
-    assert all(given) or not any(given), "dx, dr, di are given together or not at all"
-    if not given[0]:
-        dx, dr, di = (torch.empty(B, T, D, device=x.device, dtype=x.dtype) for _ in range(3))
+    _like("dy", dy, x)
+    _dense("states", states, x, sshape, torch.float32)
+    if dfinal is not None:
+        _dense("dfinal", dfinal, x, (n, D), torch.float32)
+    outs = (dx, dr, di)
+    fresh = all(t is None for t in outs)
+    assert fresh or all(t is not None for t in outs), "dx, dr, di are given together or not at all"
+    if fresh:
+        dx, dr, di = (_empty(x, x.shape, x.dtype) for _ in range(3))
+    else:
+        for name, t in zip(("dx", "dr", "di"), outs):
+            _dense(name, t, x, x.shape, x.dtype)
     ddecay = torch.empty(D, device=x.device, dtype=torch.float32)
     dh0 = torch.empty(n, D, device=x.device, dtype=torch.float32)
     parts = L.load().thm_gated_scan_bwd_parts(T, D, n, int(cu_seqlens is not None), L.dtype_code(x))
@@ -453,30 +466,37 @@ def gated_scan_bwd(x, r, i, decay, states, dy, dfinal=None, cu_seqlens=None, dx=
                                         L.ptr(dfinal), L.ptr(cu_seqlens), L.ptr(dx), L.ptr(dr), L.ptr(di),
                                         L.ptr(ddecay), L.ptr(dh0), L.ptr(work), x.stride(0), x.stride(1), r.stride(0),
                                         r.stride(1), i.stride(0), i.stride(1), dy.stride(0), dy.stride(1), B, T, D, n,
-                                        int(not given[0]), L.dtype_code(x), L.stream_of(x)), "thm_gated_scan_bwd")
+                                        int(fresh), L.dtype_code(x), L.stream_of(x)), "thm_gated_scan_bwd")
     return dx, dr, di, ddecay, dh0
 
 
 def _rows(name, t):
     """(rows, row stride) of a [..., C] tensor whose leading dimensions collapse to one."""
-    _unit_channels(**{name: t})
+    C = t.shape[-1]
+    if t.is_contiguous():
+        return (t.numel() // C if C else 0), C
     rows, stride = 1, None
     for size, st in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
         if size != 1:
-            assert stride is None or rows == 0 or st == stride * rows, f"{name}'s leading dimensions must collapse to rows"
+            assert stride is None or rows == 0 or st == stride * rows, \
+                f"{name}'s leading dimensions must collapse to rows"
             stride = st if stride is None else stride
         rows *= size
-    return rows, (t.shape[-1] if stride is None else stride)
+    return rows, (C if stride is None else stride)
 
 
 def _norm_args(x, group, weight, bias, gate, activation):
     _cuda(x, weight, bias, gate)
     assert x.dim() >= 1, "x must be [..., C]"
-    _float_in(x)
-    _same(x, gate=gate)
+    _channel_last(x, "x")
     C = x.shape[-1]
     assert group >= 1 and C % group == 0, f"C={C} is not a multiple of the group size {group}"
-    _dense(x, (C,), torch.float32, weight=weight, bias=bias)
+    if gate is not None:
+        _like("gate", gate, x)
+    if weight is not None:
+        _dense("weight", weight, x, (C,), torch.float32)
+    if bias is not None:
+        _dense("bias", bias, x, (C,), torch.float32)
     assert activation in _ACT, f"unknown activation {activation!r}"
     return C
 
@@ -498,9 +518,10 @@ def group_norm(x, group: int, weight=None, bias=None, gate=None, activation=None
     C = _norm_args(x, group, weight, bias, gate, activation)
     R, xs = _rows("x", x)
     zs = _rows("gate", gate)[1] if gate is not None else 0
-    _dense(x, x.shape, x.dtype, out=out)
     if out is None:
-        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        out = _empty(x, x.shape, x.dtype)
+    else:
+        _dense("out", out, x, x.shape, x.dtype)
     L.check(L.load().thm_group_norm_fwd(L.ptr(x), L.ptr(gate), L.ptr(weight), L.ptr(bias), L.ptr(out), xs, zs, R, C,
                                         int(group), int(bool(center)), _ACT[activation], float(eps), L.dtype_code(x),
                                         L.stream_of(x)), "thm_group_norm_fwd")
@@ -517,13 +538,13 @@ def group_norm_bwd(x, dy, group: int, weight=None, bias=None, gate=None, activat
     """
     C = _norm_args(x, group, weight, bias, gate, activation)
     _cuda(dy)
-    _same(x, dy=dy)
+    _like("dy", dy, x)
     R, xs = _rows("x", x)
     gs = _rows("dy", dy)[1]
     zs = _rows("gate", gate)[1] if gate is not None else 0
     dev = x.device
-    dx = torch.empty(x.shape, device=dev, dtype=x.dtype)
-    dgate = torch.empty(x.shape, device=dev, dtype=x.dtype) if gate is not None else None
+    dx = _empty(x, x.shape, x.dtype)
+    dgate = _empty(x, x.shape, x.dtype) if gate is not None else None
     dweight = torch.empty(C, device=dev, dtype=torch.float32) if weight is not None else None
     dbias = torch.empty(C, device=dev, dtype=torch.float32) if bias is not None else None
     work = None
@@ -539,13 +560,12 @@ def group_norm_bwd(x, dy, group: int, weight=None, bias=None, gate=None, activat
 def _conv_args(x, weight, bias, activation):
     _cuda(x, weight, bias)
     assert x.dim() == 3, "x must be [B, S, D]"
-    _float_in(x)
-    _unit_channels(x=x)
+    _channel_last(x, "x")
     B, S, D = x.shape
     assert weight.dim() == 2 and weight.shape[1] >= 1, "weight must be [D, W]"
     W = weight.shape[1]
-    _dense(x, (D, W), torch.float32, weight=weight)
-    _dense(x, (D,), torch.float32, bias=bias)
+    _dense("weight", weight, x, (D, W), torch.float32)
+    _dense("bias", bias, x, (D,), torch.float32)
     assert activation in _ACT, f"unknown activation {activation!r}"
     return B, S, D, W
 
@@ -563,12 +583,15 @@ def causal_conv1d_step(x, state, weight, bias, activation=None, out=None, state_
     B, S, D, W = _conv_args(x, weight, bias, activation)
     assert S <= 64, f"S={S}: the carried-state form takes at most 64 tokens (causal_conv1d takes long runs)"
     _cuda(state)
-    _dense(x, (B, W - 1, D), x.dtype, state=state, state_out=state_out)
-    _dense(x, x.shape, x.dtype, out=out)
+    _dense("state", state, x, (B, W - 1, D), x.dtype)
     if out is None:
-        out = torch.empty(B, S, D, device=x.device, dtype=x.dtype)
+        out = _empty(x, x.shape, x.dtype)
+    else:
+        _dense("out", out, x, x.shape, x.dtype)
     if state_out is None:
         state_out = torch.empty_like(state)
+    else:
+        _dense("state_out", state_out, x, (B, W - 1, D), x.dtype)
     L.check(L.load().thm_causal_conv1d_step(L.ptr(x), L.ptr(state), L.ptr(weight), L.ptr(bias), L.ptr(out),
                                             L.ptr(state_out), x.stride(0), x.stride(1), B, S, D, W, L.dtype_code(x),
                                             _ACT[activation], L.stream_of(x)), "thm_causal_conv1d_step")
@@ -585,9 +608,8 @@ def causal_conv1d_bwd(x, weight, bias, dy, activation=None):
     """
     B, S, D, W = _conv_args(x, weight, bias, activation)
     _cuda(dy)
-    _same(x, dy=dy)
-    _unit_channels(dy=dy)
-    dx = torch.empty(B, S, D, device=x.device, dtype=x.dtype)
+    _like("dy", dy, x)
+    dx = _empty(x, x.shape, x.dtype)
     dweight = torch.empty(D, W, device=x.device, dtype=torch.float32)
     dbias = torch.empty(D, device=x.device, dtype=torch.float32)
     parts = L.load().thm_causal_conv1d_bwd_parts(B, S, D)
