@@ -328,9 +328,12 @@ __device__ __forceinline__ float2 apply(float4 m, float2 h) {
   return __ffma2_rn(make_float2(m.x, m.y), h, make_float2(m.z, m.w));
 }
 
-// What the blocks of a cluster tell each other about a round: a map each, double-buffered.
-// A block sends round j + 2 only after it has all of round j + 1, and each block sends round
-// j + 1 after a block barrier that follows its reads of round j: no map is overwritten unread.
+// What the blocks of a cluster tell each other about a round: a map each, DEPTH rounds deep.
+// A block that receives round j right after sending it sends round j + 2 only after it
+// has all of round j + 1, which each block sends after a block barrier that follows its reads of
+// round j: 2 are enough. One that receives a round behind sends round j + 2 once it has
+// round j, which a block sends before it reads round j - 1: 4 rounds are in use.
+template <int DEPTH>
 struct Exchange {
   float4 (*slots)[8][32];
   uint64_t* bar;
@@ -340,8 +343,7 @@ struct Exchange {
       : slots(s), bar(b), nblk(n), rank(r), ok(true) {
     if (nblk > 1) {
       if (threadIdx.x == 0) {
-        mbar_init(&bar[0], 1);
-        mbar_init(&bar[1], 1);
+        for (int k = 0; k < DEPTH; ++k) mbar_init(&bar[k], 1);
         fence_mbar_init();
       }
       cluster_barrier();  // every block of the cluster runs, its barriers set up, before one sends
@@ -349,7 +351,7 @@ struct Exchange {
   }
   // One warp: send this block's map of round j to every block.
   __device__ __forceinline__ void send(int j, float4 m) {
-    const int lane = threadIdx.x & 31, par = j & 1;
+    const int lane = threadIdx.x & 31, par = j % DEPTH;
     if (lane == 0) mbar_arrive_expect_tx(&bar[par], nblk * 32 * (int)sizeof(float4));
     const uint32_t slot = smem_u32(&slots[par][rank][lane]), b = smem_u32(&bar[par]);
     for (int k = 0; k < nblk; ++k) {
@@ -365,8 +367,8 @@ struct Exchange {
   // All threads: the state that enters this block's tile of round j, and in `carry` the one
   // that enters the next round.
   __device__ __forceinline__ float2 receive(int j, float2& carry, unsigned* status) {
-    const int lane = threadIdx.x & 31, par = j & 1;
-    if (ok) ok = mbar_wait(&bar[par], (j >> 1) & 1, status);
+    const int lane = threadIdx.x & 31, par = j % DEPTH;
+    if (ok) ok = mbar_wait(&bar[par], (j / DEPTH) & 1, status);
     float2 mine = carry;
     for (int k = 0; k < nblk; ++k) {
       if (k == rank) mine = carry;
@@ -424,11 +426,13 @@ __device__ __forceinline__ void fill(uint8_t* tile, const void* t, long long fir
   for (int k = 0; k < rows; ++k) put_pair<T>(tile, k, load_pair<T, false>(q + k * stride, two).get());
 }
 
-// Stages, and resident blocks an SM: three of 80 registers a thread forward and two of 128
-// backward for bf16; for fp32 shared memory holds fewer.
-template <typename T>
+// Stages, and resident blocks an SM: for bf16 three of 80 registers a thread forward, two of 128
+// in a chain of blocks (which keeps two tiles in registers) and backward; for fp32 shared memory
+// holds two, without the room that finishing a round behind takes.
+template <typename T, bool CHAIN>
 struct Fwd {
-  static constexpr int kStages = 2, kPerSm = sizeof(T) == 2 ? 3 : 2;
+  static constexpr int kStages = 2, kPerSm = sizeof(T) == 2 && !CHAIN ? 3 : 2;
+  static constexpr bool kBehind = CHAIN && sizeof(T) == 2;  // a tile is finished a round behind
   using R = Ring<T, 3, kStages>;
 };
 template <typename T>
@@ -437,16 +441,20 @@ struct Bwd {
   using R = Ring<T, 4, kStages>;
 };
 
-template <typename T, bool TMA>
-__global__ void __launch_bounds__(32 * kWarps, Fwd<T>::kPerSm)
+// CHAIN: blocks in clusters. A round's exchange takes as long as half a tile's arithmetic, so for
+// bf16 a block scans its next tile before it receives the last one's entering state, two tiles in
+// registers (B1 T131072 D2048: 618 -> 578 us).
+template <typename T, bool TMA, bool CHAIN>
+__global__ void __launch_bounds__(32 * kWarps, Fwd<T, CHAIN>::kPerSm)
     scan_tiles(const __grid_constant__ Args p, const __grid_constant__ Maps tm) {
+  constexpr bool BEHIND = Fwd<T, CHAIN>::kBehind;
+  constexpr int NS = Fwd<T, CHAIN>::kStages, NM = BEHIND ? 3 : 2, DEPTH = BEHIND ? 4 : 2;
   extern __shared__ __align__(128) uint8_t stages[];
-  __shared__ __align__(16) float4 maps[2][kWarps][32];
-  __shared__ __align__(16) float4 slots[2][8][32];
-  __shared__ __align__(8) uint64_t full[Fwd<T>::kStages], xbar[2];
-  constexpr int NS = Fwd<T>::kStages;
+  __shared__ __align__(16) float4 maps[NM][kWarps][32];
+  __shared__ __align__(16) float4 slots[CHAIN ? DEPTH : 1][8][32];
+  __shared__ __align__(8) uint64_t full[NS], xbar[DEPTH];
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int nblk = cluster_size(), rank = cluster_rank();
+  const int nblk = CHAIN ? cluster_size() : 1, rank = CHAIN ? cluster_rank() : 0;
   const Lane ln(blockIdx.y * kCols, p.D);
   const int n = blockIdx.z;
   T* y = static_cast<T*>(p.y) + ln.c;
@@ -456,8 +464,8 @@ __global__ void __launch_bounds__(32 * kWarps, Fwd<T>::kPerSm)
       if (t % (nblk * kWarps) == w && ln.on) store_pair<T, false>(y + t * p.D, f2(0.f), ln.two);
     return;
   }
-  typename Fwd<T>::R ring(stages, full);
-  Exchange ex(slots, xbar, nblk, rank);
+  typename Fwd<T, CHAIN>::R ring(stages, full);
+  Exchange<DEPTH> ex(slots, xbar, nblk, rank);
   const Seq q = sequence(p, n);
   y += (q.batch * p.T + q.lo) * p.D;
   const float2 ndecay = neg_decay(ln, p.decay);
@@ -472,8 +480,10 @@ __global__ void __launch_bounds__(32 * kWarps, Fwd<T>::kPerSm)
   if (TMA && threadIdx.x == 0)
     for (int j = 0; j < NS; ++j) ask(j);
   const int own = (warp * kRows * kCols + 2 * lane) * (int)sizeof(T);
-  for (int j = 0; j < rounds; ++j) {
-    const int tile = j * nblk + rank, row0 = tile * kChunk + warp * kRows, par = j & 1;
+
+  // The lane's tokens of step j from zero, their maps' last one into shared memory.
+  auto scan_tile = [&](int j, float2(&A)[kRows], float2(&S)[kRows]) {
+    const int tile = j * nblk + rank, row0 = tile * kChunk + warp * kRows;
     const int have = min(max(q.len - row0, 0), kRows);  // rows of the lane's 8 that there are
     uint8_t *xs = ring.slot(j, 0) + own, *rs = ring.slot(j, 1) + own, *is = ring.slot(j, 2) + own;
     if constexpr (TMA) {
@@ -490,7 +500,6 @@ __global__ void __launch_bounds__(32 * kWarps, Fwd<T>::kPerSm)
       put_pair<T>(xs, k, f2(0.f));
     }
     if (TMA && have < kRows) fence_proxy_async_smem();  // before TMA writes there again
-    float2 A[kRows], S[kRows];
     RawPair<T> r[kRows];
 #pragma unroll
     for (int k = 0; k < kRows; ++k) r[k] = get_pair<T>(rs, k);
@@ -508,47 +517,85 @@ __global__ void __launch_bounds__(32 * kWarps, Fwd<T>::kPerSm)
       scan_rows(std::true_type());
     else
       scan_rows(std::false_type());
-    maps[par][warp][lane] = make_float4(A[kRows - 1].x, A[kRows - 1].y, S[kRows - 1].x, S[kRows - 1].y);
-    __syncthreads();
-    if (TMA && threadIdx.x == 0) ask(j + NS);
-    float2 h = carry, hin;
-    if (nblk == 1) {
+    maps[j % NM][warp][lane] = make_float4(A[kRows - 1].x, A[kRows - 1].y, S[kRows - 1].x, S[kRows - 1].y);
+  };
+  // The tile of step j, entered by h, the lane's run by hin: its states.
+  auto emit = [&](int j, float2 h, float2 hin, const float2(&A)[kRows], const float2(&S)[kRows]) {
+    const int tile = j * nblk + rank, row0 = tile * kChunk + warp * kRows;
+    const int have = min(max(q.len - row0, 0), kRows);
+    if (p.states != nullptr && warp == 0 && tile < ntiles) ln.store(p.states + (q.slot + tile) * p.D, h);
+    if (!ln.on) return;
+    T* yr = y + (long long)row0 * p.D;
+    if (have == kRows) {
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) store_pair<T, TMA>(yr + (long long)k * p.D, __ffma2_rn(A[k], hin, S[k]), ln.two);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kRows; ++k)
+        if (k < have) store_pair<T, TMA>(yr + (long long)k * p.D, __ffma2_rn(A[k], hin, S[k]), ln.two);
+    }
+  };
+  if constexpr (!CHAIN) {
+    float2 A[kRows], S[kRows];
+    for (int j = 0; j < rounds; ++j) {
+      scan_tile(j, A, S);
+      __syncthreads();
+      if (TMA && threadIdx.x == 0) ask(j + NS);
+      const float2 h = carry;
+      float2 hin = carry;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         if (w == warp) hin = carry;
-        carry = apply(maps[par][w][lane], carry);
+        carry = apply(maps[j % NM][w][lane], carry);
       }
-    } else {
+      emit(j, h, hin, A, S);
+    }
+  } else {
+    auto finish = [&](int j, const float2(&A)[kRows], const float2(&S)[kRows]) {
+      const float2 h = ex.receive(j, carry, &g_status_scan);
+      float2 hin = h;
+      for (int w = 0; w < warp; ++w) hin = apply(maps[j % NM][w][lane], hin);
+      emit(j, h, hin, A, S);
+    };
+    auto scan_and_send = [&](int j, float2(&A)[kRows], float2(&S)[kRows]) {
+      scan_tile(j, A, S);
+      __syncthreads();
+      if (TMA && threadIdx.x == 0) ask(j + NS);
       if (warp == kWarps - 1) {
         float2 ta = f2(1.f), ts = f2(0.f);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float4 m = maps[par][w][lane];
+          const float4 m = maps[j % NM][w][lane];
           ta = __fmul2_rn(ta, make_float2(m.x, m.y));
           ts = apply(m, ts);
         }
         ex.send(j, make_float4(ta.x, ta.y, ts.x, ts.y));
       }
-      h = ex.receive(j, carry, &g_status_scan);
-      hin = h;
-      for (int w = 0; w < warp; ++w) hin = apply(maps[par][w][lane], hin);
-    }
-    if (p.states != nullptr && warp == 0 && tile < ntiles) ln.store(p.states + (q.slot + tile) * p.D, h);
-    if (ln.on) {
-      T* yr = y + (long long)row0 * p.D;
-      if (have == kRows) {
-#pragma unroll
-        for (int k = 0; k < kRows; ++k)
-          store_pair<T, TMA>(yr + (long long)k * p.D, __ffma2_rn(A[k], hin, S[k]), ln.two);
-      } else {
-#pragma unroll
-        for (int k = 0; k < kRows; ++k)
-          if (k < have) store_pair<T, TMA>(yr + (long long)k * p.D, __ffma2_rn(A[k], hin, S[k]), ln.two);
+    };
+    float2 A0[kRows], S0[kRows];
+    if constexpr (BEHIND) {
+      float2 A1[kRows], S1[kRows];
+      for (int j = 0; j < rounds; j += 2) {
+        scan_and_send(j, A0, S0);
+        if (j > 0) finish(j - 1, A1, S1);
+        if (j + 1 < rounds) {
+          scan_and_send(j + 1, A1, S1);
+          finish(j, A0, S0);
+        }
+      }
+      if (rounds & 1)
+        finish(rounds - 1, A0, S0);
+      else if (rounds > 0)
+        finish(rounds - 1, A1, S1);
+    } else {
+      for (int j = 0; j < rounds; ++j) {
+        scan_and_send(j, A0, S0);
+        finish(j, A0, S0);
       }
     }
   }
   if (p.final_state != nullptr && rank == 0 && warp == 0) ln.store(p.final_state + (long long)n * p.D, carry);
-  if (nblk > 1) cluster_barrier();  // no block leaves while another may still send to it
+  if (CHAIN) cluster_barrier();  // no block leaves while another may still send to it
 }
 
 // --------------------------------------------------------------------------- backward
@@ -582,7 +629,7 @@ __global__ void __launch_bounds__(32 * kWarps, Bwd<T>::kPerSm)
     return;
   }
   typename Bwd<T>::R ring(stages, full);
-  Exchange ex(slots, xbar, nblk, rank);
+  Exchange<2> ex(slots, xbar, nblk, rank);
   const Seq q = sequence(p, n);
   const long long first = (q.batch * p.T + q.lo) * p.D;
   const float2 ndecay = neg_decay(ln, p.decay);
@@ -774,25 +821,22 @@ constexpr int kDirectTokens = 16;
 
 // Blocks that share a sequence: as many as fit the GPU at once, and no more than a sequence has
 // pairs of tiles for. Measured on bf16, forward: B8 T4096 D2048 (256 sequences of channels)
-// 127 us alone, 141 with two blocks each, 158 with eight; B1 T131072 D2048 2473 us alone, 618
-// with eight. Where a grid of single blocks leaves less than a second round to fill and sequences
-// are long, halves of them fill it better (B16 T8192: 446 us alone, 426 with two, 476 with four;
-// backward 846, 803, 858). Packed lengths are not known here: the longest of n random pieces
-// has about (1 + ln n) / n of the rows, and the rest of the work fits beside it (65537 rows in 5
-// pieces backward: 902 us alone, 622, 506 and 517 with two, four, eight; 20011 rows in 37 pieces
-// forward fp32: 80, 86, 111, 164).
-int cluster_blocks(int T, int D, int nseq, bool packed, int per_sm) {
+// 127 us alone, 141 with two blocks each, 158 with eight; B16 T8192 446 us alone, 484 with two;
+// B1 T131072 2473 us alone, 578 with eight. Packed lengths are not known here: the longest of n
+// random pieces has about (1 + ln n) / n of the rows, and the rest of the work fits beside it
+// (65537 rows in 5 pieces backward: 902 us alone, 622, 506 and 517 with two, four, eight; 20011
+// rows in 37 pieces forward fp32: 80, 86, 111, 164).
+int cluster_blocks(int T, int D, int nseq, bool packed, int chain_per_sm) {
   const double cols = (D + kCols - 1) / kCols, longest = packed ? (1. + std::log((double)nseq)) / nseq : 1.;
   const double base = packed ? cols / longest : cols * nseq, tiles = T * longest / kChunk;
-  const double slots = (double)sm_count() * per_sm;
-  if (base > slots) return base < 2 * slots && tiles >= 96 ? 2 : 1;
   int n = 1;
-  while (n < 8 && base * n * 2 <= slots && tiles >= 4 * n) n *= 2;
+  while (n < 8 && base * n * 2 <= (double)sm_count() * chain_per_sm && tiles >= 4 * n) n *= 2;
   return n;
 }
 
 int bwd_cluster(int T, int D, int nseq, bool packed, int dtype) {
-  return cluster_blocks(T, D, nseq, packed, dtype == THM_BF16 ? Bwd<__nv_bfloat16>::kPerSm : Bwd<float>::kPerSm);
+  const int per_sm = dtype == THM_BF16 ? Bwd<__nv_bfloat16>::kPerSm : Bwd<float>::kPerSm;
+  return cluster_blocks(T, D, nseq, packed, per_sm);
 }
 
 template <typename K>
@@ -822,7 +866,6 @@ int launch_tiles(K kernel, const Args& p, const Maps& tm, int n, int seqs, int s
 template <typename T>
 int run_fwd(const Args& p, int B, int seqs, int dtype, cudaStream_t st) {
   constexpr int elem = sizeof(T);
-  const int per_sm = Fwd<T>::kPerSm;
   if (p.T <= kDirectTokens) {
     const dim3 grid((p.D + 2 * kDirectThreads - 1) / (2 * kDirectThreads), seqs);
     if (multiples(2 * elem, elem, p.D, {p.x, p.r, p.i, p.y}, {p.xb, p.xt, p.rb, p.rt, p.ib, p.it}))
@@ -831,15 +874,19 @@ int run_fwd(const Args& p, int B, int seqs, int dtype, cudaStream_t st) {
       scan_direct<T, false><<<grid, kDirectThreads, 0, st>>>(p);
     return check_launch();
   }
-  const int n = cluster_blocks(p.T, p.D, p.nseq, p.cu != nullptr, per_sm);
+  const int n = cluster_blocks(p.T, p.D, p.nseq, p.cu != nullptr, Fwd<T, true>::kPerSm);
   Maps tm{};
   bool tma = multiples(16, elem, p.D, {p.x, p.r, p.i, p.y}, {B > 1 ? p.xb : 0, p.xt, B > 1 ? p.rb : 0, p.rt, B > 1 ? p.ib : 0, p.it});
   tma = tma && encode(&tm.in[0], dtype, p.x, p.xb, p.xt, B, p.T, p.D) == THM_OK &&
         encode(&tm.in[1], dtype, p.r, p.rb, p.rt, B, p.T, p.D) == THM_OK &&
         encode(&tm.in[2], dtype, p.i, p.ib, p.it, B, p.T, p.D) == THM_OK;
-  const int smem = Fwd<T>::R::kBytes;
-  return tma ? launch_tiles(scan_tiles<T, true>, p, tm, n, seqs, smem, st)
-             : launch_tiles(scan_tiles<T, false>, p, tm, n, seqs, smem, st);
+  constexpr int smem = Fwd<T, false>::R::kBytes;
+  static_assert(smem == Fwd<T, true>::R::kBytes);
+  if (n > 1)
+    return tma ? launch_tiles(scan_tiles<T, true, true>, p, tm, n, seqs, smem, st)
+               : launch_tiles(scan_tiles<T, false, true>, p, tm, n, seqs, smem, st);
+  return tma ? launch_tiles(scan_tiles<T, true, false>, p, tm, 1, seqs, smem, st)
+             : launch_tiles(scan_tiles<T, false, false>, p, tm, 1, seqs, smem, st);
 }
 
 template <typename T>

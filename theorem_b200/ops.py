@@ -345,10 +345,12 @@ def chunk_local_cumsum(g_inc, scale: float = 1.0, out=None):
 # These calls serve single tokens too, where the launch takes 2 to 3 us on the GPU and the host
 # sets the pace: the checks are plain comparisons, and messages are only formed on failure.
 def _like(name, t, ref):
-    """t has ref's shape, dtype and device, and unit stride over channels."""
+    """t's strides; t has ref's shape, dtype and device, and unit stride over channels."""
     assert t.shape == ref.shape and t.dtype == ref.dtype and t.device == ref.device, \
         f"{name} must be {tuple(ref.shape)} {ref.dtype} on {ref.device}"
-    assert t.shape[-1] <= 1 or t.stride(-1) == 1, f"{name} must have unit stride over channels"
+    st = t.stride()
+    assert st[-1] == 1 or t.shape[-1] <= 1, f"{name} must have unit stride over channels"
+    return st
 
 
 def _dense(name, t, ref, shape, dtype):
@@ -364,27 +366,29 @@ def _empty(ref, shape, dtype):
     return torch.empty(shape, dtype=dtype, device=ref.device)
 
 
-def _channel_last(x, what):
-    assert x.dtype in (torch.float32, torch.bfloat16), f"unsupported dtype {x.dtype} (float32 or bfloat16)"
-    assert x.shape[-1] <= 1 or x.stride(-1) == 1, f"{what} must have unit stride over channels"
+def _channel_last(x):
+    """x's strides; x is fp32 or bf16 with unit stride over channels."""
+    assert x.dtype is torch.bfloat16 or x.dtype is torch.float32, f"unsupported dtype {x.dtype} (float32 or bfloat16)"
+    st = x.stride()
+    assert st[-1] == 1 or x.shape[-1] <= 1, "x must have unit stride over channels"
+    return st
 
 
 def _scan_args(x, r, i, decay, cu_seqlens):
-    """(B, T, D, sequences, shape of the chunk states)."""
+    """(B, T, D, sequences, shape of the chunk states, batch and time strides of x, r, i)."""
     _cuda(x, r, i, decay, cu_seqlens)
-    assert x.dim() == 3, "x must be [B, T, D]"
-    _channel_last(x, "x")
-    _like("r", r, x)
-    _like("i", i, x)
-    B, T, D = x.shape
+    shape = x.shape
+    assert len(shape) == 3, "x must be [B, T, D]"
+    strides = _channel_last(x)[:2] + _like("r", r, x)[:2] + _like("i", i, x)[:2]
+    B, T, D = shape
     _dense("decay", decay, x, (D,), torch.float32)
     if cu_seqlens is None:
-        return B, T, D, B, (B, (T + BT - 1) // BT, D)
+        return B, T, D, B, (B, (T + BT - 1) // BT, D), strides
     assert B == 1, "packed sequences share one batch entry: x must be [1, T, D]"
     assert cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 2, "cu_seqlens must hold N + 1 >= 2 row offsets"
     n = cu_seqlens.numel() - 1
     _dense("cu_seqlens", cu_seqlens, x, (n + 1,), torch.int32)
-    return B, T, D, n, (B, T // BT + n, D)
+    return B, T, D, n, (B, T // BT + n, D), strides
 
 
 @_on_input_device
@@ -408,7 +412,7 @@ def gated_scan(x, r, i, decay, h0=None, cu_seqlens=None, want_states: bool = Fal
     [B, ceil(T / 64), D] fp32; packed, sequence n's start at slot cu[n] // 64 + n of
     [1, T // 64 + N, D] and unused slots are 0.
     """
-    B, T, D, n, sshape = _scan_args(x, r, i, decay, cu_seqlens)
+    B, T, D, n, sshape, strides = _scan_args(x, r, i, decay, cu_seqlens)
     if h0 is not None:
         _cuda(h0)
         _dense("h0", h0, x, (n, D), torch.float32)
@@ -427,10 +431,10 @@ def gated_scan(x, r, i, decay, h0=None, cu_seqlens=None, want_states: bool = Fal
     if want_states:
         make = torch.zeros if cu_seqlens is not None else torch.empty
         states = make(sshape, device=x.device, dtype=torch.float32)
-    L.check(L.load().thm_gated_scan_fwd(L.ptr(x), L.ptr(r), L.ptr(i), L.ptr(decay), L.ptr(h0), L.ptr(cu_seqlens),
-                                        L.ptr(y), L.ptr(final), L.ptr(states), x.stride(0), x.stride(1), r.stride(0),
-                                        r.stride(1), i.stride(0), i.stride(1), B, T, D, n, int(fresh),
-                                        L.dtype_code(x), L.stream_of(x)), "thm_gated_scan_fwd")
+    ptr = L.ptr
+    L.check(L.load().thm_gated_scan_fwd(x.data_ptr(), r.data_ptr(), i.data_ptr(), decay.data_ptr(), ptr(h0),
+                                        ptr(cu_seqlens), y.data_ptr(), final.data_ptr(), ptr(states), *strides, B, T, D,
+                                        n, int(fresh), L.dtype_code(x), L.stream_of(x)), "thm_gated_scan_fwd")
     return y, final, states
 
 
@@ -444,9 +448,9 @@ def gated_scan_bwd(x, r, i, decay, states, dy, dfinal=None, cu_seqlens=None, dx=
     treated as in ``gated_scan``. Sums over tokens are in fp32 in a fixed order, so results
     repeat bit for bit.
     """
-    B, T, D, n, sshape = _scan_args(x, r, i, decay, cu_seqlens)
+    B, T, D, n, sshape, strides = _scan_args(x, r, i, decay, cu_seqlens)
     _cuda(states, dy, dfinal)
-    _like("dy", dy, x)
+    strides += _like("dy", dy, x)[:2]
     _dense("states", states, x, sshape, torch.float32)
     if dfinal is not None:
         _dense("dfinal", dfinal, x, (n, D), torch.float32)
@@ -464,9 +468,8 @@ def gated_scan_bwd(x, r, i, decay, states, dy, dfinal=None, cu_seqlens=None, dx=
     work = torch.empty(parts, D, device=x.device, dtype=torch.float32)
     L.check(L.load().thm_gated_scan_bwd(L.ptr(x), L.ptr(r), L.ptr(i), L.ptr(decay), L.ptr(states), L.ptr(dy),
                                         L.ptr(dfinal), L.ptr(cu_seqlens), L.ptr(dx), L.ptr(dr), L.ptr(di),
-                                        L.ptr(ddecay), L.ptr(dh0), L.ptr(work), x.stride(0), x.stride(1), r.stride(0),
-                                        r.stride(1), i.stride(0), i.stride(1), dy.stride(0), dy.stride(1), B, T, D, n,
-                                        int(fresh), L.dtype_code(x), L.stream_of(x)), "thm_gated_scan_bwd")
+                                        L.ptr(ddecay), L.ptr(dh0), L.ptr(work), *strides, B, T, D, n, int(fresh),
+                                        L.dtype_code(x), L.stream_of(x)), "thm_gated_scan_bwd")
     return dx, dr, di, ddecay, dh0
 
 
@@ -488,7 +491,7 @@ def _rows(name, t):
 def _norm_args(x, group, weight, bias, gate, activation):
     _cuda(x, weight, bias, gate)
     assert x.dim() >= 1, "x must be [..., C]"
-    _channel_last(x, "x")
+    _channel_last(x)
     C = x.shape[-1]
     assert group >= 1 and C % group == 0, f"C={C} is not a multiple of the group size {group}"
     if gate is not None:
@@ -560,14 +563,14 @@ def group_norm_bwd(x, dy, group: int, weight=None, bias=None, gate=None, activat
 def _conv_args(x, weight, bias, activation):
     _cuda(x, weight, bias)
     assert x.dim() == 3, "x must be [B, S, D]"
-    _channel_last(x, "x")
+    strides = _channel_last(x)[:2]
     B, S, D = x.shape
     assert weight.dim() == 2 and weight.shape[1] >= 1, "weight must be [D, W]"
     W = weight.shape[1]
     _dense("weight", weight, x, (D, W), torch.float32)
     _dense("bias", bias, x, (D,), torch.float32)
     assert activation in _ACT, f"unknown activation {activation!r}"
-    return B, S, D, W
+    return B, S, D, W, strides
 
 
 @_on_input_device
@@ -580,7 +583,7 @@ def causal_conv1d_step(x, state, weight, bias, activation=None, out=None, state_
     prefill it is the last W - 1 rows of its input. x has unit stride over D, any strides over
     B and S; W <= 8; weight, bias fp32 (kernels/causal_conv1d/kernel.py:170-230 from zeros).
     """
-    B, S, D, W = _conv_args(x, weight, bias, activation)
+    B, S, D, W, strides = _conv_args(x, weight, bias, activation)
     assert S <= 64, f"S={S}: the carried-state form takes at most 64 tokens (causal_conv1d takes long runs)"
     _cuda(state)
     _dense("state", state, x, (B, W - 1, D), x.dtype)
@@ -593,7 +596,7 @@ def causal_conv1d_step(x, state, weight, bias, activation=None, out=None, state_
     else:
         _dense("state_out", state_out, x, (B, W - 1, D), x.dtype)
     L.check(L.load().thm_causal_conv1d_step(L.ptr(x), L.ptr(state), L.ptr(weight), L.ptr(bias), L.ptr(out),
-                                            L.ptr(state_out), x.stride(0), x.stride(1), B, S, D, W, L.dtype_code(x),
+                                            L.ptr(state_out), *strides, B, S, D, W, L.dtype_code(x),
                                             _ACT[activation], L.stream_of(x)), "thm_causal_conv1d_step")
     return out, state_out
 
@@ -606,16 +609,15 @@ def causal_conv1d_bwd(x, weight, bias, dy, activation=None):
     x, dy [B, S, D] fp32 or bf16 of one dtype, unit stride over D, any strides over B and S;
     W <= 8. Sums over tokens are in fp32 in a fixed order, so results repeat bit for bit.
     """
-    B, S, D, W = _conv_args(x, weight, bias, activation)
+    B, S, D, W, strides = _conv_args(x, weight, bias, activation)
     _cuda(dy)
-    _like("dy", dy, x)
+    strides += _like("dy", dy, x)[:2]
     dx = _empty(x, x.shape, x.dtype)
     dweight = torch.empty(D, W, device=x.device, dtype=torch.float32)
     dbias = torch.empty(D, device=x.device, dtype=torch.float32)
     parts = L.load().thm_causal_conv1d_bwd_parts(B, S, D)
     work = torch.empty(max(parts, 0), W + 1, D, device=x.device, dtype=torch.float32)
     L.check(L.load().thm_causal_conv1d_bwd(L.ptr(x), L.ptr(weight), L.ptr(bias), L.ptr(dy), L.ptr(dx), L.ptr(dweight),
-                                           L.ptr(dbias), L.ptr(work), x.stride(0), x.stride(1), dy.stride(0),
-                                           dy.stride(1), B, S, D, W, L.dtype_code(x), _ACT[activation],
+                                           L.ptr(dbias), L.ptr(work), *strides, B, S, D, W, L.dtype_code(x), _ACT[activation],
                                            L.stream_of(x)), "thm_causal_conv1d_bwd")
     return dx, dweight, dbias
