@@ -128,6 +128,25 @@ def test_strided_and_unaligned_inputs(shift, dtype):
     _check_step(x, w, b, st, None, out, st2, dtype)
 
 
+def test_time_major_inputs():
+    from theorem_b200 import ops
+    x, dy, w, b, _ = _inputs(3, 200, 64, 4, BF, seed=3)
+    tm = [t.transpose(0, 1).contiguous().to(DEV).transpose(0, 1) for t in (x, dy)]
+    _check_bwd(x, dy, w, b, "silu", ops.causal_conv1d_bwd(tm[0], w.to(DEV), b.to(DEV), tm[1], activation="silu"), BF)
+
+
+def test_offsets_past_32_bits():
+    from theorem_b200 import ops
+    D, tail = 2048, 500
+    S = (1 << 20) + tail
+    x = torch.randn(1, S, D, device=DEV, dtype=BF, generator=torch.Generator(DEV).manual_seed(0))
+    w, b = torch.full((D, 4), 0.25, device=DEV), torch.zeros(D, device=DEV)
+    xt = x[:, -tail:].contiguous()
+    a = ops.causal_conv1d_bwd(x, w, b, x, activation="silu")[0][:, -tail + 3:]  # 3 rows see what came before
+    c = ops.causal_conv1d_bwd(xt, w, b, xt, activation="silu")[0][:, 3:]
+    assert torch.equal(a, c)
+
+
 def test_empty_repeat_and_capture():
     from theorem_b200 import ops
     e = torch.empty(0, 5, 64, device=DEV)

@@ -113,6 +113,57 @@ def test_strided_and_unaligned_inputs(T, shift, dtype):
     _check_bwd(x, r, i, decay, h0, dy, df, grads, dtype)
 
 
+@pytest.mark.parametrize("T", [65, 1100])
+def test_time_major_and_expanded_inputs(T):
+    """A [T, B, D] tensor seen as [B, T, D], and a gate that all sequences share (stride 0)."""
+    from theorem_b200 import ops
+    B, D = 3, 64
+    x, r, i, decay, h0, dy, df = _inputs(B, T, D, BF, seed=T)
+    i = i[:1].expand(B, T, D)
+    tm = [t.transpose(0, 1).contiguous().to(DEV).transpose(0, 1) for t in (x, r, dy)]
+    ie = i[:1].to(DEV).expand(B, T, D)
+    out = ops.gated_scan(tm[0], tm[1], ie, decay.to(DEV), h0=h0.to(DEV), want_states=True)
+    assert out[0].is_contiguous()
+    _check_fwd(x, r, i, decay, h0, out, BF)
+    grads = ops.gated_scan_bwd(tm[0], tm[1], ie, decay.to(DEV), out[2], tm[2], dfinal=df.to(DEV))
+    _check_bwd(x, r, i, decay, h0, dy, df, grads, BF)
+
+
+@pytest.mark.parametrize("T", [1, 40, 3000])
+def test_final_in_place_of_h0(T):
+    """Short runs, single blocks and chains of blocks: the state moves on in its own buffer."""
+    from theorem_b200 import ops
+    x, r, i, decay, h0, _, _ = _inputs(1, T, 128, BF, seed=T)
+    args = _d(x, r, i, decay)
+    y, fin, _ = ops.gated_scan(*args, h0=h0.to(DEV))
+    st = h0.to(DEV)
+    y2, fin2, _ = ops.gated_scan(*args, h0=st, final=st)
+    assert fin2 is st and torch.equal(st, fin) and torch.equal(y, y2)
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements a tensor: the last rows equal the same rows run on their own from the
+    chunk state that entered them, and so do their gradients."""
+    from theorem_b200 import ops
+    D, tail = 2048, 640
+    T = (1 << 20) + 64 * 17
+    assert T * D > 1 << 31
+    x = torch.randn(1, T, D, device=DEV, dtype=BF, generator=torch.Generator(DEV).manual_seed(0))
+    dec = torch.full((D,), 0.2, device=DEV)
+    y, fin, st = ops.gated_scan(x, x, x, dec, want_states=True)
+    xt = x[:, -tail:]
+    y2, fin2, st2 = ops.gated_scan(xt, xt, xt, dec, h0=st[:, -tail // 64].contiguous(), want_states=True)
+    e = 1e-5  # two orders of the same fp32 sums; y also by one bf16 step of its value
+    assert (fin - fin2).abs().max() <= e and (st[:, -tail // 64:] - st2).abs().max() <= e
+    assert ((y[:, -tail:].float() - y2.float()).abs() <= e + 2 ** -7 * y2.float().abs()).all()
+    del y, y2
+    df = torch.ones(1, D, device=DEV)
+    a = ops.gated_scan_bwd(x, x, x, dec, st, x, dfinal=df)
+    b = ops.gated_scan_bwd(xt, xt, xt, dec, st2, xt, dfinal=df)
+    for p, q in zip(a[:3], b[:3]):
+        assert ((p[:, -tail:].float() - q.float()).abs() <= e + 2 ** -7 * q.float().abs()).all()
+
+
 PACKS = [  # row offsets, rows
     ([0, 1, 2, 3], 3), ([0, 0, 0], 5), ([0, 64, 64, 191, 200], 200), ([3, 10, 10, 75, 331], 400),
     ([0, 129, 130, 700, 701], 777), ([0, 1500], 1500),

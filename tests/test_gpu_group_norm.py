@@ -142,6 +142,31 @@ def test_row_strides_and_unaligned_addresses(shift, dtype):
            dtype)
 
 
+def test_in_place():
+    from theorem_b200 import ops
+    x, _, z, w, b = [t.to(DEV) for t in _inputs(500, 384, BF, 6, True, True)]
+    kw = dict(activation="silu", center=False)
+    want = ops.group_norm(x, 128, w, b, gate=z, **kw)
+    for k in range(2):
+        xs, zs = x.clone(), z.clone()
+        out = (xs, zs)[k]
+        assert ops.group_norm(xs, 128, w, b, gate=zs, out=out, **kw) is out and torch.equal(out, want)
+
+
+def test_offsets_past_32_bits():
+    from theorem_b200 import ops
+    C, tail = 4096, 300
+    R = (1 << 19) + tail
+    x = torch.randn(R, C, device=DEV, dtype=BF, generator=torch.Generator(DEV).manual_seed(0))
+    w = torch.ones(C, device=DEV)
+    kw = dict(activation="silu", center=False)
+    xt = x[-tail:].clone()
+    assert torch.equal(ops.group_norm(x, 128, w, gate=x, **kw)[-tail:], ops.group_norm(xt, 128, w, gate=xt, **kw))
+    a = ops.group_norm_bwd(x, x, 128, w, gate=x, **kw)
+    b = ops.group_norm_bwd(xt, xt, 128, w, gate=xt, **kw)
+    assert torch.equal(a[0][-tail:], b[0]) and torch.equal(a[1][-tail:], b[1])
+
+
 def test_large_mean_keeps_the_variance():
     """A mean 1000 times the deviation: the centred sum keeps what a difference of sums loses."""
     from theorem_b200 import ops

@@ -25,6 +25,11 @@ over the chunks and h, v_new never reach HBM; with a conv width of 4 the v
 conv also runs inside recompute_w_u (ops.recompute_w_u_conv: v is read only
 there, so it never reaches HBM). ``fused=False`` keeps the separate v conv,
 recompute_w_u, chunk_fwd_h and chunk_fwd_o launches.
+
+With ``norm_weight`` the output goes through a per-head RMS norm and, if the call has one, a
+SiLU gate, in one more launch (ops.group_norm, in place on o):
+
+    o = o / sqrt(mean over the head of o^2 + eps) * norm_weight (* silu(gate))
 """
 from __future__ import annotations
 
@@ -37,7 +42,7 @@ class GatedDeltaNetForward:
     """Callable layer forward; holds the depthwise conv weights [H*K, W] / [H*V, W]."""
 
     def __init__(self, H: int, K: int, V: int, conv_weights, conv_biases, activation: str = "silu",
-                 scale: float | None = None, fused: bool = True):
+                 scale: float | None = None, fused: bool = True, norm_weight=None, norm_eps: float = 1e-5):
         assert len(conv_weights) == 3 and len(conv_biases) == 3, "q, k, v conv weights and biases"
         self.H, self.K, self.V = H, K, V
         self.wq, self.wk, self.wv = (w.contiguous().float() for w in conv_weights)
@@ -45,6 +50,11 @@ class GatedDeltaNetForward:
         self.activation = activation
         self.scale = K ** -0.5 if scale is None else float(scale)
         self.fused = fused
+        self.norm_weight, self.norm_eps = None, float(norm_eps)
+        if norm_weight is not None:  # [V], shared by the heads, or [H*V]
+            assert norm_weight.shape in ((V,), (H * V,)), f"norm_weight must be [{V}] or [{H * V}]"
+            w = norm_weight.float()
+            self.norm_weight = (w.repeat(H) if w.shape[0] != H * V else w).contiguous()
         self._buf: dict = {}
 
     def uses_fused(self, dtype) -> bool:
@@ -72,7 +82,18 @@ class GatedDeltaNetForward:
             )
         return self._buf
 
-    def __call__(self, xq, xk, xv, beta, g, h0=None, out=None, final_state: bool = True):
+    def __call__(self, xq, xk, xv, beta, g, h0=None, out=None, final_state: bool = True, gate=None):
+        """(o [B, T, H, V], final state or None). ``gate`` [B, T, H*V] needs ``norm_weight``."""
+        assert gate is None or self.norm_weight is not None, "gate goes with norm_weight"
+        o, fin = self._layer(xq, xk, xv, beta, g, h0, out, final_state)
+        if self.norm_weight is not None:
+            B, T = xq.shape[:2]
+            flat = o.view(B, T, self.H * self.V)
+            ops.group_norm(flat, self.V, self.norm_weight, gate=gate, activation=None if gate is None else "silu",
+                           center=False, eps=self.norm_eps, out=flat)
+        return o, fin
+
+    def _layer(self, xq, xk, xv, beta, g, h0, out, final_state):
         B, T, Dq = xq.shape
         H, K, V = self.H, self.K, self.V
         assert Dq == H * K and xk.shape == xq.shape and xv.shape == (B, T, H * V)
@@ -105,6 +126,7 @@ class GatedDeltaNetForward:
         [B,H,K,V] fp32 when ``h0`` is given)."""
         B, T, D = xq.shape
         assert B % slices == 0, "B must split into equal groups"
+        assert self.norm_weight is None, "the host pipeline runs the layer without its output norm"
         assert all(t.is_pinned() for t in (xq, xk, xv, beta, g, out)), "host tensors must be pinned"
         bs = B // slices
         dev = torch.device("cuda", torch.cuda.current_device())

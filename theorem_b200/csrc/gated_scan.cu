@@ -594,8 +594,10 @@ __global__ void __launch_bounds__(32 * kWarps, Fwd<T, CHAIN>::kPerSm)
       }
     }
   }
+  // No block leaves while another may still send to it, and final_state may be h0: every block has
+  // read that by now.
+  if (CHAIN) cluster_barrier();
   if (p.final_state != nullptr && rank == 0 && warp == 0) ln.store(p.final_state + (long long)n * p.D, carry);
-  if (CHAIN) cluster_barrier();  // no block leaves while another may still send to it
 }
 
 // --------------------------------------------------------------------------- backward
@@ -773,6 +775,7 @@ __global__ void __launch_bounds__(32 * kWarps, Bwd<T>::kPerSm)
     else
       grad_rows(std::false_type());
   }
+  if (nblk > 1) cluster_barrier();  // as in the forward kernel, of dh0 and dfinal
   // ddecay over the block's warps, in order.
   __syncthreads();
   back[0][warp][lane] = ddecay;
@@ -784,7 +787,6 @@ __global__ void __launch_bounds__(32 * kWarps, Bwd<T>::kPerSm)
     ln.store(p.ddecay_part + ((long long)n * nblk + rank) * p.D, d);
     if (p.dh0 != nullptr && rank == 0) ln.store(p.dh0 + (long long)n * p.D, carry);
   }
-  if (nblk > 1) cluster_barrier();
 }
 
 struct StoreColumn {

@@ -407,7 +407,8 @@ def gated_scan(x, r, i, decay, h0=None, cu_seqlens=None, want_states: bool = Fal
     each from its h0; cu[0] may be > 0 and sequences may be empty (final = h0). Rows before the
     first sequence and behind the last are 0 in a fresh y and left as they are in a given one.
 
-    Returns (y [B, T, D] in x's dtype, final [N, D] fp32, states). The state is carried in fp32.
+    Returns (y [B, T, D] in x's dtype, final [N, D] fp32, states). The state is carried in fp32; a
+    given y must not overlap the inputs; at most 65534 sequences.
     ``want_states`` keeps the state entering each 64-token chunk for ``gated_scan_bwd``:
     [B, ceil(T / 64), D] fp32; packed, sequence n's start at slot cu[n] // 64 + n of
     [1, T // 64 + N, D] and unused slots are 0.
@@ -516,7 +517,7 @@ def group_norm(x, group: int, weight=None, bias=None, gate=None, activation=None
     (RMS norm per head). x, gate [..., C] fp32 or bf16 of one dtype, unit stride over C, the
     leading dimensions collapsible to rows (any row stride); weight, bias [C] fp32 or None;
     activation None or "silu"; group <= 4096. Statistics in fp32, variance from centred
-    values. Returns y, contiguous, like x.
+    values. Returns y, contiguous, like x; ``out`` may be x or gate (in place).
     """
     C = _norm_args(x, group, weight, bias, gate, activation)
     R, xs = _rows("x", x)
