@@ -20,7 +20,7 @@ def test_gated_scan_rejects_arguments_without_gpu():
     assert f(*no_cu, *q6, -1, 8, 8, -1, 0, 0, None) == _lib.THM_ERR_INVALID  # negative size
     assert f(*no_cu, *q6, 2, 8, 8, 3, 0, 0, None) == _lib.THM_ERR_INVALID    # nseq != B without cu_seqlens
     assert f(*p9, *q6, 2, 8, 8, 2, 0, 0, None) == _lib.THM_ERR_INVALID       # packed with B = 2
-    assert f(*no_cu, *q6, 65535, 1, 8, 65535, 0, 0, None) == _lib.THM_ERR_UNSUPPORTED
+    assert f(*no_cu, *q6, 1 << 27, 1, 8, 1 << 27, 0, 0, None) == _lib.THM_ERR_UNSUPPORTED
     assert f(*([None] * 9), *q6, 1, 8, 8, 1, 0, 0, None) == _lib.THM_ERR_INVALID  # null pointers
     assert f(*([None] * 9), *q6, 1, 8, 0, 1, 0, 0, None) == _lib.THM_OK      # no channels
     assert f(*([None] * 9), *q6, 0, 8, 8, 0, 0, 0, None) == _lib.THM_OK      # no sequences

@@ -33,7 +33,9 @@ struct Args {
   void *y, *dx, *dr, *di;
   float *states, *final_state, *ddecay_part, *dh0;
   long long xb, xt, rb, rt, ib, it, gb, gt;  // strides of x, r, i, dy over batch and time
-  int T, D, nseq, zero_rest;
+  int T, D, nseq;
+  int cols;          // runs of 64 channels of a sequence
+  int first, count;  // of the launch: its first (sequence, run of channels) and how many
 };
 
 // Rows of sequence n: dense batches have T rows at batch entry n, packed ones the rows
@@ -253,15 +255,16 @@ __device__ __forceinline__ bool plain_decays(float2 nd) {
 }
 
 // --------------------------------------------------------------------------- forward, few tokens
-// A lane walks its two channels token by token: single-token steps and short runs, where there
-// is nothing to split along time and a launch is all the latency there is.
+// A lane walks its two channels token by token, a warp 64 channels of a sequence: single-token
+// steps and short runs, where there is nothing to split along time and a launch is all the
+// latency there is.
 constexpr int kDirectThreads = 64;
 
 template <typename T, bool PAIRED>
 __global__ void __launch_bounds__(kDirectThreads) scan_direct(const Args p) {
-  const Lane ln(((blockIdx.x * kDirectThreads + threadIdx.x) >> 5) * 64, p.D);
-  const int n = blockIdx.y;
-  if (!ln.on) return;
+  const int chain = (blockIdx.x * kDirectThreads + threadIdx.x) >> 5, n = chain / p.cols;
+  const Lane ln(chain % p.cols * 64, p.D);
+  if (!ln.on || chain >= p.count) return;
   T* y = static_cast<T*>(p.y) + ln.c;
   if (n == p.nseq) {  // rows of no sequence
     for (long long t = rest_row(p, 0); t < p.T; t = rest_row(p, t + 1))
@@ -455,8 +458,8 @@ __global__ void __launch_bounds__(32 * kWarps, Fwd<T, CHAIN>::kPerSm)
   __shared__ __align__(8) uint64_t full[NS], xbar[DEPTH];
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int nblk = CHAIN ? cluster_size() : 1, rank = CHAIN ? cluster_rank() : 0;
-  const Lane ln(blockIdx.y * kCols, p.D);
-  const int n = blockIdx.z;
+  const int chain = p.first + blockIdx.x / nblk, n = chain / p.cols, col = chain % p.cols * kCols;
+  const Lane ln(col, p.D);
   T* y = static_cast<T*>(p.y) + ln.c;
   if (n == p.nseq) {  // rows of no sequence, in turn over the cluster's warps
     const int w = rank * kWarps + warp;
@@ -475,7 +478,7 @@ __global__ void __launch_bounds__(32 * kWarps, Fwd<T, CHAIN>::kPerSm)
   const int rounds = (ntiles + nblk - 1) / nblk;
   auto ask = [&](int j) {
     const int tile = j * nblk + rank;
-    if (tile < ntiles) ring.ask(tm.in, j, blockIdx.y * kCols, q.lo + tile * kChunk, (int)q.batch);
+    if (tile < ntiles) ring.ask(tm.in, j, col, q.lo + tile * kChunk, (int)q.batch);
   };
   if (TMA && threadIdx.x == 0)
     for (int j = 0; j < NS; ++j) ask(j);
@@ -617,8 +620,8 @@ __global__ void __launch_bounds__(32 * kWarps, Bwd<T>::kPerSm)
   constexpr int NS = Bwd<T>::kStages;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int nblk = cluster_size(), rank = cluster_rank();
-  const Lane ln(blockIdx.y * kCols, p.D);
-  const int n = blockIdx.z;
+  const int chain = p.first + blockIdx.x / nblk, n = chain / p.cols, col = chain % p.cols * kCols;
+  const Lane ln(col, p.D);
   T *dx = static_cast<T*>(p.dx) + ln.c, *dr = static_cast<T*>(p.dr) + ln.c, *di = static_cast<T*>(p.di) + ln.c;
   if (n == p.nseq) {
     const int w = rank * kWarps + warp;
@@ -642,7 +645,7 @@ __global__ void __launch_bounds__(32 * kWarps, Bwd<T>::kPerSm)
   const int rounds = (ntiles + nblk - 1) / nblk;
   auto ask = [&](int j) {
     const int tile = ntiles - 1 - (j * nblk + rank);
-    if (tile >= 0) ring.ask(tm.in, j, blockIdx.y * kCols, q.lo + tile * kChunk, (int)q.batch);
+    if (tile >= 0) ring.ask(tm.in, j, col, q.lo + tile * kChunk, (int)q.batch);
   };
   if (TMA && threadIdx.x == 0)
     for (int j = 0; j < NS; ++j) ask(j);
@@ -828,28 +831,34 @@ constexpr int kDirectTokens = 16;
 // random pieces has about (1 + ln n) / n of the rows, and the rest of the work fits beside it
 // (65537 rows in 5 pieces backward: 902 us alone, 622, 506 and 517 with two, four, eight; 20011
 // rows in 37 pieces forward fp32: 80, 86, 111, 164).
-int cluster_blocks(int T, int D, int nseq, bool packed, int chain_per_sm) {
-  const double cols = (D + kCols - 1) / kCols, longest = packed ? (1. + std::log((double)nseq)) / nseq : 1.;
-  const double base = packed ? cols / longest : cols * nseq, tiles = T * longest / kChunk;
+int cluster_blocks(double chains, double tokens, int slots) {
   int n = 1;
-  while (n < 8 && base * n * 2 <= (double)sm_count() * chain_per_sm && tiles >= 4 * n) n *= 2;
+  while (n < 8 && chains * n * 2 <= slots && tokens / kChunk >= 4 * n) n *= 2;
   return n;
+}
+int packed_blocks(int T, int cols, int nseq, int slots) {
+  const double longest = (1. + std::log((double)nseq)) / nseq;
+  return cluster_blocks(cols / longest, T * longest, slots);
 }
 
 int bwd_cluster(int T, int D, int nseq, bool packed, int dtype) {
-  const int per_sm = dtype == THM_BF16 ? Bwd<__nv_bfloat16>::kPerSm : Bwd<float>::kPerSm;
-  return cluster_blocks(T, D, nseq, packed, per_sm);
+  const int slots = sm_count() * (dtype == THM_BF16 ? Bwd<__nv_bfloat16>::kPerSm : Bwd<float>::kPerSm);
+  const int cols = (D + kCols - 1) / kCols;
+  return packed ? packed_blocks(T, cols, nseq, slots) : cluster_blocks((double)nseq * cols, T, slots);
 }
 
+// `count` sequences of channels from `first` on, n blocks each.
 template <typename K>
-int launch_tiles(K kernel, const Args& p, const Maps& tm, int n, int seqs, int smem, cudaStream_t st) {
+int launch_tiles(K kernel, Args p, const Maps& tm, int n, int first, int count, int smem, cudaStream_t st) {
+  p.first = first;
+  p.count = count;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
     cudaGetLastError();
     return THM_ERR_CUDA;
   }
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3(n, (p.D + kCols - 1) / kCols, seqs);
+  cfg.gridDim = dim3((unsigned)(n * count));
   cfg.blockDim = dim3(32 * kWarps);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -866,17 +875,18 @@ int launch_tiles(K kernel, const Args& p, const Maps& tm, int n, int seqs, int s
 }
 
 template <typename T>
-int run_fwd(const Args& p, int B, int seqs, int dtype, cudaStream_t st) {
+int run_fwd(Args p, int B, int seqs, int dtype, cudaStream_t st) {
   constexpr int elem = sizeof(T);
+  const int count = seqs * p.cols;
   if (p.T <= kDirectTokens) {
-    const dim3 grid((p.D + 2 * kDirectThreads - 1) / (2 * kDirectThreads), seqs);
+    const unsigned grid = (unsigned)((count + kDirectThreads / 32 - 1) / (kDirectThreads / 32));
+    p.count = count;
     if (multiples(2 * elem, elem, p.D, {p.x, p.r, p.i, p.y}, {p.xb, p.xt, p.rb, p.rt, p.ib, p.it}))
       scan_direct<T, true><<<grid, kDirectThreads, 0, st>>>(p);
     else
       scan_direct<T, false><<<grid, kDirectThreads, 0, st>>>(p);
     return check_launch();
   }
-  const int n = cluster_blocks(p.T, p.D, p.nseq, p.cu != nullptr, Fwd<T, true>::kPerSm);
   Maps tm{};
   bool tma = multiples(16, elem, p.D, {p.x, p.r, p.i, p.y}, {B > 1 ? p.xb : 0, p.xt, B > 1 ? p.rb : 0, p.rt, B > 1 ? p.ib : 0, p.it});
   tma = tma && encode(&tm.in[0], dtype, p.x, p.xb, p.xt, B, p.T, p.D) == THM_OK &&
@@ -884,15 +894,32 @@ int run_fwd(const Args& p, int B, int seqs, int dtype, cudaStream_t st) {
         encode(&tm.in[2], dtype, p.i, p.ib, p.it, B, p.T, p.D) == THM_OK;
   constexpr int smem = Fwd<T, false>::R::kBytes;
   static_assert(smem == Fwd<T, true>::R::kBytes);
-  if (n > 1)
-    return tma ? launch_tiles(scan_tiles<T, true, true>, p, tm, n, seqs, smem, st)
-               : launch_tiles(scan_tiles<T, false, true>, p, tm, n, seqs, smem, st);
-  return tma ? launch_tiles(scan_tiles<T, true, false>, p, tm, 1, seqs, smem, st)
-             : launch_tiles(scan_tiles<T, false, false>, p, tm, 1, seqs, smem, st);
+  auto run = [&](int n, int first, int cnt) {
+    if (n > 1)
+      return tma ? launch_tiles(scan_tiles<T, true, true>, p, tm, n, first, cnt, smem, st)
+                 : launch_tiles(scan_tiles<T, false, true>, p, tm, n, first, cnt, smem, st);
+    return tma ? launch_tiles(scan_tiles<T, true, false>, p, tm, 1, first, cnt, smem, st)
+               : launch_tiles(scan_tiles<T, false, false>, p, tm, 1, first, cnt, smem, st);
+  };
+  const int chain_slots = sm_count() * Fwd<T, true>::kPerSm, slots = sm_count() * Fwd<T, false>::kPerSm;
+  // All blocks of a launch take about as long, so a few sequences more than the GPU holds cost as
+  // much as a whole round of them: what is left over whole rounds runs as chains of blocks, in a
+  // launch of its own (B16 T8192 D2048 bf16, 68 of 512 left over: 446 us in one launch, 424 in two).
+  const int rest = count % slots;
+  if (p.cu == nullptr && count > slots && rest > 0) {
+    const int n = cluster_blocks(rest, p.T, chain_slots);
+    if (n > 1) {
+      const int e = run(1, 0, count - rest);
+      return e != THM_OK ? e : run(n, count - rest, rest);
+    }
+  }
+  return run(p.cu == nullptr ? cluster_blocks(count, p.T, chain_slots) : packed_blocks(p.T, p.cols, p.nseq, chain_slots), 0,
+             count);
 }
 
 template <typename T>
 int run_bwd(const Args& p, int B, int seqs, int dtype, int n, cudaStream_t st) {
+  const int count = seqs * p.cols;
   constexpr int elem = sizeof(T);
   Maps tm{};
   bool tma = multiples(16, elem, p.D, {p.x, p.r, p.i, p.dy, p.dx, p.dr, p.di},
@@ -902,15 +929,16 @@ int run_bwd(const Args& p, int B, int seqs, int dtype, int n, cudaStream_t st) {
         encode(&tm.in[2], dtype, p.i, p.ib, p.it, B, p.T, p.D) == THM_OK &&
         encode(&tm.in[3], dtype, p.dy, p.gb, p.gt, B, p.T, p.D) == THM_OK;
   const int smem = Bwd<T>::R::kBytes;
-  return tma ? launch_tiles(scan_bwd_tiles<T, true>, p, tm, n, seqs, smem, st)
-             : launch_tiles(scan_bwd_tiles<T, false>, p, tm, n, seqs, smem, st);
+  return tma ? launch_tiles(scan_bwd_tiles<T, true>, p, tm, n, 0, count, smem, st)
+             : launch_tiles(scan_bwd_tiles<T, false>, p, tm, n, 0, count, smem, st);
 }
 
 int check_sizes(int B, int T, int D, int nseq, const int* cu, int dtype) {
   if (B < 0 || T < 0 || D < 0 || nseq < 0) return THM_ERR_INVALID;
   if (dtype != THM_F32 && dtype != THM_BF16) return THM_ERR_INVALID;
   if (cu != nullptr ? B != 1 : nseq != B) return THM_ERR_INVALID;
-  if (nseq >= 65535 || (D + kCols - 1) / kCols > 65535) return THM_ERR_UNSUPPORTED;
+  // (sequence, 64 channels) pairs, times the blocks of a cluster, are counted in 31 bits.
+  if (((long long)nseq + 1) * ((D + kCols - 1) / kCols) >= 1ll << 27) return THM_ERR_UNSUPPORTED;
   return THM_OK;
 }
 
@@ -933,7 +961,7 @@ extern "C" int thm_gated_scan_fwd(const void* x, const void* r, const void* i, c
   p.x = x; p.r = r; p.i = i; p.decay = decay; p.h0 = h0; p.cu = cu_seqlens;
   p.y = y; p.final_state = final_state; p.states = states;
   p.xb = x_bs; p.xt = x_ts; p.rb = r_bs; p.rt = r_ts; p.ib = i_bs; p.it = i_ts;
-  p.T = T; p.D = D; p.nseq = nseq;
+  p.T = T; p.D = D; p.nseq = nseq; p.cols = (D + gscan::kCols - 1) / gscan::kCols;
   const int seqs = nseq + (cu_seqlens != nullptr && zero_rest);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return dtype == THM_BF16 ? gscan::run_fwd<__nv_bfloat16>(p, B, seqs, dtype, st)
@@ -963,7 +991,7 @@ extern "C" int thm_gated_scan_bwd(const void* x, const void* r, const void* i, c
   p.states = const_cast<float*>(states);
   p.dx = dx; p.dr = dr; p.di = di; p.ddecay_part = workspace; p.dh0 = dh0;
   p.xb = x_bs; p.xt = x_ts; p.rb = r_bs; p.rt = r_ts; p.ib = i_bs; p.it = i_ts; p.gb = dy_bs; p.gt = dy_ts;
-  p.T = T; p.D = D; p.nseq = nseq;
+  p.T = T; p.D = D; p.nseq = nseq; p.cols = (D + gscan::kCols - 1) / gscan::kCols;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   int parts = 0;
   if (nseq > 0) {

@@ -408,7 +408,7 @@ def gated_scan(x, r, i, decay, h0=None, cu_seqlens=None, want_states: bool = Fal
     first sequence and behind the last are 0 in a fresh y and left as they are in a given one.
 
     Returns (y [B, T, D] in x's dtype, final [N, D] fp32, states). The state is carried in fp32; a
-    given y must not overlap the inputs; at most 65534 sequences.
+    given y must not overlap the inputs.
     ``want_states`` keeps the state entering each 64-token chunk for ``gated_scan_bwd``:
     [B, ceil(T / 64), D] fp32; packed, sequence n's start at slot cu[n] // 64 + n of
     [1, T // 64 + N, D] and unused slots are 0.
