@@ -135,8 +135,8 @@ __device__ __forceinline__ float2 through_silu(float2 g, float2 u) {
 // the strip count for dx only, not for dw and db; rows past the sequence come as zeros, whose du
 // is 0.
 //
-// The rows come by TMA, a ring's worth (8 or 12) of both tensors at a time, into a ring of
-// stages of the warp's own: no block barrier, no address arithmetic, and the bytes in flight
+// The rows come by TMA, a ring's worth (fp32) or two of both tensors at a time, into stages of the
+// warp's own: no block barrier, no address arithmetic, and the bytes in flight
 // take no registers (loads of 4 rows ahead into registers left HBM at a third of its rate).
 // Where addresses or strides are no multiples of 16 bytes (TMA false), the lanes fill their own
 // slots.
@@ -144,8 +144,9 @@ template <typename T, int W>
 struct Bwd {
   static constexpr int kNB = (W - 1 + 2 * kBlockRows - 1) / kBlockRows;  // blocks of rows in a ring
   static constexpr int kRing = kNB * kBlockRows;
-  static constexpr int kTile = kRing * kCols * (int)sizeof(T);
-  static constexpr int kStages = sizeof(T) == 2 ? 4 : 2;
+  static constexpr int kStep = sizeof(T) == 2 ? 2 * kRing : kRing;  // rows of a stage
+  static constexpr int kTile = kStep * kCols * (int)sizeof(T);
+  static constexpr int kStages = 2;
   static constexpr int kBytes = kWarps * kStages * 2 * kTile;
 };
 
@@ -153,7 +154,7 @@ template <typename T, int W, bool ACT, bool TMA>
 __global__ void __launch_bounds__(32 * kWarps, W <= 5 ? 3 : 2)
     conv_bwd(const __grid_constant__ BwdArgs p, const __grid_constant__ BwdMaps tm) {
   using C = Bwd<T, W>;
-  constexpr int RB = kBlockRows, RING = C::kRing, NS = C::kStages;
+  constexpr int RB = kBlockRows, RING = C::kRing, STEP = C::kStep, NS = C::kStages;
   extern __shared__ __align__(128) uint8_t stages[];
   __shared__ float2 fold[kWarps][32];
   __shared__ __align__(8) uint64_t full[kWarps][NS];
@@ -168,15 +169,15 @@ __global__ void __launch_bounds__(32 * kWarps, W <= 5 ? 3 : 2)
     fence_mbar_init();
   }
   __syncwarp();
-  const int steps = t0 < t1 ? (t1 - t0 + W - 1 + RING - 1) / RING : 0;
+  const int steps = t0 < t1 ? (t1 - t0 + W - 1 + STEP - 1) / STEP : 0;
   bool ok = true;
   auto ask = [&](int j) {
     if (j >= steps || !ok) return;
     uint64_t* bar = &full[warp][j % NS];
     uint8_t* slot = ring + (j % NS) * 2 * C::kTile;
     mbar_arrive_expect_tx(bar, 2 * C::kTile);
-    tma_load_3d(slot, &tm.x, bar, blockIdx.x * kCols, t0 + j * RING, blockIdx.z);
-    tma_load_3d(slot + C::kTile, &tm.dy, bar, blockIdx.x * kCols, t0 + j * RING, blockIdx.z);
+    tma_load_3d(slot, &tm.x, bar, blockIdx.x * kCols, t0 + j * STEP, blockIdx.z);
+    tma_load_3d(slot + C::kTile, &tm.dy, bar, blockIdx.x * kCols, t0 + j * STEP, blockIdx.z);
   };
   if (TMA && lane == 0)
     for (int j = 0; j < NS; ++j) ask(j);
@@ -197,12 +198,12 @@ __global__ void __launch_bounds__(32 * kWarps, W <= 5 ? 3 : 2)
   for (int k = 1; k < W; ++k)  // the rows before the strip
     if (on && t0 < t1 && t0 - k >= 0) xw[RING - k] = load_pair<T, TMA>(x + (t0 - k) * p.xt, two);
   for (int j = 0; j < steps; ++j) {
-    const int tb = t0 + j * RING;
+    const int tb = t0 + j * STEP;
     uint8_t* slot = ring + (j % NS) * 2 * C::kTile + 2 * lane * (int)sizeof(T);
     if constexpr (TMA) {
       if (ok) ok = mbar_wait(&full[warp][j % NS], (j / NS) & 1, &g_status_conv_grad);
     } else {
-      for (int k = 0; k < RING; ++k) {
+      for (int k = 0; k < STEP; ++k) {
         const bool there = on && tb + k < p.S;
         float2 xv = f2(0.f), gv = f2(0.f);
         if (there) {
@@ -214,8 +215,9 @@ __global__ void __launch_bounds__(32 * kWarps, W <= 5 ? 3 : 2)
       }
     }
 #pragma unroll
-    for (int i = 0; i < C::kNB; ++i) {
+    for (int i = 0; i < STEP / RB; ++i) {
       const int t = tb + i * RB, r0 = i * RB + RING;  // ring index of row t
+      if (t >= t1 + W - 1) break;
 #pragma unroll
       for (int k = 0; k < RB; ++k) {
         xw[(r0 + k) % RING] = get_pair<T>(slot + (i * RB + k) * kCols * sizeof(T));
@@ -258,10 +260,11 @@ __global__ void __launch_bounds__(32 * kWarps, W <= 5 ? 3 : 2)
         }
       }
     }
-    dx += (long long)RING * p.D;
+    dx += (long long)STEP * p.D;
     __syncwarp();  // the stage has been read
     if (TMA && lane == 0) ask(j + NS);
   }
+  let_dependents_launch();
   // The strips' sums, added in the order of the rows.
   float* part = p.part + ((long long)blockIdx.z * gridDim.y + blockIdx.y) * (W + 1) * p.D;
 #pragma unroll
@@ -291,12 +294,22 @@ struct StoreGrads {
   }
 };
 
-// Rows of a warp's strip: long ones, of which the halo is little, where there are enough.
+// Rows of a warp's strip: blocks of a launch take about as long, so what counts is how many rounds
+// of resident blocks (three an SM) there are and what one takes: the strip's rows, and about 12
+// more for the halo, the first loads and the sums.
 int strip_rows(int B, int S, int D) {
-  const long long cols = (long long)B * ((D + kCols - 1) / kCols);
-  int rows = 128;
-  while (rows > 16 && cols * ((S + kWarps * rows - 1) / (kWarps * rows)) < 2ll * sm_count()) rows /= 2;
-  return rows;
+  const long long cols = (long long)B * ((D + kCols - 1) / kCols), slots = 3ll * sm_count();
+  int best = 16;
+  long long least = -1;
+  for (int rows = 16; rows <= 256; rows += kBlockRows) {
+    const long long blocks = cols * ((S + (long long)kWarps * rows - 1) / (kWarps * rows));
+    const long long cost = (blocks + slots - 1) / slots * (rows + 12);
+    if (least < 0 || cost < least) {
+      least = cost;
+      best = rows;
+    }
+  }
+  return best;
 }
 
 template <typename F>
@@ -363,8 +376,8 @@ int launch_bwd(const BwdArgs& p, dim3 grid, int B, int W, bool act, int dtype, c
     constexpr int kW = decltype(w)::value;
     using C = Bwd<T, kW>;
     BwdMaps tm{};
-    const bool tma = (bits & 15) == 0 && encode(&tm.x, dtype, p.x, p.xb, p.xt, B, p.S, p.D, C::kRing) == THM_OK &&
-                     encode(&tm.dy, dtype, p.dy, p.gb, p.gt, B, p.S, p.D, C::kRing) == THM_OK;
+    const bool tma = (bits & 15) == 0 && encode(&tm.x, dtype, p.x, p.xb, p.xt, B, p.S, p.D, C::kStep) == THM_OK &&
+                     encode(&tm.dy, dtype, p.dy, p.gb, p.gt, B, p.S, p.D, C::kStep) == THM_OK;
     auto k = tma ? (act ? conv_bwd<T, kW, true, true> : conv_bwd<T, kW, false, true>)
                  : (act ? conv_bwd<T, kW, true, false> : conv_bwd<T, kW, false, false>);
     if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes) != cudaSuccess) {
@@ -436,6 +449,5 @@ extern "C" int thm_causal_conv1d_bwd(const void* x, const float* weight, const f
                                     : convg::launch_bwd<float>(p, grid, B, W, act, dtype, st);
     if (e != THM_OK) return e;
   }
-  sum_parts(workspace, parts, (W + 1) * D, convg::StoreGrads{dweight, dbias, D, W}, st);
-  return check_launch();
+  return sum_parts(workspace, parts, (W + 1) * D, convg::StoreGrads{dweight, dbias, D, W}, st);
 }

@@ -779,6 +779,7 @@ __global__ void __launch_bounds__(32 * kWarps, Bwd<T>::kPerSm)
       grad_rows(std::false_type());
   }
   if (nblk > 1) cluster_barrier();  // as in the forward kernel, of dh0 and dfinal
+  let_dependents_launch();
   // ddecay over the block's warps, in order.
   __syncthreads();
   back[0][warp][lane] = ddecay;
@@ -1002,6 +1003,5 @@ extern "C" int thm_gated_scan_bwd(const void* x, const void* r, const void* i, c
                                     : gscan::run_bwd<float>(p, B, seqs, dtype, n, st);
     if (e != THM_OK) return e;
   }
-  sum_parts(workspace, parts, D, gscan::StoreColumn{ddecay}, st);
-  return check_launch();
+  return sum_parts(workspace, parts, D, gscan::StoreColumn{ddecay}, st);
 }

@@ -334,6 +334,7 @@ __global__ void __launch_bounds__(max_threads(VEC, NV), (VEC * NV == 8 && sizeof
     dz += ostep;
   }
   if (p.part == nullptr) return;
+  let_dependents_launch();
   // One row of dw (and db) sums for the block: the block's rows are added in order.
   const int span = p.gpc * p.G, first = blockIdx.x * span;
   const int npass = (FLAGS & kBias) != 0 ? 2 : 1;
@@ -538,8 +539,7 @@ extern "C" int thm_group_norm_bwd(const void* x, const void* gate, const float* 
     rows = (int)q.grid.y;
   }
   if (params) {
-    sum_parts(workspace, rows, bias != nullptr ? 2 * C : C, gnorm::StoreParams{dweight, dbias, C}, st);
-    return check_launch();
+    return sum_parts(workspace, rows, bias != nullptr ? 2 * C : C, gnorm::StoreParams{dweight, dbias, C}, st);
   }
   return THM_OK;
 }

@@ -74,6 +74,11 @@ __device__ __forceinline__ void silu_grad(float x, float& y, float& dy) {
   dy = s * (1.f + x * (1.f - s));
 }
 
+// A kernel's blocks say that a launch which was allowed to start early may do so; that one waits
+// until all of them have ended and their writes are there.
+__device__ __forceinline__ void let_dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // out[map(c)] = sum over the n rows of part [n, M], column c: the second half of a
 // reduction over all tokens whose first half left one row per block. 32 threads share a
 // column (rows k, k + 32, ... each) and are added in a fixed order, so the result does not
@@ -81,6 +86,7 @@ __device__ __forceinline__ void silu_grad(float x, float& y, float& dy) {
 template <typename Map>
 __global__ void __launch_bounds__(1024) sum_parts_kernel(const float* __restrict__ part, int n, int M, Map map) {
   __shared__ float sh[32][33];
+  wait_for_predecessor();
   const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   float acc = 0.f;
@@ -97,9 +103,23 @@ __global__ void __launch_bounds__(1024) sum_parts_kernel(const float* __restrict
   if (lane == 0 && blockIdx.x * 32 + k < M) map(blockIdx.x * 32 + k, acc);
 }
 
+// Launched so that it may be set up while the kernel that leaves `part` ends. Returns a thm_status.
 template <typename Map>
-inline void sum_parts(const float* part, int n, int M, Map map, cudaStream_t st) {
-  sum_parts_kernel<<<(M + 31) / 32, 1024, 0, st>>>(part, n, M, map);
+inline int sum_parts(const float* part, int n, int M, Map map, cudaStream_t st) {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3((M + 31) / 32);
+  cfg.blockDim = dim3(1024);
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, sum_parts_kernel<Map>, part, n, M, map) != cudaSuccess) {
+    cudaGetLastError();
+    return THM_ERR_CUDA;
+  }
+  return THM_OK;
 }
 
 }  // namespace thm
