@@ -26,11 +26,16 @@ def _on_input_device(fn):
         t = args[0] if args else None
         if not isinstance(t, torch.Tensor):
             t = next((a for a in (*args, *kw.values()) if torch.is_tensor(a)), None)
-        if t is not None and t.is_cuda and t.device.index != torch.cuda.current_device():
+        if t is not None and t.is_cuda and t.get_device() != torch.cuda.current_device():
             with torch.cuda.device(t.device):
                 return fn(*args, **kw)
         return fn(*args, **kw)
     return wrapped
+
+
+def _on_gpu(x):
+    """x is a CUDA tensor (the others are checked against its device)."""
+    assert x.is_cuda, "theorem_b200 ops need CUDA tensors (there is no CPU fallback)"
 
 
 def _cuda(*ts):
@@ -346,7 +351,7 @@ def chunk_local_cumsum(g_inc, scale: float = 1.0, out=None):
 # sets the pace: the checks are plain comparisons, and messages are only formed on failure.
 def _like(name, t, ref):
     """t's strides; t has ref's shape, dtype and device, and unit stride over channels."""
-    assert t.shape == ref.shape and t.dtype == ref.dtype and t.device == ref.device, \
+    assert t.shape == ref.shape and t.dtype is ref.dtype and t.get_device() == ref.get_device(), \
         f"{name} must be {tuple(ref.shape)} {ref.dtype} on {ref.device}"
     st = t.stride()
     assert st[-1] == 1 or t.shape[-1] <= 1, f"{name} must have unit stride over channels"
@@ -355,7 +360,7 @@ def _like(name, t, ref):
 
 def _dense(name, t, ref, shape, dtype):
     """t is a contiguous ``shape`` of ``dtype`` on ref's device."""
-    assert t.shape == shape and t.dtype == dtype and t.device == ref.device and t.is_contiguous(), \
+    assert t.shape == shape and t.dtype is dtype and t.get_device() == ref.get_device() and t.is_contiguous(), \
         f"{name} must be a contiguous {tuple(shape)} {dtype} on {ref.device}"
 
 
@@ -376,7 +381,7 @@ def _channel_last(x):
 
 def _scan_args(x, r, i, decay, cu_seqlens):
     """(B, T, D, sequences, shape of the chunk states, batch and time strides of x, r, i)."""
-    _cuda(x, r, i, decay, cu_seqlens)
+    _on_gpu(x)
     shape = x.shape
     assert len(shape) == 3, "x must be [B, T, D]"
     strides = _channel_last(x)[:2] + _like("r", r, x)[:2] + _like("i", i, x)[:2]
@@ -415,7 +420,6 @@ def gated_scan(x, r, i, decay, h0=None, cu_seqlens=None, want_states: bool = Fal
     """
     B, T, D, n, sshape, strides = _scan_args(x, r, i, decay, cu_seqlens)
     if h0 is not None:
-        _cuda(h0)
         _dense("h0", h0, x, (n, D), torch.float32)
     fresh = y is None
     if fresh:
@@ -450,7 +454,6 @@ def gated_scan_bwd(x, r, i, decay, states, dy, dfinal=None, cu_seqlens=None, dx=
     repeat bit for bit.
     """
     B, T, D, n, sshape, strides = _scan_args(x, r, i, decay, cu_seqlens)
-    _cuda(states, dy, dfinal)
     strides += _like("dy", dy, x)[:2]
     _dense("states", states, x, sshape, torch.float32)
     if dfinal is not None:
@@ -490,7 +493,7 @@ def _rows(name, t):
 
 
 def _norm_args(x, group, weight, bias, gate, activation):
-    _cuda(x, weight, bias, gate)
+    _on_gpu(x)
     assert x.dim() >= 1, "x must be [..., C]"
     _channel_last(x)
     C = x.shape[-1]
@@ -541,7 +544,6 @@ def group_norm_bwd(x, dy, group: int, weight=None, bias=None, gate=None, activat
     fixed order, so results repeat bit for bit.
     """
     C = _norm_args(x, group, weight, bias, gate, activation)
-    _cuda(dy)
     _like("dy", dy, x)
     R, xs = _rows("x", x)
     gs = _rows("dy", dy)[1]
@@ -562,7 +564,7 @@ def group_norm_bwd(x, dy, group: int, weight=None, bias=None, gate=None, activat
 
 
 def _conv_args(x, weight, bias, activation):
-    _cuda(x, weight, bias)
+    _on_gpu(x)
     assert x.dim() == 3, "x must be [B, S, D]"
     strides = _channel_last(x)[:2]
     B, S, D = x.shape
@@ -586,7 +588,6 @@ def causal_conv1d_step(x, state, weight, bias, activation=None, out=None, state_
     """
     B, S, D, W, strides = _conv_args(x, weight, bias, activation)
     assert S <= 64, f"S={S}: the carried-state form takes at most 64 tokens (causal_conv1d takes long runs)"
-    _cuda(state)
     _dense("state", state, x, (B, W - 1, D), x.dtype)
     if out is None:
         out = _empty(x, x.shape, x.dtype)
@@ -611,7 +612,6 @@ def causal_conv1d_bwd(x, weight, bias, dy, activation=None):
     W <= 8. Sums over tokens are in fp32 in a fixed order, so results repeat bit for bit.
     """
     B, S, D, W, strides = _conv_args(x, weight, bias, activation)
-    _cuda(dy)
     strides += _like("dy", dy, x)[:2]
     dx = _empty(x, x.shape, x.dtype)
     dweight = torch.empty(D, W, device=x.device, dtype=torch.float32)
