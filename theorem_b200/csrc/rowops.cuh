@@ -1,6 +1,6 @@
 // rowops.cuh -- device helpers of the channel-last row kernels (gated scan, group
-// norm, conv step and backward): vectors of channels in and out of registers, and
-// the sigmoid / SiLU pair with its derivative.
+// norm, conv step and backward): vectors of channels in and out of registers, sigmoid and
+// SiLU, and the second half of sums over all tokens.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -62,16 +62,10 @@ __device__ __forceinline__ float sigmoid(float x) {
   return rcp_approx(1.f + exp_for<T>(-x));
 }
 
-// silu(x) = x s and silu'(x) = s (1 + x (1 - s)), s = sigmoid(x).
+// silu(x) = x sigmoid(x).
 template <typename T>
 __device__ __forceinline__ float silu_of(float x) {
   return x * sigmoid<T>(x);
-}
-template <typename T>
-__device__ __forceinline__ void silu_grad(float x, float& y, float& dy) {
-  const float s = sigmoid<T>(x);
-  y = x * s;
-  dy = s * (1.f + x * (1.f - s));
 }
 
 // A kernel's blocks say that a launch which was allowed to start early may do so; that one waits
