@@ -203,15 +203,31 @@ __global__ void __launch_bounds__(32 * kWarps, W <= 5 ? 3 : 2)
     if constexpr (TMA) {
       if (ok) ok = mbar_wait(&full[warp][j % NS], (j / NS) & 1, &g_status_conv_grad);
     } else {
-      for (int k = 0; k < STEP; ++k) {
-        const bool there = on && tb + k < p.S;
-        float2 xv = f2(0.f), gv = f2(0.f);
-        if (there) {
-          xv = load_pair<T, false>(x + (tb + k) * p.xt, two);
-          gv = load_pair<T, false>(dy + (tb + k) * p.gt, two);
+// Four rows at a time, loads without conditions so that all are in flight at once: rows past the
+// sequence repeat its last and are then taken as zeros, a second channel that is not there repeats
+// the first.
+#pragma unroll
+      for (int k0 = 0; k0 < STEP; k0 += RB) {
+        T v[2][RB][2];
+        const int next = two ? 1 : 0;
+        if (on) {
+#pragma unroll
+          for (int k = 0; k < RB; ++k) {
+            const long long t = min(tb + k0 + k, p.S - 1);
+            v[0][k][0] = x[t * p.xt];
+            v[0][k][1] = x[t * p.xt + next];
+            v[1][k][0] = dy[t * p.gt];
+            v[1][k][1] = dy[t * p.gt + next];
+          }
+#pragma unroll
+          for (int k = 0; k < RB; ++k)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              const float2 f = make_float2(to_f32<T>(v[n][k][0]), to_f32<T>(v[n][k][1]));
+              store_pair<T, true>(reinterpret_cast<T*>(slot + n * C::kTile + (k0 + k) * kCols * sizeof(T)),
+                                  tb + k0 + k < p.S ? f : f2(0.f), true);
+            }
         }
-        store_pair<T, true>(reinterpret_cast<T*>(slot + k * kCols * sizeof(T)), xv, true);
-        store_pair<T, true>(reinterpret_cast<T*>(slot + C::kTile + k * kCols * sizeof(T)), gv, true);
       }
     }
 #pragma unroll

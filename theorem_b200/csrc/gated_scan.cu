@@ -89,8 +89,14 @@ struct RawPair<float> {
 // The pair at p as one access (PAIRED: addresses and strides allow it) or as two.
 template <typename T, bool PAIRED>
 __device__ __forceinline__ RawPair<T> load_pair(const T* p, bool two) {
-  if constexpr (PAIRED) return *reinterpret_cast<const RawPair<T>*>(p);
-  return RawPair<T>::of(make_float2(to_f32<T>(p[0]), two ? to_f32<T>(p[1]) : 0.f));
+  if constexpr (PAIRED) {
+    return *reinterpret_cast<const RawPair<T>*>(p);
+  } else if constexpr (sizeof(T) == 2) {
+    const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
+    return {u[0] | (two ? (uint32_t)u[1] << 16 : 0u)};
+  } else {
+    return {make_float2(p[0], two ? p[1] : 0.f)};
+  }
 }
 template <typename T, bool PAIRED>
 __device__ __forceinline__ void store_pair(T* p, float2 f, bool two) {
@@ -422,11 +428,23 @@ template <typename T>
 __device__ __forceinline__ void put_pair(uint8_t* tile, int k, float2 f) {
   *reinterpret_cast<RawPair<T>*>(tile + k * kCols * sizeof(T)) = RawPair<T>::of(f);
 }
-// A lane's first `rows` rows of a tensor into its slots, without TMA.
+// A lane's first `rows` rows of a tensor into its slots, without TMA. Loads without conditions, so
+// that all are in flight at once: rows past the last repeat it (the caller overwrites them), and a
+// second channel that is not there repeats the first.
 template <typename T>
 __device__ __forceinline__ void fill(uint8_t* tile, const void* t, long long first, long long stride, int rows, bool two) {
+  if (rows == 0) return;
   const T* q = static_cast<const T*>(t) + first;
-  for (int k = 0; k < rows; ++k) put_pair<T>(tile, k, load_pair<T, false>(q + k * stride, two).get());
+  const int next = two ? 1 : 0;
+  T v[kRows][2];
+#pragma unroll
+  for (int k = 0; k < kRows; ++k) {
+    const T* row = q + min(k, rows - 1) * stride;
+    v[k][0] = row[0];
+    v[k][1] = row[next];
+  }
+#pragma unroll
+  for (int k = 0; k < kRows; ++k) put_pair<T>(tile, k, make_float2(to_f32<T>(v[k][0]), to_f32<T>(v[k][1])));
 }
 
 // Stages, and resident blocks an SM: for bf16 three of 80 registers a thread forward, two of 128
