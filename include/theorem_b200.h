@@ -221,7 +221,7 @@ int thm_sp_prefix_fold(const float* M, const float* S, const float* x0, float* o
  *
  * x, r, i, dy [B,T,D] in `dtype`, unit stride over D, strides *_bs (batch) and
  * *_ts (time) in elements; y, dx, dr, di [B,T,D] contiguous in `dtype`; decay
- * [D] >= 0, h0, final_state, dfinal, dh0 [nseq,D] fp32 (h0, final_state, states,
+ * [D] >= 0 and finite, h0, final_state, dfinal, dh0 [nseq,D] fp32 (h0, final_state, states,
  * dfinal, dh0 may be NULL; final_state may be h0, dh0 may be dfinal). A token
  * with r < -43 (-inf) holds the state and gets zero gradients, whatever x and i
  * are there.
@@ -281,7 +281,7 @@ int thm_group_norm_bwd_parts(long long R, int C, int G);
  *   (THM_LAYOUT_BSD, l2norm_group 0); sums over tokens in a fixed order.
  *   workspace [thm_causal_conv1d_bwd_parts(B, S, D), W + 1, D] fp32.
  * x, dy in `dtype`, unit stride over D, strides *_bs, *_ts in elements; out, dx,
- * states contiguous; weight, bias fp32; 1 <= W <= 8.
+ * states contiguous; weight, bias fp32; 1 <= W <= 8; bwd: B <= 65535.
  * ------------------------------------------------------------------------- */
 int thm_causal_conv1d_step(const void* x, const void* state, const float* weight, const float* bias, void* out,
                            void* state_out, long long x_bs, long long x_ts, int B, int S, int D, int W, int dtype,

@@ -80,6 +80,23 @@ def test_decays_past_the_plain_range(T, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("T", [5, 200])
+def test_large_decay_behind_a_closed_gate(T, dtype):
+    """A decay of hundreds with a nearly closed gate is an ordinary memory: decay sigmoid(r) counts,
+    not decay."""
+    from theorem_b200 import ops
+    B, D = 2, 64
+    x, r, i, decay, h0, dy, df = _inputs(B, T, D, dtype, seed=T)
+    decay = 100.0 + 40.0 * torch.arange(D).float()
+    r = (r - 8.0).to(dtype)
+    args = _d(x, r, i, decay)
+    out = ops.gated_scan(*args, h0=h0.to(DEV), want_states=True)
+    _check_fwd(x, r, i, decay, h0, out, dtype)
+    grads = ops.gated_scan_bwd(*args, out[2], dy.to(DEV), dfinal=df.to(DEV))
+    _check_bwd(x, r, i, decay, h0, dy, df, grads, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("T", [1, 100])
 def test_defaults_without_h0_and_dfinal(T, dtype):
     from theorem_b200 import ops

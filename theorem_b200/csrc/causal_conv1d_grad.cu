@@ -171,8 +171,10 @@ __global__ void __launch_bounds__(32 * kWarps, W <= 5 ? 3 : 2)
   __syncwarp();
   const int steps = t0 < t1 ? (t1 - t0 + W - 1 + STEP - 1) / STEP : 0;
   bool ok = true;
+  int asked = 0, failed = 0;
   auto ask = [&](int j) {
     if (j >= steps || !ok) return;
+    asked = j + 1;
     uint64_t* bar = &full[warp][j % NS];
     uint8_t* slot = ring + (j % NS) * 2 * C::kTile;
     mbar_arrive_expect_tx(bar, 2 * C::kTile);
@@ -201,7 +203,10 @@ __global__ void __launch_bounds__(32 * kWarps, W <= 5 ? 3 : 2)
     const int tb = t0 + j * STEP;
     uint8_t* slot = ring + (j % NS) * 2 * C::kTile + 2 * lane * (int)sizeof(T);
     if constexpr (TMA) {
-      if (ok) ok = mbar_wait(&full[warp][j % NS], (j / NS) & 1, &g_status_conv_grad);
+      if (ok) {
+        ok = mbar_wait(&full[warp][j % NS], (j / NS) & 1, &g_status_conv_grad);
+        failed = j;
+      }
     } else {
 // Four rows at a time, loads without conditions so that all are in flight at once: rows past the
 // sequence repeat its last and are then taken as zeros, a second channel that is not there repeats
@@ -280,6 +285,8 @@ __global__ void __launch_bounds__(32 * kWarps, W <= 5 ? 3 : 2)
     __syncwarp();  // the stage has been read
     if (TMA && lane == 0) ask(j + NS);
   }
+  if (TMA && lane == 0)  // after a wait that ran out: once more for what is still on its way here
+    for (int j = failed; !ok && j < asked; ++j) mbar_wait(&full[warp][j % NS], (j / NS) & 1, &g_status_conv_grad);
   let_dependents_launch();
   // The strips' sums, added in the order of the rows.
   float* part = p.part + ((long long)blockIdx.z * gridDim.y + blockIdx.y) * (W + 1) * p.D;
@@ -351,7 +358,7 @@ int check_sizes(int B, int S, int D, int W, int act, int dtype) {
   if (B < 0 || S < 0 || D < 0 || W <= 0) return THM_ERR_INVALID;
   if (act != THM_ACT_NONE && act != THM_ACT_SILU) return THM_ERR_INVALID;
   if (dtype != THM_F32 && dtype != THM_BF16) return THM_ERR_INVALID;
-  if (W > kMaxW) return THM_ERR_UNSUPPORTED;
+  if (W > kMaxW || S > 1 << 30) return THM_ERR_UNSUPPORTED;
   return THM_OK;
 }
 

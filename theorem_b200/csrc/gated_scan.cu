@@ -143,12 +143,17 @@ __device__ __forceinline__ float min_nan(float a, float b) {  // NaN when either
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
 // Below this gate logit a token holds the state: sigmoid(r) < 2^-62 changes no fp32 state of
 // the size of x by even 1e-2 of a rounding step, and x and i may hold anything.
 constexpr float kHoldBelow = -43.f;
-// e^-87 is the smallest decay of one token that stays a normal number.
-constexpr float kMaxDecay = 87.f;
+// e^-87 is the smallest decay of one token that stays a normal number: L is limited to it.
+constexpr float kMaxL = 87.f;
 
 // A token of two channels is computed in one of two ways. PLAIN tokens have 1e-6 <= decay <= 1
 // on every channel of the warp and no held token among the warp's 8 (both checked once a tile,
@@ -182,7 +187,7 @@ __device__ __forceinline__ void sigmoids(float2 r, float2 i, float2& s, float2& 
   if constexpr (!PLAIN) s = make_float2(r.x < kHoldBelow ? 0.f : s.x, r.y < kHoldBelow ? 0.f : s.y);
 }
 
-// a = e^-L and t = a - 1 from nL = -L, 0 <= L <= 87 (PLAIN: 1), both to fp32 accuracy and
+// a = e^-L and t = a - 1 from nL = -L, L >= 0 (PLAIN: L <= 1), both to fp32 accuracy and
 // without the special-function unit, whose exponential is off by up to 2^-22, always to the same
 // side: in a product over a memory of hundreds of tokens that adds up. e^f - 1 is a polynomial
 // fitted by reweighted least squares, over -1 <= f <= 0 (largest relative error 2.7e-9) or, after
@@ -199,6 +204,7 @@ __device__ __forceinline__ void decay_pair(float2 nL, float2& a, float2& t) {
     t = __ffma2_rn(__fmul2_rn(nL, nL), c, nL);
     a = __fadd2_rn(t, f2(1.f));
   } else {
+    nL = make_float2(max_nan(nL.x, -kMaxL), max_nan(nL.y, -kMaxL));
     constexpr float kMagic = 12582912.f;  // 1.5 2^23: adding it rounds to an integer in the low bits
     const float2 km = __ffma2_rn(nL, f2(1.4426950408889634f), f2(kMagic));
     const float2 k = __fadd2_rn(km, f2(-kMagic));
@@ -216,7 +222,7 @@ __device__ __forceinline__ void decay_pair(float2 nL, float2& a, float2& t) {
 }
 __device__ __forceinline__ float2 m2_of(float2 t) { return __fmul2_rn(t, __ffma2_rn(t, f2(-1.f), f2(-2.f))); }
 
-// One token of two channels: h -> a h + b. `ndecay` is -decay, limited to kMaxDecay.
+// One token of two channels: h -> a h + b. `ndecay` is -decay.
 template <typename T, bool PLAIN>
 __device__ __forceinline__ void token_pair(float2 x, float2 r, float2 i, float2 ndecay, float2& a, float2& b) {
   float2 s, p, t;
@@ -253,7 +259,7 @@ __device__ __forceinline__ bool any_held(RawPair<T> m) {
 // -decay of a lane's channels; channels that it does not have do not keep its warp from PLAIN.
 __device__ __forceinline__ float2 neg_decay(const Lane& ln, const float* decay) {
   const float2 d = ln.load(decay);
-  return make_float2(ln.on ? -min_nan(d.x, kMaxDecay) : -1.f, ln.two ? -min_nan(d.y, kMaxDecay) : -1.f);
+  return make_float2(ln.on ? -d.x : -1.f, ln.two ? -d.y : -1.f);
 }
 __device__ __forceinline__ bool plain_decays(float2 nd) {
   return __all_sync(0xffffffffu, -nd.x >= kPlainDecayMin && -nd.x <= kPlainDecayMax && -nd.y >= kPlainDecayMin &&
@@ -395,9 +401,10 @@ struct Ring {
   static constexpr int kBytes = NSTAGE * kStage;
   uint8_t* base;
   uint64_t* full;
+  int asked, failed;  // steps asked for (one thread), and the first whose wait ran out
   bool ok;
 
-  __device__ __forceinline__ Ring(uint8_t* b, uint64_t* f) : base(b), full(f), ok(true) {
+  __device__ __forceinline__ Ring(uint8_t* b, uint64_t* f) : base(b), full(f), asked(0), failed(0), ok(true) {
     if (threadIdx.x == 0) {
       for (int k = 0; k < NSTAGE; ++k) mbar_init(&full[k], 1);
       fence_mbar_init();
@@ -408,6 +415,7 @@ struct Ring {
   // One thread: ask for the tiles of step j, rows from `row` of batch entry `batch`.
   __device__ __forceinline__ void ask(const CUtensorMap* in, int j, int col, int row, int batch) {
     if (!ok) return;
+    asked = j + 1;
     uint64_t* bar = &full[j % NSTAGE];
     mbar_arrive_expect_tx(bar, kStage);
 #pragma unroll
@@ -416,7 +424,14 @@ struct Ring {
   // All threads: the tiles of step j are there. After a wait that ran out no further one is
   // entered and nothing more is asked for: the kernel ends, and the device status says why.
   __device__ __forceinline__ void wait(int j, unsigned* status) {
-    if (ok) ok = mbar_wait(&full[j % NSTAGE], (j / NSTAGE) & 1, status);
+    if (!ok) return;
+    ok = mbar_wait(&full[j % NSTAGE], (j / NSTAGE) & 1, status);
+    failed = j;
+  }
+  // The thread that asked, before it leaves: after a wait that ran out, once more for what is still
+  // on its way into this block's memory.
+  __device__ __forceinline__ void drain(unsigned* status) {
+    for (int j = failed; !ok && j < asked; ++j) mbar_wait(&full[j % NSTAGE], (j / NSTAGE) & 1, status);
   }
 };
 
@@ -615,6 +630,7 @@ __global__ void __launch_bounds__(32 * kWarps, Fwd<T, CHAIN>::kPerSm)
       }
     }
   }
+  if (TMA && threadIdx.x == 0) ring.drain(&g_status_scan);
   // No block leaves while another may still send to it, and final_state may be h0: every block has
   // read that by now.
   if (CHAIN) cluster_barrier();
@@ -796,6 +812,7 @@ __global__ void __launch_bounds__(32 * kWarps, Bwd<T>::kPerSm)
     else
       grad_rows(std::false_type());
   }
+  if (TMA && threadIdx.x == 0) ring.drain(&g_status_scan);
   if (nblk > 1) cluster_barrier();  // as in the forward kernel, of dh0 and dfinal
   let_dependents_launch();
   // ddecay over the block's warps, in order.
@@ -847,16 +864,17 @@ constexpr int kDirectTokens = 16;
 // pairs of tiles for. Measured on bf16, forward: B8 T4096 D2048 (256 sequences of channels)
 // 127 us alone, 141 with two blocks each, 158 with eight; B16 T8192 446 us alone, 484 with two;
 // B1 T131072 2473 us alone, 578 with eight. Packed lengths are not known here: the longest of n
-// random pieces has about (1 + ln n) / n of the rows, and the rest of the work fits beside it
-// (65537 rows in 5 pieces backward: 902 us alone, 622, 506 and 517 with two, four, eight; 20011
-// rows in 37 pieces forward fp32: 80, 86, 111, 164).
+// random pieces has about (1 + ln n) / n of the rows, and the rest of the work fits beside it; of
+// a few pieces one may have nearly all, and more blocks than needed cost little (65537 rows in 5
+// pieces backward: 902 us alone, 622, 506 and 517 with two, four, eight; other cuts with four up
+// to 618; 20011 rows in 37 pieces forward fp32: 80, 86, 111, 164).
 int cluster_blocks(double chains, double tokens, int slots) {
   int n = 1;
   while (n < 8 && chains * n * 2 <= slots && tokens / kChunk >= 4 * n) n *= 2;
   return n;
 }
 int packed_blocks(int T, int cols, int nseq, int slots) {
-  const double longest = (1. + std::log((double)nseq)) / nseq;
+  const double longest = nseq <= 8 ? 1. : (1. + std::log((double)nseq)) / nseq;
   return cluster_blocks(cols / longest, T * longest, slots);
 }
 
@@ -956,6 +974,7 @@ int check_sizes(int B, int T, int D, int nseq, const int* cu, int dtype) {
   if (B < 0 || T < 0 || D < 0 || nseq < 0) return THM_ERR_INVALID;
   if (dtype != THM_F32 && dtype != THM_BF16) return THM_ERR_INVALID;
   if (cu != nullptr ? B != 1 : nseq != B) return THM_ERR_INVALID;
+  if (T > 1 << 30) return THM_ERR_UNSUPPORTED;  // rows, and those of a last round, count in 31 bits
   // (sequence, 64 channels) pairs, times the blocks of a cluster, are counted in 31 bits.
   if (((long long)nseq + 1) * ((D + kCols - 1) / kCols) >= 1ll << 27) return THM_ERR_UNSUPPORTED;
   return THM_OK;

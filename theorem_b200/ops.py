@@ -404,7 +404,7 @@ def gated_scan(x, r, i, decay, h0=None, cu_seqlens=None, want_states: bool = Fal
         a_t = exp(-decay sigmoid(r_t)),  h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(i_t) x_t
 
     x, r, i [B, T, D] fp32 or bf16 of one dtype, unit stride over D, any strides over B and
-    T; decay [D] fp32 >= 0; h0 [N, D] fp32 (zeros if None). Any T: T = 1 with ``final=h0`` is
+    T; decay [D] fp32, finite and >= 0; h0 [N, D] fp32 (zeros if None). Any T: T = 1 with ``final=h0`` is
     the in-place single-token step. A token with r < -43 (sigmoid(r) < 2^-62, -inf) holds the
     state, whatever x and i hold there (pad a batch with it and ``final`` is each sequence's own).
 
