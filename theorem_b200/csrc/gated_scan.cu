@@ -245,10 +245,15 @@ __device__ __forceinline__ RawPair<T> min_pair(RawPair<T> u, RawPair<T> v) {
     return {make_float2(fminf(u.v.x, v.v.x), fminf(u.v.y, v.v.y))};
   }
 }
-template <typename T>
-__device__ __forceinline__ RawPair<T> min_rows(const RawPair<T> (&r)[8]) {
-  return min_pair(min_pair(min_pair(r[0], r[1]), min_pair(r[2], r[3])),
-                  min_pair(min_pair(r[4], r[5]), min_pair(r[6], r[7])));
+template <typename T, int N>
+__device__ __forceinline__ RawPair<T> min_rows(const RawPair<T> (&r)[N]) {
+  RawPair<T> m[N / 2];
+#pragma unroll
+  for (int k = 0; k < N / 2; ++k) m[k] = min_pair(r[k], r[k + N / 2]);
+  if constexpr (N == 2)
+    return m[0];
+  else
+    return min_rows<T, N / 2>(m);
 }
 template <typename T>
 __device__ __forceinline__ bool any_held(RawPair<T> m) {
@@ -317,8 +322,7 @@ __global__ void __launch_bounds__(kDirectThreads) scan_direct(const Args p) {
 // sequence: block k takes tiles k, k + n, ... . Each round the blocks send their tiles' maps to
 // one another's shared memory, counted in by an mbarrier, so the chain along time costs one
 // such exchange for n tiles, and x, r, i are still read once.
-constexpr int kWarps = 8, kRows = 8, kCols = 64;
-static_assert(kWarps * kRows == kChunk, "a tile is a chunk");
+constexpr int kCols = 64;
 
 struct Maps {  // of x, r, i, dy, where TMA carries the tiles
   CUtensorMap in[4];
@@ -446,7 +450,7 @@ __device__ __forceinline__ void put_pair(uint8_t* tile, int k, float2 f) {
 // A lane's first `rows` rows of a tensor into its slots, without TMA. Loads without conditions, so
 // that all are in flight at once: rows past the last repeat it (the caller overwrites them), and a
 // second channel that is not there repeats the first.
-template <typename T>
+template <typename T, int kRows>
 __device__ __forceinline__ void fill(uint8_t* tile, const void* t, long long first, long long stride, int rows, bool two) {
   if (rows == 0) return;
   const T* q = static_cast<const T*>(t) + first;
@@ -467,13 +471,13 @@ __device__ __forceinline__ void fill(uint8_t* tile, const void* t, long long fir
 // holds two, without the room that finishing a round behind takes.
 template <typename T, bool CHAIN>
 struct Fwd {
-  static constexpr int kStages = 2, kPerSm = sizeof(T) == 2 && !CHAIN ? 3 : 2;
+  static constexpr int kStages = 2, kPerSm = sizeof(T) == 2 && !CHAIN ? 3 : 2, kWarps = CHAIN ? 4 : 8;
   static constexpr bool kBehind = CHAIN && sizeof(T) == 2;  // a tile is finished a round behind
   using R = Ring<T, 3, kStages>;
 };
 template <typename T>
 struct Bwd {
-  static constexpr int kStages = sizeof(T) == 2 ? 2 : 1, kPerSm = 2;
+  static constexpr int kStages = sizeof(T) == 2 ? 3 : 1, kPerSm = 2, kWarps = 4;
   using R = Ring<T, 4, kStages>;
 };
 
@@ -481,8 +485,9 @@ struct Bwd {
 // bf16 a block scans its next tile before it receives the last one's entering state, two tiles in
 // registers (B1 T131072 D2048: 618 -> 578 us).
 template <typename T, bool TMA, bool CHAIN>
-__global__ void __launch_bounds__(32 * kWarps, Fwd<T, CHAIN>::kPerSm)
+__global__ void __launch_bounds__(32 * Fwd<T, CHAIN>::kWarps, Fwd<T, CHAIN>::kPerSm)
     scan_tiles(const __grid_constant__ Args p, const __grid_constant__ Maps tm) {
+  constexpr int kWarps = Fwd<T, CHAIN>::kWarps, kRows = kChunk / kWarps;
   constexpr bool BEHIND = Fwd<T, CHAIN>::kBehind;
   constexpr int NS = Fwd<T, CHAIN>::kStages, NM = BEHIND ? 3 : 2, DEPTH = BEHIND ? 4 : 2;
   extern __shared__ __align__(128) uint8_t stages[];
@@ -526,9 +531,9 @@ __global__ void __launch_bounds__(32 * kWarps, Fwd<T, CHAIN>::kPerSm)
       if (tile < ntiles) ring.wait(j, &g_status_scan);
     } else if (ln.on) {
       const long long t = q.lo + row0;
-      fill<T>(xs, p.x, q.batch * p.xb + t * p.xt + ln.c, p.xt, have, ln.two);
-      fill<T>(rs, p.r, q.batch * p.rb + t * p.rt + ln.c, p.rt, have, ln.two);
-      fill<T>(is, p.i, q.batch * p.ib + t * p.it + ln.c, p.it, have, ln.two);
+      fill<T, kRows>(xs, p.x, q.batch * p.xb + t * p.xt + ln.c, p.xt, have, ln.two);
+      fill<T, kRows>(rs, p.r, q.batch * p.rb + t * p.rt + ln.c, p.rt, have, ln.two);
+      fill<T, kRows>(is, p.i, q.batch * p.ib + t * p.it + ln.c, p.it, have, ln.two);
     }
     for (int k = have; k < kRows; ++k) {  // rows past the sequence's end hold the state
       put_pair<T>(rs, k, f2(-INFINITY));
@@ -644,8 +649,9 @@ __global__ void __launch_bounds__(32 * kWarps, Fwd<T, CHAIN>::kPerSm)
 // backward maps only: every tile's entering state is known. x and dy are read again from the
 // tile after the barrier, so a stage is refilled at the next step's barrier.
 template <typename T, bool TMA>
-__global__ void __launch_bounds__(32 * kWarps, Bwd<T>::kPerSm)
+__global__ void __launch_bounds__(32 * Bwd<T>::kWarps, Bwd<T>::kPerSm)
     scan_bwd_tiles(const __grid_constant__ Args p, const __grid_constant__ Maps tm) {
+  constexpr int kWarps = Bwd<T>::kWarps, kRows = kChunk / kWarps;
   extern __shared__ __align__(128) uint8_t stages[];
   __shared__ __align__(16) float4 maps[2][kWarps][32];
   __shared__ __align__(16) float2 back[2][kWarps][32];
@@ -700,10 +706,10 @@ __global__ void __launch_bounds__(32 * kWarps, Bwd<T>::kPerSm)
       if (tile >= 0) ring.wait(j, &g_status_scan);
     } else if (ln.on) {
       const long long t = q.lo + row0;
-      fill<T>(xs, p.x, q.batch * p.xb + t * p.xt + ln.c, p.xt, have, ln.two);
-      fill<T>(rs, p.r, q.batch * p.rb + t * p.rt + ln.c, p.rt, have, ln.two);
-      fill<T>(is, p.i, q.batch * p.ib + t * p.it + ln.c, p.it, have, ln.two);
-      fill<T>(gs, p.dy, q.batch * p.gb + t * p.gt + ln.c, p.gt, have, ln.two);
+      fill<T, kRows>(xs, p.x, q.batch * p.xb + t * p.xt + ln.c, p.xt, have, ln.two);
+      fill<T, kRows>(rs, p.r, q.batch * p.rb + t * p.rt + ln.c, p.rt, have, ln.two);
+      fill<T, kRows>(is, p.i, q.batch * p.ib + t * p.it + ln.c, p.it, have, ln.two);
+      fill<T, kRows>(gs, p.dy, q.batch * p.gb + t * p.gt + ln.c, p.gt, have, ln.two);
     }
     for (int k = have; k < kRows; ++k) {
       put_pair<T>(rs, k, f2(-INFINITY));
@@ -886,7 +892,7 @@ int bwd_cluster(int T, int D, int nseq, bool packed, int dtype) {
 
 // `count` sequences of channels from `first` on, n blocks each.
 template <typename K>
-int launch_tiles(K kernel, Args p, const Maps& tm, int n, int first, int count, int smem, cudaStream_t st) {
+int launch_tiles(K kernel, int warps, Args p, const Maps& tm, int n, int first, int count, int smem, cudaStream_t st) {
   p.first = first;
   p.count = count;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
@@ -896,7 +902,7 @@ int launch_tiles(K kernel, Args p, const Maps& tm, int n, int first, int count, 
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
   cfg.gridDim = dim3((unsigned)(n * count));
-  cfg.blockDim = dim3(32 * kWarps);
+  cfg.blockDim = dim3(32 * warps);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -933,10 +939,10 @@ int run_fwd(Args p, int B, int seqs, int dtype, cudaStream_t st) {
   static_assert(smem == Fwd<T, true>::R::kBytes);
   auto run = [&](int n, int first, int cnt) {
     if (n > 1)
-      return tma ? launch_tiles(scan_tiles<T, true, true>, p, tm, n, first, cnt, smem, st)
-                 : launch_tiles(scan_tiles<T, false, true>, p, tm, n, first, cnt, smem, st);
-    return tma ? launch_tiles(scan_tiles<T, true, false>, p, tm, 1, first, cnt, smem, st)
-               : launch_tiles(scan_tiles<T, false, false>, p, tm, 1, first, cnt, smem, st);
+      return tma ? launch_tiles(scan_tiles<T, true, true>, Fwd<T, true>::kWarps, p, tm, n, first, cnt, smem, st)
+                 : launch_tiles(scan_tiles<T, false, true>, Fwd<T, true>::kWarps, p, tm, n, first, cnt, smem, st);
+    return tma ? launch_tiles(scan_tiles<T, true, false>, Fwd<T, false>::kWarps, p, tm, 1, first, cnt, smem, st)
+               : launch_tiles(scan_tiles<T, false, false>, Fwd<T, false>::kWarps, p, tm, 1, first, cnt, smem, st);
   };
   const int chain_slots = sm_count() * Fwd<T, true>::kPerSm, slots = sm_count() * Fwd<T, false>::kPerSm;
   // All blocks of a launch take about as long, so a few sequences more than the GPU holds cost as
@@ -966,8 +972,8 @@ int run_bwd(const Args& p, int B, int seqs, int dtype, int n, cudaStream_t st) {
         encode(&tm.in[2], dtype, p.i, p.ib, p.it, B, p.T, p.D) == THM_OK &&
         encode(&tm.in[3], dtype, p.dy, p.gb, p.gt, B, p.T, p.D) == THM_OK;
   const int smem = Bwd<T>::R::kBytes;
-  return tma ? launch_tiles(scan_bwd_tiles<T, true>, p, tm, n, 0, count, smem, st)
-             : launch_tiles(scan_bwd_tiles<T, false>, p, tm, n, 0, count, smem, st);
+  return tma ? launch_tiles(scan_bwd_tiles<T, true>, Bwd<T>::kWarps, p, tm, n, 0, count, smem, st)
+             : launch_tiles(scan_bwd_tiles<T, false>, Bwd<T>::kWarps, p, tm, n, 0, count, smem, st);
 }
 
 int check_sizes(int B, int T, int D, int nseq, const int* cu, int dtype) {
