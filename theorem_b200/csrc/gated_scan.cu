@@ -156,7 +156,7 @@ constexpr float kHoldBelow = -43.f;
 constexpr float kMaxL = 87.f;
 
 // A token of two channels is computed in one of two ways. PLAIN tokens have 1e-6 <= decay <= 1
-// on every channel of the warp and no held token among the warp's 8 (both checked once a tile,
+// on every channel of the warp and no held token among the warp's 16 (both checked once a tile,
 // which costs a bf16 minimum a row): no range reduction, no selects, a third fewer
 // instructions. Others take the general way.
 constexpr float kPlainDecayMin = 1e-6f, kPlainDecayMax = 1.f;
@@ -308,10 +308,13 @@ __global__ void __launch_bounds__(kDirectThreads) scan_direct(const Args p) {
 }
 
 // --------------------------------------------------------------------------- tiles
-// A block takes 64 channels and tiles of 64 tokens (one chunk), 8 tokens a warp, two channels
-// a lane. A lane scans its 8 tokens from zero and leaves the run's map h -> A h + S in shared
+// A block takes 64 channels and tiles of 64 tokens (one chunk), 16 tokens a warp, two channels
+// a lane. A lane scans its 16 tokens from zero and leaves the run's map h -> A h + S in shared
 // memory; after one barrier every lane composes the maps before its own with the state that
-// enters the tile, and its tokens' states are local + (product of a) x (entering state).
+// enters the tile, and its tokens' states are local + (product of a) x (entering state). Long
+// runs a lane make the arithmetic independent work for its own latencies and the maps few: 16
+// tokens beat 8 with twice the warps on an SM (forward B16 T8192 D2048 389 against 399 us, B1
+// T131072 519 against 573, backward B1 T65536 469 against 535), 4 (606 us) and 32 (408 us).
 //
 // Tiles come by TMA, so loading costs the warps no addresses; the barrier that the maps need
 // also says that a tile has been read, and its stage is refilled there. Where addresses or
@@ -322,7 +325,8 @@ __global__ void __launch_bounds__(kDirectThreads) scan_direct(const Args p) {
 // sequence: block k takes tiles k, k + n, ... . Each round the blocks send their tiles' maps to
 // one another's shared memory, counted in by an mbarrier, so the chain along time costs one
 // such exchange for n tiles, and x, r, i are still read once.
-constexpr int kCols = 64;
+constexpr int kWarps = 4, kRows = 16, kCols = 64;
+static_assert(kWarps * kRows == kChunk, "a tile is a chunk");
 
 struct Maps {  // of x, r, i, dy, where TMA carries the tiles
   CUtensorMap in[4];
@@ -450,7 +454,7 @@ __device__ __forceinline__ void put_pair(uint8_t* tile, int k, float2 f) {
 // A lane's first `rows` rows of a tensor into its slots, without TMA. Loads without conditions, so
 // that all are in flight at once: rows past the last repeat it (the caller overwrites them), and a
 // second channel that is not there repeats the first.
-template <typename T, int kRows>
+template <typename T>
 __device__ __forceinline__ void fill(uint8_t* tile, const void* t, long long first, long long stride, int rows, bool two) {
   if (rows == 0) return;
   const T* q = static_cast<const T*>(t) + first;
@@ -466,28 +470,28 @@ __device__ __forceinline__ void fill(uint8_t* tile, const void* t, long long fir
   for (int k = 0; k < kRows; ++k) put_pair<T>(tile, k, make_float2(to_f32<T>(v[k][0]), to_f32<T>(v[k][1])));
 }
 
-// Stages, and resident blocks an SM: for bf16 three of 80 registers a thread forward, two of 128
-// in a chain of blocks (which keeps two tiles in registers) and backward; for fp32 shared memory
-// holds two, without the room that finishing a round behind takes.
+// Stages, and resident blocks an SM: for bf16 three of 153 registers a thread forward (four of 128
+// were slower: 416 against 389 us), two of 240 in a chain of blocks, which keeps two tiles in
+// registers, and backward; for fp32 shared memory holds two, without the room that finishing a
+// round behind takes.
 template <typename T, bool CHAIN>
 struct Fwd {
-  static constexpr int kStages = 2, kPerSm = sizeof(T) == 2 && !CHAIN ? 3 : 2, kWarps = CHAIN ? 4 : 8;
+  static constexpr int kStages = 2, kPerSm = sizeof(T) == 2 && !CHAIN ? 3 : 2;
   static constexpr bool kBehind = CHAIN && sizeof(T) == 2;  // a tile is finished a round behind
   using R = Ring<T, 3, kStages>;
 };
 template <typename T>
 struct Bwd {
-  static constexpr int kStages = sizeof(T) == 2 ? 3 : 1, kPerSm = 2, kWarps = 4;
+  static constexpr int kStages = sizeof(T) == 2 ? 3 : 1, kPerSm = 2;
   using R = Ring<T, 4, kStages>;
 };
 
 // CHAIN: blocks in clusters. A round's exchange takes as long as half a tile's arithmetic, so for
 // bf16 a block scans its next tile before it receives the last one's entering state, two tiles in
-// registers (B1 T131072 D2048: 618 -> 578 us).
+// registers (B1 T131072 D2048, with 8 tokens a warp: 618 -> 578 us).
 template <typename T, bool TMA, bool CHAIN>
-__global__ void __launch_bounds__(32 * Fwd<T, CHAIN>::kWarps, Fwd<T, CHAIN>::kPerSm)
+__global__ void __launch_bounds__(32 * kWarps, Fwd<T, CHAIN>::kPerSm)
     scan_tiles(const __grid_constant__ Args p, const __grid_constant__ Maps tm) {
-  constexpr int kWarps = Fwd<T, CHAIN>::kWarps, kRows = kChunk / kWarps;
   constexpr bool BEHIND = Fwd<T, CHAIN>::kBehind;
   constexpr int NS = Fwd<T, CHAIN>::kStages, NM = BEHIND ? 3 : 2, DEPTH = BEHIND ? 4 : 2;
   extern __shared__ __align__(128) uint8_t stages[];
@@ -525,15 +529,15 @@ __global__ void __launch_bounds__(32 * Fwd<T, CHAIN>::kWarps, Fwd<T, CHAIN>::kPe
   // The lane's tokens of step j from zero, their maps' last one into shared memory.
   auto scan_tile = [&](int j, float2(&A)[kRows], float2(&S)[kRows]) {
     const int tile = j * nblk + rank, row0 = tile * kChunk + warp * kRows;
-    const int have = min(max(q.len - row0, 0), kRows);  // rows of the lane's 8 that there are
+    const int have = min(max(q.len - row0, 0), kRows);  // rows of the lane's 16 that there are
     uint8_t *xs = ring.slot(j, 0) + own, *rs = ring.slot(j, 1) + own, *is = ring.slot(j, 2) + own;
     if constexpr (TMA) {
       if (tile < ntiles) ring.wait(j, &g_status_scan);
     } else if (ln.on) {
       const long long t = q.lo + row0;
-      fill<T, kRows>(xs, p.x, q.batch * p.xb + t * p.xt + ln.c, p.xt, have, ln.two);
-      fill<T, kRows>(rs, p.r, q.batch * p.rb + t * p.rt + ln.c, p.rt, have, ln.two);
-      fill<T, kRows>(is, p.i, q.batch * p.ib + t * p.it + ln.c, p.it, have, ln.two);
+      fill<T>(xs, p.x, q.batch * p.xb + t * p.xt + ln.c, p.xt, have, ln.two);
+      fill<T>(rs, p.r, q.batch * p.rb + t * p.rt + ln.c, p.rt, have, ln.two);
+      fill<T>(is, p.i, q.batch * p.ib + t * p.it + ln.c, p.it, have, ln.two);
     }
     for (int k = have; k < kRows; ++k) {  // rows past the sequence's end hold the state
       put_pair<T>(rs, k, f2(-INFINITY));
@@ -643,15 +647,14 @@ __global__ void __launch_bounds__(32 * Fwd<T, CHAIN>::kWarps, Fwd<T, CHAIN>::kPe
 }
 
 // --------------------------------------------------------------------------- backward
-// The same tiles from the back. A lane keeps s, p, t = a - 1 and the injected term of its 8
+// The same tiles from the back. A lane keeps s, p, t = a - 1 and the injected term of its 16
 // tokens; two maps a warp go through shared memory, the forward one (h, from the chunk's kept
 // state) and the backward one (G_t = a_t dh_t, from the tile behind). Clusters exchange the
 // backward maps only: every tile's entering state is known. x and dy are read again from the
 // tile after the barrier, so a stage is refilled at the next step's barrier.
 template <typename T, bool TMA>
-__global__ void __launch_bounds__(32 * Bwd<T>::kWarps, Bwd<T>::kPerSm)
+__global__ void __launch_bounds__(32 * kWarps, Bwd<T>::kPerSm)
     scan_bwd_tiles(const __grid_constant__ Args p, const __grid_constant__ Maps tm) {
-  constexpr int kWarps = Bwd<T>::kWarps, kRows = kChunk / kWarps;
   extern __shared__ __align__(128) uint8_t stages[];
   __shared__ __align__(16) float4 maps[2][kWarps][32];
   __shared__ __align__(16) float2 back[2][kWarps][32];
@@ -706,10 +709,10 @@ __global__ void __launch_bounds__(32 * Bwd<T>::kWarps, Bwd<T>::kPerSm)
       if (tile >= 0) ring.wait(j, &g_status_scan);
     } else if (ln.on) {
       const long long t = q.lo + row0;
-      fill<T, kRows>(xs, p.x, q.batch * p.xb + t * p.xt + ln.c, p.xt, have, ln.two);
-      fill<T, kRows>(rs, p.r, q.batch * p.rb + t * p.rt + ln.c, p.rt, have, ln.two);
-      fill<T, kRows>(is, p.i, q.batch * p.ib + t * p.it + ln.c, p.it, have, ln.two);
-      fill<T, kRows>(gs, p.dy, q.batch * p.gb + t * p.gt + ln.c, p.gt, have, ln.two);
+      fill<T>(xs, p.x, q.batch * p.xb + t * p.xt + ln.c, p.xt, have, ln.two);
+      fill<T>(rs, p.r, q.batch * p.rb + t * p.rt + ln.c, p.rt, have, ln.two);
+      fill<T>(is, p.i, q.batch * p.ib + t * p.it + ln.c, p.it, have, ln.two);
+      fill<T>(gs, p.dy, q.batch * p.gb + t * p.gt + ln.c, p.gt, have, ln.two);
     }
     for (int k = have; k < kRows; ++k) {
       put_pair<T>(rs, k, f2(-INFINITY));
@@ -892,7 +895,7 @@ int bwd_cluster(int T, int D, int nseq, bool packed, int dtype) {
 
 // `count` sequences of channels from `first` on, n blocks each.
 template <typename K>
-int launch_tiles(K kernel, int warps, Args p, const Maps& tm, int n, int first, int count, int smem, cudaStream_t st) {
+int launch_tiles(K kernel, Args p, const Maps& tm, int n, int first, int count, int smem, cudaStream_t st) {
   p.first = first;
   p.count = count;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
@@ -902,7 +905,7 @@ int launch_tiles(K kernel, int warps, Args p, const Maps& tm, int n, int first, 
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
   cfg.gridDim = dim3((unsigned)(n * count));
-  cfg.blockDim = dim3(32 * warps);
+  cfg.blockDim = dim3(32 * kWarps);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -939,10 +942,10 @@ int run_fwd(Args p, int B, int seqs, int dtype, cudaStream_t st) {
   static_assert(smem == Fwd<T, true>::R::kBytes);
   auto run = [&](int n, int first, int cnt) {
     if (n > 1)
-      return tma ? launch_tiles(scan_tiles<T, true, true>, Fwd<T, true>::kWarps, p, tm, n, first, cnt, smem, st)
-                 : launch_tiles(scan_tiles<T, false, true>, Fwd<T, true>::kWarps, p, tm, n, first, cnt, smem, st);
-    return tma ? launch_tiles(scan_tiles<T, true, false>, Fwd<T, false>::kWarps, p, tm, 1, first, cnt, smem, st)
-               : launch_tiles(scan_tiles<T, false, false>, Fwd<T, false>::kWarps, p, tm, 1, first, cnt, smem, st);
+      return tma ? launch_tiles(scan_tiles<T, true, true>, p, tm, n, first, cnt, smem, st)
+                 : launch_tiles(scan_tiles<T, false, true>, p, tm, n, first, cnt, smem, st);
+    return tma ? launch_tiles(scan_tiles<T, true, false>, p, tm, 1, first, cnt, smem, st)
+               : launch_tiles(scan_tiles<T, false, false>, p, tm, 1, first, cnt, smem, st);
   };
   const int chain_slots = sm_count() * Fwd<T, true>::kPerSm, slots = sm_count() * Fwd<T, false>::kPerSm;
   // All blocks of a launch take about as long, so a few sequences more than the GPU holds cost as
@@ -972,8 +975,8 @@ int run_bwd(const Args& p, int B, int seqs, int dtype, int n, cudaStream_t st) {
         encode(&tm.in[2], dtype, p.i, p.ib, p.it, B, p.T, p.D) == THM_OK &&
         encode(&tm.in[3], dtype, p.dy, p.gb, p.gt, B, p.T, p.D) == THM_OK;
   const int smem = Bwd<T>::R::kBytes;
-  return tma ? launch_tiles(scan_bwd_tiles<T, true>, Bwd<T>::kWarps, p, tm, n, 0, count, smem, st)
-             : launch_tiles(scan_bwd_tiles<T, false>, Bwd<T>::kWarps, p, tm, n, 0, count, smem, st);
+  return tma ? launch_tiles(scan_bwd_tiles<T, true>, p, tm, n, 0, count, smem, st)
+             : launch_tiles(scan_bwd_tiles<T, false>, p, tm, n, 0, count, smem, st);
 }
 
 int check_sizes(int B, int T, int D, int nseq, const int* cu, int dtype) {
