@@ -10,6 +10,9 @@ Ops (functional API in ``theorem_b200.ops``; drop-in ``custom_kernel``s in
                      rule (tcgen05, state resident in TMEM)
 * chunk_fwd_o     -- chunkwise output (tcgen05 + TMEM)
 * chain           -- the gated-DeltaNet layer forward built from the above
+* gated_scan, group_norm, causal_conv1d_step and their backward passes
+                  -- per-channel gated recurrence, norm per head, conv by tokens
+* recurrent       -- the gated recurrent block built from those, with gradients
 
 All compute runs in ``libtheorem_b200.so`` (C ABI: include/theorem_b200.h);
 the Python layer only validates, allocates and launches.

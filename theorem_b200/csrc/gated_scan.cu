@@ -277,7 +277,9 @@ __device__ __forceinline__ bool plain_decays(float2 nd) {
 // latency there is.
 constexpr int kDirectThreads = 64;
 
-template <typename T, bool PAIRED>
+// BATCH tokens' loads are in flight together: 4 for runs (a token 0.15 us instead of 0.35), 1 for
+// fewer, in fewer registers (B256 T1: 4.5 us instead of 5.5).
+template <typename T, bool PAIRED, int BATCH>
 __global__ void __launch_bounds__(kDirectThreads) scan_direct(const Args p) {
   const int chain = (blockIdx.x * kDirectThreads + threadIdx.x) >> 5, n = chain / p.cols;
   const Lane ln(chain % p.cols * 64, p.D);
@@ -295,15 +297,28 @@ __global__ void __launch_bounds__(kDirectThreads) scan_direct(const Args p) {
   y += (q.batch * p.T + q.lo) * p.D;
   const float2 ndecay = neg_decay(ln, p.decay);
   float2 h = p.h0 != nullptr ? ln.load(p.h0 + (long long)n * p.D) : f2(0.f);
-  for (int k = 0; k < q.len; ++k) {
+  auto token = [&](int k, RawPair<T> xv, RawPair<T> rv, RawPair<T> iv) {
     if (p.states != nullptr && k % kChunk == 0) ln.store(p.states + (q.slot + k / kChunk) * p.D, h);
     float2 a, b;
-    token_pair<T, false>(load_pair<T, PAIRED>(x + k * p.xt, ln.two).get(),
-                         load_pair<T, PAIRED>(r + k * p.rt, ln.two).get(),
-                         load_pair<T, PAIRED>(i + k * p.it, ln.two).get(), ndecay, a, b);
+    token_pair<T, false>(xv.get(), rv.get(), iv.get(), ndecay, a, b);
     h = __ffma2_rn(a, h, b);
     store_pair<T, PAIRED>(y + (long long)k * p.D, h, ln.two);
+  };
+  int k = 0;
+  for (; BATCH > 1 && k + BATCH <= q.len; k += BATCH) {
+    RawPair<T> xv[BATCH], rv[BATCH], iv[BATCH];
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      rv[u] = load_pair<T, PAIRED>(r + (k + u) * p.rt, ln.two);
+      iv[u] = load_pair<T, PAIRED>(i + (k + u) * p.it, ln.two);
+      xv[u] = load_pair<T, PAIRED>(x + (k + u) * p.xt, ln.two);
+    }
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) token(k + u, xv[u], rv[u], iv[u]);
   }
+  for (; k < q.len; ++k)
+    token(k, load_pair<T, PAIRED>(x + k * p.xt, ln.two), load_pair<T, PAIRED>(r + k * p.rt, ln.two),
+          load_pair<T, PAIRED>(i + k * p.it, ln.two));
   if (p.final_state != nullptr) ln.store(p.final_state + (long long)n * p.D, h);
 }
 
@@ -320,6 +335,9 @@ __global__ void __launch_bounds__(kDirectThreads) scan_direct(const Args p) {
 // also says that a tile has been read, and its stage is refilled there. Where addresses or
 // strides are no multiples of 16 bytes (TMA false), the lanes fill their own slots with plain
 // loads.
+//
+// B16 T8192 D2048 bf16 takes 389 us, 5.5 TB/s (0.84 of a copy): between HBM, the special-function
+// unit (63 % busy, four operations an element) and the latencies of 12 warps an SM.
 //
 // Where there are too few channels to fill the GPU, a cluster of up to 8 blocks shares a
 // sequence: block k takes tiles k, k + n, ... . Each round the blocks send their tiles' maps to
@@ -651,7 +669,9 @@ __global__ void __launch_bounds__(32 * kWarps, Fwd<T, CHAIN>::kPerSm)
 // tokens; two maps a warp go through shared memory, the forward one (h, from the chunk's kept
 // state) and the backward one (G_t = a_t dh_t, from the tile behind). Clusters exchange the
 // backward maps only: every tile's entering state is known. x and dy are read again from the
-// tile after the barrier, so a stage is refilled at the next step's barrier.
+// tile after the barrier, so a stage is refilled at the next step's barrier. B8 T4096 D2048 bf16
+// takes 213 us, 4.4 TB/s (0.67 of a copy): 53 instructions per 32 elements from 8 warps an SM, and
+// 256 blocks on 148 SMs.
 template <typename T, bool TMA>
 __global__ void __launch_bounds__(32 * kWarps, Bwd<T>::kPerSm)
     scan_bwd_tiles(const __grid_constant__ Args p, const __grid_constant__ Maps tm) {
@@ -866,8 +886,13 @@ int encode(CUtensorMap* m, int dtype, const void* base, long long bs, long long 
                       base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-// Up to this many tokens a lane's serial walk beats the tiles.
-constexpr int kDirectTokens = 16;
+// Up to how many tokens a lane's serial walk beats the tiles, by the sequences of 64 channels.
+// Measured (us, bf16, D 2048, walk / tiles): 32 sequences 4.1 / 4.0 at 16 tokens, 256 5.3 / 5.0
+// at 24, 2048 11.1 / 19.0 at 32 and 20.1 / 15.5 at 64, 8192 33 / 68 and 71 / 62.
+int direct_tokens(int count) {
+  const int most = 14 + count / 48;
+  return most < 48 ? most : 48;
+}
 
 // Blocks that share a sequence: as many as fit the GPU at once, and no more than a sequence has
 // pairs of tiles for. Measured on bf16, forward: B8 T4096 D2048 (256 sequences of channels)
@@ -924,13 +949,13 @@ template <typename T>
 int run_fwd(Args p, int B, int seqs, int dtype, cudaStream_t st) {
   constexpr int elem = sizeof(T);
   const int count = seqs * p.cols;
-  if (p.T <= kDirectTokens) {
+  if (p.T <= direct_tokens(count)) {
     const unsigned grid = (unsigned)((count + kDirectThreads / 32 - 1) / (kDirectThreads / 32));
     p.count = count;
-    if (multiples(2 * elem, elem, p.D, {p.x, p.r, p.i, p.y}, {p.xb, p.xt, p.rb, p.rt, p.ib, p.it}))
-      scan_direct<T, true><<<grid, kDirectThreads, 0, st>>>(p);
-    else
-      scan_direct<T, false><<<grid, kDirectThreads, 0, st>>>(p);
+    const bool paired = multiples(2 * elem, elem, p.D, {p.x, p.r, p.i, p.y}, {p.xb, p.xt, p.rb, p.rt, p.ib, p.it});
+    auto kernel = p.T < 4 ? (paired ? scan_direct<T, true, 1> : scan_direct<T, false, 1>)
+                          : (paired ? scan_direct<T, true, 4> : scan_direct<T, false, 4>);
+    kernel<<<grid, kDirectThreads, 0, st>>>(p);
     return check_launch();
   }
   Maps tm{};
