@@ -21,6 +21,7 @@ def test_gated_scan_rejects_arguments_without_gpu():
     assert f(*no_cu, *q6, 2, 8, 8, 3, 0, 0, None) == _lib.THM_ERR_INVALID    # nseq != B without cu_seqlens
     assert f(*p9, *q6, 2, 8, 8, 2, 0, 0, None) == _lib.THM_ERR_INVALID       # packed with B = 2
     assert f(*no_cu, *q6, 1 << 27, 1, 8, 1 << 27, 0, 0, None) == _lib.THM_ERR_UNSUPPORTED
+    assert f(*no_cu, *q6, 1, (1 << 30) + 1, 8, 1, 0, 0, None) == _lib.THM_ERR_UNSUPPORTED
     assert f(*([None] * 9), *q6, 1, 8, 8, 1, 0, 0, None) == _lib.THM_ERR_INVALID  # null pointers
     assert f(*([None] * 9), *q6, 1, 8, 0, 1, 0, 0, None) == _lib.THM_OK      # no channels
     assert f(*([None] * 9), *q6, 0, 8, 8, 0, 0, 0, None) == _lib.THM_OK      # no sequences
@@ -63,6 +64,8 @@ def test_conv_step_and_bwd_reject_arguments_without_gpu():
     assert f(*([None] * 6), 8, 8, 0, 1, 8, 4, 0, 0, None) == _lib.THM_OK
     assert g(*p8, 8, 8, 8, 8, 1, 1, 8, 9, 0, 0, None) == _lib.THM_ERR_UNSUPPORTED
     assert g(*p8, 8, 8, 8, 8, 1, -1, 8, 4, 0, 0, None) == _lib.THM_ERR_INVALID
+    assert g(*p8, 8, 8, 8, 8, 1, (1 << 30) + 1, 8, 4, 0, 0, None) == _lib.THM_ERR_UNSUPPORTED
+    assert g(*p8, 8, 8, 8, 8, 65536, 1, 8, 4, 0, 0, None) == _lib.THM_ERR_UNSUPPORTED
     assert g(*([None] * 8), 8, 8, 8, 8, 1, 1, 8, 4, 0, 0, None) == _lib.THM_ERR_INVALID
     assert lib.thm_causal_conv1d_bwd_parts(0, 8, 8) == 0
     assert lib.thm_causal_conv1d_bwd_parts(2, 1, 8) == 2

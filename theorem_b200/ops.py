@@ -466,8 +466,8 @@ def gated_scan_bwd(x, r, i, decay, states, dy, dfinal=None, cu_seqlens=None, dx=
     else:
         for name, t in zip(("dx", "dr", "di"), outs):
             _dense(name, t, x, x.shape, x.dtype)
-    ddecay = torch.empty(D, device=x.device, dtype=torch.float32)
-    dh0 = torch.empty(n, D, device=x.device, dtype=torch.float32)
+    ddecay = torch.empty_like(decay)
+    dh0 = torch.empty(n, D, device=x.device, dtype=torch.float32) if dfinal is None else torch.empty_like(dfinal)
     parts = L.load().thm_gated_scan_bwd_parts(T, D, n, int(cu_seqlens is not None), L.dtype_code(x))
     work = torch.empty(parts, D, device=x.device, dtype=torch.float32)
     L.check(L.load().thm_gated_scan_bwd(L.ptr(x), L.ptr(r), L.ptr(i), L.ptr(decay), L.ptr(states), L.ptr(dy),
@@ -551,8 +551,8 @@ def group_norm_bwd(x, dy, group: int, weight=None, bias=None, gate=None, activat
     dev = x.device
     dx = _empty(x, x.shape, x.dtype)
     dgate = _empty(x, x.shape, x.dtype) if gate is not None else None
-    dweight = torch.empty(C, device=dev, dtype=torch.float32) if weight is not None else None
-    dbias = torch.empty(C, device=dev, dtype=torch.float32) if bias is not None else None
+    dweight = torch.empty_like(weight) if weight is not None else None
+    dbias = torch.empty_like(bias) if bias is not None else None
     work = None
     if weight is not None or bias is not None:
         work = torch.empty(L.load().thm_group_norm_bwd_parts(R, C, int(group)), 2, C, device=dev, dtype=torch.float32)
@@ -614,8 +614,7 @@ def causal_conv1d_bwd(x, weight, bias, dy, activation=None):
     B, S, D, W, strides = _conv_args(x, weight, bias, activation)
     strides += _like("dy", dy, x)[:2]
     dx = _empty(x, x.shape, x.dtype)
-    dweight = torch.empty(D, W, device=x.device, dtype=torch.float32)
-    dbias = torch.empty(D, device=x.device, dtype=torch.float32)
+    dweight, dbias = torch.empty_like(weight), torch.empty_like(bias)
     parts = L.load().thm_causal_conv1d_bwd_parts(B, S, D)
     work = torch.empty(max(parts, 0), W + 1, D, device=x.device, dtype=torch.float32)
     L.check(L.load().thm_causal_conv1d_bwd(L.ptr(x), L.ptr(weight), L.ptr(bias), L.ptr(dy), L.ptr(dx), L.ptr(dweight),
