@@ -188,6 +188,43 @@ def test_training_step_and_decode_step_replay_in_graphs():
     assert all(torch.equal(a, b) for a, b in zip(toks_eager, got)) and torch.equal(st.h, st_eager.h)
 
 
+def test_two_streams_at_once():
+    """Training steps of two blocks interleaved on two streams give what each gives alone."""
+    blocks, ins, alone = [], [], []
+    for k, (B, T, D) in enumerate(((1, 3000, 256), (6, 400, 512))):
+        blocks.append(_block(_params(D, 4, seed=k, bias=False), 64, False))
+        ins.append([t.to(DEV) for t in _inputs(B, T, D, BF, seed=k)])
+
+    def step(k):
+        x, r, i, z, dy = ins[k]
+        y, st, saved = blocks[k](x, r, i, z, want_grad=True)
+        return [y, st.h, *blocks[k].backward(saved, dy).values()]
+
+    for k in range(2):
+        alone.append(step(k))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(4):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(step(k))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for g in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(alone[k], g))
+
+
+def test_arguments_by_name():
+    from theorem_b200 import ops
+    x = torch.randn(2, 40, 64, device=DEV)
+    dec = torch.full((64,), 0.1, device=DEV)
+    a = ops.gated_scan(x, x, x, dec)[0]
+    assert torch.equal(a, ops.gated_scan(x=x, r=x, i=x, decay=dec)[0])
+    assert torch.equal(ops.group_norm(x, 16), ops.group_norm(x=x, group=16))
+
+
 @pytest.mark.parametrize("K", [128, 64])
 @pytest.mark.parametrize("gated", [True, False])
 def test_deltanet_layer_with_output_norm(K, gated):
