@@ -98,7 +98,8 @@ def _check(x, dy, z, w, b, G, act, center, eps, y, grads, dtype):
 SHAPES = [  # rows, channels, group
     (1, 1, 1), (1, 128, 128), (64, 2048, 128), (5, 48, 16), (3, 40, 8), (7, 6, 2), (300, 64, 64), (9, 196, 49),
     (33, 96, 3), (4, 1024, 1024), (3, 1032, 1032), (2, 4096, 4096), (5, 4095, 4095), (3, 2050, 1025), (11, 129, 129),
-    (6, 260, 130), (2, 8192, 256), (1500, 24, 12), (2, 3000, 1500), (257, 520, 260),
+    (6, 260, 130), (2, 8192, 256), (40, 392, 49), (21, 808, 101), (3, 5416, 677),
+    (5, 2600, 650), (2, 8184, 4092), (9, 264, 33), (4, 1960, 490), (1500, 24, 12), (2, 3000, 1500), (257, 520, 260),
 ]
 
 
@@ -186,6 +187,26 @@ def test_constant_rows_and_zero_rows():
     for center in (True, False):
         g = ops.group_norm_bwd(x, torch.ones_like(x), 32, center=center)[0]
         assert torch.isfinite(g).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_groups_that_cut_vectors_keep_to_themselves(dtype):
+    """NaN in a neighbouring group that shares a 16-byte vector reaches neither sums nor gradients, in
+    place as well."""
+    from theorem_b200 import ops
+    R, C, G = 70, 392, 49
+    x, dy, z, w, b = [t.to(DEV) for t in _inputs(R, C, dtype, 3, True, True)]
+    kw = dict(activation="silu", center=True)
+    y, g = ops.group_norm(x, G, w, b, gate=z, **kw), ops.group_norm_bwd(x, dy, G, w, b, gate=z, **kw)
+    own = slice(49, 98)
+    bad = [t.clone() for t in (x, dy, z)]
+    for t in bad:
+        t[:, 98:] = float("nan")
+        t[:, :49] = float("inf")
+    y2, g2 = ops.group_norm(bad[0], G, w, b, gate=bad[2], **kw), ops.group_norm_bwd(bad[0], bad[1], G, w, b, gate=bad[2], **kw)
+    assert torch.equal(y2[:, own], y[:, own])
+    assert all(torch.equal(p[..., own], q[..., own]) for p, q in zip(g2, g))
+    assert torch.equal(ops.group_norm(x, G, w, b, gate=z, out=x, **kw), y)
 
 
 def test_non_finite_values_stay_in_their_group():

@@ -110,18 +110,47 @@ __device__ __forceinline__ float2 sigmoid2(float2 x) {
 
 // A thread's share of a group: NV vectors of VEC channels as fp32 pairs (a single channel has
 // an empty second half).
-template <typename T, int VEC, int NV>
+//
+// EDGE: the group's borders are no multiples of a vector, but the rows' are. Its lanes then take the
+// aligned vectors that cover it, two of which may hold channels of its neighbours: those are taken
+// as zeros, which no sum sees, and not stored.
+template <typename T, int VEC, int NV, bool EDGE>
 struct Share {
   static constexpr int kPairs = (VEC * NV + 1) / 2;
   using Vec = Pack<T, VEC>;
   int c0, step;    // channel of vector j: c0 + j step
   bool have[NV];
+  uint32_t valid;  // EDGE: which channels are the group's, bit j VEC + e
 
   __device__ __forceinline__ Share(const Args& p, const Place& q) {
-    c0 = q.on ? q.group * p.G + q.lane * VEC : 0;
     step = q.width * VEC;
+    valid = 0;
+    if constexpr (EDGE) {
+      const int first = q.group * p.G, end = first + p.G;
+      c0 = q.on ? first / VEC * VEC + q.lane * VEC : 0;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) have[j] = q.on && (q.lane + j * q.width) * VEC < p.G;
+      for (int j = 0; j < NV; ++j) {
+        have[j] = q.on && c0 + j * step < end;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (have[j] && c0 + j * step + e >= first && c0 + j * step + e < end) valid |= 1u << (j * VEC + e);
+      }
+    } else {
+      c0 = q.on ? q.group * p.G + q.lane * VEC : 0;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) have[j] = q.on && (q.lane + j * q.width) * VEC < p.G;
+    }
+  }
+  __device__ __forceinline__ bool mine(int j, int e) const { return EDGE ? (valid >> (j * VEC + e)) & 1 : have[j]; }
+  // Zeros for what is not the group's (absent vectors are zeros as loaded).
+  __device__ __forceinline__ void mask(float2 (&f)[kPairs]) const {
+    if constexpr (EDGE) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (!mine(j, e)) at(f, j, e) = 0.f;
+    }
   }
   // The vectors at t (channel c0 of a row); absent ones, and all where there is no row, are 0.
   __device__ __forceinline__ void load(const T* t, bool ok, Vec (&raw)[NV]) const {
@@ -154,6 +183,17 @@ struct Share {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       if (!(have[j] && ok)) continue;
+      if constexpr (EDGE) {
+        constexpr uint32_t kAll = (1u << VEC) - 1;
+        if (((valid >> (j * VEC)) & kAll) != kAll) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const int k = j * VEC + e;
+            if (mine(j, e)) r[j * step + e] = from_f32<T>(k & 1 ? f[k / 2].y : f[k / 2].x);
+          }
+          continue;
+        }
+      }
       if constexpr (VEC == 1) {
         r[j * step] = from_f32<T>(j & 1 ? f[j / 2].y : f[j / 2].x);
       } else {
@@ -181,7 +221,7 @@ struct Share {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) at(f, j, e) = have[j] ? (t != nullptr ? t[c0 + j * step + e] : absent) : 0.f;
+      for (int e = 0; e < VEC; ++e) at(f, j, e) = mine(j, e) ? (t != nullptr ? t[c0 + j * step + e] : absent) : 0.f;
   }
   // Sum of a over the thread's channels.
   static __device__ __forceinline__ float sum(const float2 (&a)[kPairs]) {
@@ -206,9 +246,9 @@ struct Share {
       for (int k = 0; k < kPairs; ++k) v[k] = __fadd2_rn(v[k], f2(-mu));
 #pragma unroll
       for (int j = 0; j < NV; ++j)
-        if (!have[j])
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) at(v, j, e) = 0.f;
+        for (int e = 0; e < VEC; ++e)
+          if (!mine(j, e)) at(v, j, e) = 0.f;
       if constexpr (VEC * NV == 1) v[0].y = 0.f;
     }
     return rsqrtf(fmaf(team_sum(dot(v, v), p.tl, sh), inv, p.eps));
@@ -219,10 +259,10 @@ struct Share {
 // them. Bound by HBM: 131072 x 2048 bf16 in groups of 128 with a gate takes 260 to 265 us, 6.1 TB/s
 // (0.93 of a copy), at 18 instructions per 32 elements; without packed arithmetic, the loads ahead
 // and the flags as template arguments it took 30 and 366 us.
-template <typename T, int VEC, int NV, int FLAGS>
+template <typename T, int VEC, int NV, bool EDGE, int FLAGS>
 __global__ void __launch_bounds__(max_threads(VEC, NV)) norm_fwd(const Args p) {
   __shared__ float sh[32];
-  using S = Share<T, VEC, NV>;
+  using S = Share<T, VEC, NV, EDGE>;
   constexpr int N = S::kPairs;
   const Place q = place(p);
   const S me(p, q);
@@ -240,6 +280,7 @@ __global__ void __launch_bounds__(max_threads(VEC, NV)) norm_fwd(const Args p) {
   for (; row - q.sub < p.R; row += step) {
     float2 v[N], z[N];
     S::widen(xr, v);
+    me.mask(v);
     if constexpr ((FLAGS & kGate) != 0) S::widen(zr, z);
     const bool more = row + step < p.R;
     me.load(x += xstep, more, xr);
@@ -265,14 +306,14 @@ __global__ void __launch_bounds__(max_threads(VEC, NV)) norm_fwd(const Args p) {
 // As above with three tensors in, two out and the parameters' sums in registers: 32768 x 2048 bf16
 // in groups of 128 with a gate takes 113 us and 3 for the second launch, 5.6 TB/s (0.86 of a copy),
 // issuing on 67 % of the cycles; three blocks of 80 registers an SM. Narrow groups are bound by
-// their instructions: 7777 x 1960 fp32 in groups of 49 with SiLU takes 75 us (0.37 of a copy; 148 with two
-// channels a lane and the flags looked up, 100 with two blocks an SM).
-template <typename T, int VEC, int NV, int FLAGS>
+// their instructions: 7777 x 1960 fp32 in groups of 49 with SiLU takes 69 us (0.40 of a copy; with single
+// elements 148 with two channels a lane and the flags looked up, 100 with two blocks an SM, then 76).
+template <typename T, int VEC, int NV, bool EDGE, int FLAGS>
 __global__ void __launch_bounds__(max_threads(VEC, NV), (VEC * NV == 8 && sizeof(T) == 2) || VEC * NV == 4 ? 3 : 1) norm_bwd(const Args p) {
   __shared__ float sh[32];
   __shared__ float2 sh2[32];
   extern __shared__ float fold[];  // [rpi][gpc * G] when a block works on several rows
-  using S = Share<T, VEC, NV>;
+  using S = Share<T, VEC, NV, EDGE>;
   constexpr int N = S::kPairs;
   const Place q = place(p);
   const S me(p, q);
@@ -297,6 +338,9 @@ __global__ void __launch_bounds__(max_threads(VEC, NV), (VEC * NV == 8 && sizeof
     S::widen(xr, v);
     S::widen(gr, d);
     if constexpr ((FLAGS & kGate) != 0) S::widen(zr, z);
+    me.mask(v);
+    me.mask(d);
+    if constexpr ((FLAGS & kGate) != 0) me.mask(z);
     const bool more = row + step < p.R;
     me.load(x += xstep, more, xr);
     me.load(dy += gstep, more, gr);
@@ -353,17 +397,17 @@ __global__ void __launch_bounds__(max_threads(VEC, NV), (VEC * NV == 8 && sizeof
     if (p.rpi == 1) {
 #pragma unroll
       for (int j = 0; j < NV; ++j)
-        if (me.have[j])
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) out[me.c0 + j * me.step + e] = S::at(dw, j, e);
+        for (int e = 0; e < VEC; ++e)
+          if (me.mine(j, e)) out[me.c0 + j * me.step + e] = S::at(dw, j, e);
       continue;
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < NV; ++j)
-      if (me.have[j])
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) fold[q.sub * span + me.c0 + j * me.step - first + e] = S::at(dw, j, e);
+      for (int e = 0; e < VEC; ++e)
+        if (me.mine(j, e)) fold[q.sub * span + me.c0 + j * me.step - first + e] = S::at(dw, j, e);
     __syncthreads();
     for (int k = threadIdx.x; k < span && first + k < p.C; k += blockDim.x) {
       float acc = 0.f;
@@ -389,45 +433,61 @@ constexpr int kMaxGroup = 4096;
 
 struct Plan {
   int vec, nv, threads;
+  bool edge;
   dim3 grid;
 };
 
 // How a call is cut up. Vectors are the widest (up to 16 bytes) that the group size, the
-// row strides and the addresses allow. `blocks`: rows of blocks wanted.
+// row strides and the addresses allow.
 Plan make_plan(Args& p, int elem, const void* const* ptrs, int nptr, int blocks_per_sm) {
   Plan q{};
   q.vec = 16 / elem;
-  uintptr_t bits = (uintptr_t)(p.G * elem);
+  uintptr_t bits = (uintptr_t)(p.C * elem);
   bits |= (uintptr_t)(p.xs * elem) | (uintptr_t)(p.zs * elem) | (uintptr_t)(p.gs * elem);
   for (int k = 0; k < nptr; ++k) bits |= reinterpret_cast<uintptr_t>(ptrs[k]);
-  while (q.vec > 1 && (bits & (q.vec * elem - 1)) != 0) q.vec >>= 1;
-  if (q.vec * elem < 16 && q.vec > 2) q.vec = 2;  // built for 16 bytes, two elements and one
-  const int nvec = (p.G + q.vec - 1) / q.vec;
+  int nvec = p.G / q.vec;
+  if ((bits & 15) != 0 || p.G % q.vec != 0) {
+    // Rows of whole vectors, groups that are not: masked borders, where they are a small part of the
+    // group (7777 x 1960 fp32 in groups of 49, backward: 69 us instead of 76 with single elements;
+    // 20000 x 1960 bf16 in groups of 245: 103 us)
+    // and a block's registers hold its vectors.
+    nvec = (p.G + 2 * q.vec - 2) / q.vec;
+    q.edge = (bits & 15) == 0 && p.G >= 4 * q.vec && nvec <= 256 * (16 / q.vec);
+    if (!q.edge) {
+      bits |= (uintptr_t)(p.G * elem);
+      q.vec = (bits & (2 * elem - 1)) == 0 ? 2 : 1;
+      nvec = p.G / q.vec;
+    }
+  }
   // Whole 16-byte vectors: a lane has one, so that more lanes have loads in flight, and never more
   // than 16 channels, whose sums and parameters fit its registers. Narrow ones: a lane has four,
   // because their sums across lanes cost more than their loads.
   const bool wide = q.vec * elem == 16;
-  const int most = wide ? 16 / q.vec : 4;  // vectors of a lane
+  const int most = wide ? 16 / q.vec : q.vec == 2 ? 4 : 8;            // vectors of a lane
+  const int least = wide ? 1 : q.vec == 1 && nvec > 128 ? 8 : 4;
   q.threads = 256;
   if (nvec <= 32 * most) {
     p.tl = 1;
-    while (p.tl < 32 && p.tl * (wide ? 1 : 4) < nvec) p.tl <<= 1;
+    while (p.tl < 32 && p.tl * least < nvec) p.tl <<= 1;
     q.nv = (nvec + p.tl - 1) / p.tl;
-    q.nv = !wide || q.nv > 2 ? 4 : q.nv;
+    q.nv = !wide ? least : q.nv > 2 ? 4 : q.nv;
     const int teams = q.threads / p.tl;
     p.gpc = teams < p.groups ? teams : p.groups;
     p.rpi = teams / p.gpc;
   } else {
     p.tl = 0;
     p.gpc = p.rpi = 1;
-    q.nv = wide ? 1 : q.vec == 2 ? 4 : 8;
+    q.nv = wide ? 1 : most;
     while (wide && nvec > 256 * q.nv) q.nv <<= 1;
     q.threads = ((nvec + q.nv - 1) / q.nv + 31) / 32 * 32;
   }
   const int gx = (p.groups + p.gpc - 1) / p.gpc;
   const long long need = (p.R + p.rpi - 1) / p.rpi;
-  long long want = (long long)sm_count() * blocks_per_sm / gx;
-  want = want < 1 ? 1 : want;
+  // As many threads as blocks_per_sm blocks of 256 an SM; no more rows of blocks than that has
+  // blocks (the workspace of the backward pass).
+  const long long full = (long long)sm_count() * blocks_per_sm;
+  long long want = full * 256 / q.threads / gx;
+  want = want < 1 ? 1 : want > full ? full : want;
   const long long gy = need < want ? need : want;
   q.grid = dim3(gx, (unsigned)(gy < 1 ? 1 : gy));
   return q;
@@ -435,33 +495,37 @@ Plan make_plan(Args& p, int elem, const void* const* ptrs, int nptr, int blocks_
 
 constexpr int kFwdBlocks = 4, kBwdBlocks = 3;
 
-template <typename T, int VEC, int NV, int FLAGS>
+template <typename T, int VEC, int NV, bool EDGE, int FLAGS>
 void launch(const Plan& q, const Args& p, bool bwd, cudaStream_t st) {
   const size_t fold = bwd && p.part != nullptr && p.rpi > 1 ? sizeof(float) * p.rpi * p.gpc * p.G : 0;
   if (bwd)
-    norm_bwd<T, VEC, NV, FLAGS><<<q.grid, q.threads, fold, st>>>(p);
+    norm_bwd<T, VEC, NV, EDGE, FLAGS><<<q.grid, q.threads, fold, st>>>(p);
   else
-    norm_fwd<T, VEC, NV, FLAGS><<<q.grid, q.threads, 0, st>>>(p);
+    norm_fwd<T, VEC, NV, EDGE, FLAGS><<<q.grid, q.threads, 0, st>>>(p);
 }
 
-template <typename T, int VEC, int NV>
+template <typename T, int VEC, int NV, bool EDGE = false>
 void launch_flags(const Plan& q, const Args& p, bool bwd, cudaStream_t st) {
   switch (p.flags) {
-    case 0: launch<T, VEC, NV, 0>(q, p, bwd, st); break;
-    case 1: launch<T, VEC, NV, 1>(q, p, bwd, st); break;
-    case 2: launch<T, VEC, NV, 2>(q, p, bwd, st); break;
-    case 3: launch<T, VEC, NV, 3>(q, p, bwd, st); break;
-    case 4: launch<T, VEC, NV, 4>(q, p, bwd, st); break;
-    case 5: launch<T, VEC, NV, 5>(q, p, bwd, st); break;
-    case 6: launch<T, VEC, NV, 6>(q, p, bwd, st); break;
-    default: launch<T, VEC, NV, 7>(q, p, bwd, st); break;
+    case 0: launch<T, VEC, NV, EDGE, 0>(q, p, bwd, st); break;
+    case 1: launch<T, VEC, NV, EDGE, 1>(q, p, bwd, st); break;
+    case 2: launch<T, VEC, NV, EDGE, 2>(q, p, bwd, st); break;
+    case 3: launch<T, VEC, NV, EDGE, 3>(q, p, bwd, st); break;
+    case 4: launch<T, VEC, NV, EDGE, 4>(q, p, bwd, st); break;
+    case 5: launch<T, VEC, NV, EDGE, 5>(q, p, bwd, st); break;
+    case 6: launch<T, VEC, NV, EDGE, 6>(q, p, bwd, st); break;
+    default: launch<T, VEC, NV, EDGE, 7>(q, p, bwd, st); break;
   }
 }
 
 template <typename T>
 int dispatch(const Plan& q, const Args& p, bool bwd, cudaStream_t st) {
   constexpr int kWide = 16 / sizeof(T);
-  if (q.vec == kWide) {
+  if (q.edge) {
+    if (q.nv == 1) launch_flags<T, kWide, 1, true>(q, p, bwd, st);
+    else if (q.nv == 2) launch_flags<T, kWide, 2, true>(q, p, bwd, st);
+    else if constexpr (sizeof(T) == 4) launch_flags<T, kWide, 4, true>(q, p, bwd, st);
+  } else if (q.vec == kWide) {
     if (q.nv == 1) launch_flags<T, kWide, 1>(q, p, bwd, st);
     else if (q.nv == 2) launch_flags<T, kWide, 2>(q, p, bwd, st);
     else if constexpr (sizeof(T) == 4) launch_flags<T, kWide, 4>(q, p, bwd, st);
