@@ -465,15 +465,16 @@ Plan make_plan(Args& p, int elem, const void* const* ptrs, int nptr, int blocks_
   const bool wide = q.vec * elem == 16;
   const int most = wide ? 16 / q.vec : q.vec == 2 ? 4 : 8;            // vectors of a lane
   const int least = wide ? 1 : q.vec == 1 && nvec > 128 ? 8 : 4;
-  q.threads = 256;
   if (nvec <= 32 * most) {
     p.tl = 1;
     while (p.tl < 32 && p.tl * least < nvec) p.tl <<= 1;
     q.nv = (nvec + p.tl - 1) / p.tl;
     q.nv = !wide ? least : q.nv > 2 ? 4 : q.nv;
-    const int teams = q.threads / p.tl;
-    p.gpc = teams < p.groups ? teams : p.groups;
+    // Blocks of equal shares of a row's groups, and no more threads than those shares have lanes.
+    const int teams = 256 / p.tl, cuts = (p.groups + teams - 1) / teams;
+    p.gpc = (p.groups + cuts - 1) / cuts;
     p.rpi = teams / p.gpc;
+    q.threads = (p.gpc * p.rpi * p.tl + 31) / 32 * 32;
   } else {
     p.tl = 0;
     p.gpc = p.rpi = 1;
@@ -486,7 +487,7 @@ Plan make_plan(Args& p, int elem, const void* const* ptrs, int nptr, int blocks_
   // As many threads as blocks_per_sm blocks of 256 an SM; no more rows of blocks than that has
   // blocks (the workspace of the backward pass).
   const long long full = (long long)sm_count() * blocks_per_sm;
-  long long want = full * 256 / q.threads / gx;
+  long long want = (long long)sm_count() * (blocks_per_sm * 256 / q.threads) / gx;
   want = want < 1 ? 1 : want > full ? full : want;
   const long long gy = need < want ? need : want;
   q.grid = dim3(gx, (unsigned)(gy < 1 ? 1 : gy));
