@@ -46,7 +46,7 @@ def _check_bwd(x, r, i, decay, h0, dy, df, out, dtype, what=""):
 SHAPES = [
     (1, 1, 1), (2, 1, 64), (64, 1, 200), (3, 2, 66), (1, 7, 63), (2, 33, 65), (2, 63, 128), (2, 64, 128), (1, 65, 130),
     (3, 127, 72), (2, 200, 321), (1, 513, 64), (1, 1030, 96), (2, 2047, 40), (1, 4097, 2), (70, 130, 64), (1, 700, 2050),
-    (70000, 1, 8), (16, 321, 2048), (300, 47, 130), (300, 49, 130), (2, 4, 70), (2, 14, 70), (2, 15, 70),
+    (70000, 1, 8), (16, 321, 2048), (300, 47, 130), (300, 49, 130), (2, 4, 70), (2, 14, 70), (2, 15, 70), (1, 4200, 64), (2, 2500, 72),
 ]
 
 

@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(kDirectThreads) scan_direct(const Args p) {
 // B16 T8192 D2048 bf16 takes 389 us, 5.5 TB/s (0.84 of a copy): between HBM, the special-function
 // unit (63 % busy, four operations an element) and the latencies of 12 warps an SM.
 //
-// Where there are too few channels to fill the GPU, a cluster of up to 8 blocks shares a
+// Where there are too few channels to fill the GPU, a cluster of up to 16 blocks shares a
 // sequence: block k takes tiles k, k + n, ... . Each round the blocks send their tiles' maps to
 // one another's shared memory, counted in by an mbarrier, so the chain along time costs one
 // such exchange for n tiles, and x, r, i are still read once.
@@ -376,12 +376,13 @@ __device__ __forceinline__ float2 apply(float4 m, float2 h) {
 // round j, which a block sends before it reads round j - 1: 4 rounds are in use.
 template <int DEPTH>
 struct Exchange {
-  float4 (*slots)[8][32];
+  float4* slots;  // [DEPTH][nblk][32], behind the stages
   uint64_t* bar;
   int nblk, rank;
   bool ok;
-  __device__ __forceinline__ Exchange(float4 (*s)[8][32], uint64_t* b, int n, int r)
-      : slots(s), bar(b), nblk(n), rank(r), ok(true) {
+  static constexpr int bytes(int n) { return n > 1 ? DEPTH * n * 32 * (int)sizeof(float4) : 0; }
+  __device__ __forceinline__ Exchange(void* s, uint64_t* b, int n, int r)
+      : slots(static_cast<float4*>(s)), bar(b), nblk(n), rank(r), ok(true) {
     if (nblk > 1) {
       if (threadIdx.x == 0) {
         for (int k = 0; k < DEPTH; ++k) mbar_init(&bar[k], 1);
@@ -394,7 +395,7 @@ struct Exchange {
   __device__ __forceinline__ void send(int j, float4 m) {
     const int lane = threadIdx.x & 31, par = j % DEPTH;
     if (lane == 0) mbar_arrive_expect_tx(&bar[par], nblk * 32 * (int)sizeof(float4));
-    const uint32_t slot = smem_u32(&slots[par][rank][lane]), b = smem_u32(&bar[par]);
+    const uint32_t slot = smem_u32(slots + (par * nblk + rank) * 32 + lane), b = smem_u32(&bar[par]);
     for (int k = 0; k < nblk; ++k) {
       uint32_t rs, rb;
       asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(rs) : "r"(slot), "r"(k));
@@ -413,7 +414,7 @@ struct Exchange {
     float2 mine = carry;
     for (int k = 0; k < nblk; ++k) {
       if (k == rank) mine = carry;
-      carry = apply(slots[par][k][lane], carry);
+      carry = apply(slots[(par * nblk + k) * 32 + lane], carry);
     }
     return mine;
   }
@@ -496,6 +497,7 @@ template <typename T, bool CHAIN>
 struct Fwd {
   static constexpr int kStages = 2, kPerSm = sizeof(T) == 2 && !CHAIN ? 3 : 2;
   static constexpr bool kBehind = CHAIN && sizeof(T) == 2;  // a tile is finished a round behind
+  static constexpr int kDepth = kBehind ? 4 : 2;
   using R = Ring<T, 3, kStages>;
 };
 template <typename T>
@@ -511,10 +513,9 @@ template <typename T, bool TMA, bool CHAIN>
 __global__ void __launch_bounds__(32 * kWarps, Fwd<T, CHAIN>::kPerSm)
     scan_tiles(const __grid_constant__ Args p, const __grid_constant__ Maps tm) {
   constexpr bool BEHIND = Fwd<T, CHAIN>::kBehind;
-  constexpr int NS = Fwd<T, CHAIN>::kStages, NM = BEHIND ? 3 : 2, DEPTH = BEHIND ? 4 : 2;
+  constexpr int NS = Fwd<T, CHAIN>::kStages, NM = BEHIND ? 3 : 2, DEPTH = Fwd<T, CHAIN>::kDepth;
   extern __shared__ __align__(128) uint8_t stages[];
   __shared__ __align__(16) float4 maps[NM][kWarps][32];
-  __shared__ __align__(16) float4 slots[CHAIN ? DEPTH : 1][8][32];
   __shared__ __align__(8) uint64_t full[NS], xbar[DEPTH];
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int nblk = CHAIN ? cluster_size() : 1, rank = CHAIN ? cluster_rank() : 0;
@@ -528,7 +529,7 @@ __global__ void __launch_bounds__(32 * kWarps, Fwd<T, CHAIN>::kPerSm)
     return;
   }
   typename Fwd<T, CHAIN>::R ring(stages, full);
-  Exchange<DEPTH> ex(slots, xbar, nblk, rank);
+  Exchange<DEPTH> ex(stages + Fwd<T, CHAIN>::R::kBytes, xbar, nblk, rank);
   const Seq q = sequence(p, n);
   y += (q.batch * p.T + q.lo) * p.D;
   const float2 ndecay = neg_decay(ln, p.decay);
@@ -678,7 +679,6 @@ __global__ void __launch_bounds__(32 * kWarps, Bwd<T>::kPerSm)
   extern __shared__ __align__(128) uint8_t stages[];
   __shared__ __align__(16) float4 maps[2][kWarps][32];
   __shared__ __align__(16) float2 back[2][kWarps][32];
-  __shared__ __align__(16) float4 slots[2][8][32];
   __shared__ __align__(8) uint64_t full[Bwd<T>::kStages], xbar[2];
   constexpr int NS = Bwd<T>::kStages;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -697,7 +697,7 @@ __global__ void __launch_bounds__(32 * kWarps, Bwd<T>::kPerSm)
     return;
   }
   typename Bwd<T>::R ring(stages, full);
-  Exchange<2> ex(slots, xbar, nblk, rank);
+  Exchange<2> ex(stages + Bwd<T>::R::kBytes, xbar, nblk, rank);
   const Seq q = sequence(p, n);
   const long long first = (q.batch * p.T + q.lo) * p.D;
   const float2 ndecay = neg_decay(ln, p.decay);
@@ -902,20 +902,26 @@ int direct_tokens(int count) {
 // a few pieces one may have nearly all, and more blocks than needed cost little (65537 rows in 5
 // pieces backward: 902 us alone, 622, 506 and 517 with two, four, eight; other cuts with four up
 // to 618; 20011 rows in 37 pieces forward fp32: 80, 86, 111, 164).
-int cluster_blocks(double chains, double tokens, int slots) {
+//
+// Sixteen, more than every GPU has to allow, only forward in bf16, where two such blocks still fit an
+// SM, and for a dozen chains at most, which find room beside each other (T44352 D272, 5 chains: 155
+// us with eight, 95 with sixteen; T32768 D1024, 16 chains: 136 and 140; backward T32768 D512: 189
+// and 208).
+int cluster_blocks(double chains, double tokens, int slots, bool wide) {
   int n = 1;
   while (n < 8 && chains * n * 2 <= slots && tokens / kChunk >= 4 * n) n *= 2;
+  if (wide && n == 8 && chains * 16 * 3 <= slots * 2 && tokens / kChunk >= 32) n = 16;
   return n;
 }
-int packed_blocks(int T, int cols, int nseq, int slots) {
+int packed_blocks(int T, int cols, int nseq, int slots, bool wide) {
   const double longest = nseq <= 8 ? 1. : (1. + std::log((double)nseq)) / nseq;
-  return cluster_blocks(cols / longest, T * longest, slots);
+  return cluster_blocks(cols / longest, T * longest, slots, wide);
 }
 
 int bwd_cluster(int T, int D, int nseq, bool packed, int dtype) {
   const int slots = sm_count() * (dtype == THM_BF16 ? Bwd<__nv_bfloat16>::kPerSm : Bwd<float>::kPerSm);
   const int cols = (D + kCols - 1) / kCols;
-  return packed ? packed_blocks(T, cols, nseq, slots) : cluster_blocks((double)nseq * cols, T, slots);
+  return packed ? packed_blocks(T, cols, nseq, slots, false) : cluster_blocks((double)nseq * cols, T, slots, false);
 }
 
 // `count` sequences of channels from `first` on, n blocks each.
@@ -924,6 +930,10 @@ int launch_tiles(K kernel, Args p, const Maps& tm, int n, int first, int count, 
   p.first = first;
   p.count = count;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+    cudaGetLastError();
+    return THM_ERR_CUDA;
+  }
+  if (n > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
     cudaGetLastError();
     return THM_ERR_CUDA;
   }
@@ -963,9 +973,9 @@ int run_fwd(Args p, int B, int seqs, int dtype, cudaStream_t st) {
   tma = tma && encode(&tm.in[0], dtype, p.x, p.xb, p.xt, B, p.T, p.D) == THM_OK &&
         encode(&tm.in[1], dtype, p.r, p.rb, p.rt, B, p.T, p.D) == THM_OK &&
         encode(&tm.in[2], dtype, p.i, p.ib, p.it, B, p.T, p.D) == THM_OK;
-  constexpr int smem = Fwd<T, false>::R::kBytes;
-  static_assert(smem == Fwd<T, true>::R::kBytes);
+  static_assert(Fwd<T, false>::R::kBytes == Fwd<T, true>::R::kBytes);
   auto run = [&](int n, int first, int cnt) {
+    const int smem = Fwd<T, true>::R::kBytes + Exchange<Fwd<T, true>::kDepth>::bytes(n);
     if (n > 1)
       return tma ? launch_tiles(scan_tiles<T, true, true>, p, tm, n, first, cnt, smem, st)
                  : launch_tiles(scan_tiles<T, false, true>, p, tm, n, first, cnt, smem, st);
@@ -978,13 +988,14 @@ int run_fwd(Args p, int B, int seqs, int dtype, cudaStream_t st) {
   // launch of its own (B16 T8192 D2048 bf16, 68 of 512 left over: 446 us in one launch, 424 in two).
   const int rest = count % slots;
   if (p.cu == nullptr && count > slots && rest > 0) {
-    const int n = cluster_blocks(rest, p.T, chain_slots);
+    const int n = cluster_blocks(rest, p.T, chain_slots, sizeof(T) == 2);
     if (n > 1) {
       const int e = run(1, 0, count - rest);
       return e != THM_OK ? e : run(n, count - rest, rest);
     }
   }
-  return run(p.cu == nullptr ? cluster_blocks(count, p.T, chain_slots) : packed_blocks(p.T, p.cols, p.nseq, chain_slots), 0,
+  return run(p.cu == nullptr ? cluster_blocks(count, p.T, chain_slots, sizeof(T) == 2)
+                               : packed_blocks(p.T, p.cols, p.nseq, chain_slots, sizeof(T) == 2), 0,
              count);
 }
 
@@ -999,7 +1010,7 @@ int run_bwd(const Args& p, int B, int seqs, int dtype, int n, cudaStream_t st) {
         encode(&tm.in[1], dtype, p.r, p.rb, p.rt, B, p.T, p.D) == THM_OK &&
         encode(&tm.in[2], dtype, p.i, p.ib, p.it, B, p.T, p.D) == THM_OK &&
         encode(&tm.in[3], dtype, p.dy, p.gb, p.gt, B, p.T, p.D) == THM_OK;
-  const int smem = Bwd<T>::R::kBytes;
+  const int smem = Bwd<T>::R::kBytes + Exchange<2>::bytes(n);
   return tma ? launch_tiles(scan_bwd_tiles<T, true>, p, tm, n, 0, count, smem, st)
              : launch_tiles(scan_bwd_tiles<T, false>, p, tm, n, 0, count, smem, st);
 }
