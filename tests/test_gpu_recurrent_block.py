@@ -216,6 +216,38 @@ def test_two_streams_at_once():
             assert all(torch.equal(a, b) for a, b in zip(alone[k], g))
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_inputs_are_left_as_they_are(dtype):
+    """No call writes into what it is given, and passes on one state repeat with others in between."""
+    from theorem_b200 import ops
+    B, T, D = 2, 200, 72
+    g = torch.Generator(DEV).manual_seed(0)
+    rn = lambda *s, dt=dtype: torch.randn(*s, generator=g, device=DEV, dtype=dt)  # noqa: E731
+
+    def make():
+        f = torch.float32
+        return dict(x=rn(B, T, D), r=rn(B, T, D), i=rn(B, T, D), dy=rn(B, T, D), h0=rn(B, D, dt=f), df=rn(B, D, dt=f),
+                    decay=rn(D, dt=f).abs(), w=rn(D, dt=f), b=rn(D, dt=f), cw=rn(D, 4, dt=f), st=rn(B, 3, D))
+
+    def run(s):
+        y, fin, states = ops.gated_scan(s["x"], s["r"], s["i"], s["decay"], h0=s["h0"], want_states=True)
+        kw = dict(gate=s["r"], activation="silu")
+        return [y, fin, states,
+                *ops.gated_scan_bwd(s["x"], s["r"], s["i"], s["decay"], states, s["dy"], dfinal=s["df"]),
+                ops.group_norm(s["x"], 24, s["w"], s["b"], **kw),
+                *ops.group_norm_bwd(s["x"], s["dy"], 24, s["w"], s["b"], **kw),
+                *ops.causal_conv1d_step(s["x"][:, :8], s["st"], s["cw"], s["b"], activation="silu"),
+                *ops.causal_conv1d_bwd(s["x"], s["cw"], s["b"], s["dy"], activation="silu")]
+
+    one, two = make(), make()
+    before = {k: v.clone() for k, v in one.items()}
+    first = run(one)
+    run(two)
+    again = run(one)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    assert all(torch.equal(one[k], v) for k, v in before.items())
+
+
 def test_arguments_by_name():
     from theorem_b200 import ops
     x = torch.randn(2, 40, 64, device=DEV)
